@@ -62,7 +62,8 @@ typedef enum welm_rope_status {
 #define WELM_ROPE_DEV_BAD_TILE 4       /* tile start/end outside [0, N], or > 64 tokens */
 #define WELM_ROPE_DEV_BAD_LENGTH 8     /* negative request length (tile builder)        */
 #define WELM_ROPE_DEV_BAD_SLOT 16      /* slot_mapping[t] >= num_slots (KV-cache write) */
-#define WELM_ROPE_DEV_WAIT_TIMEOUT 32  /* a bounded barrier wait gave up (TMA ceiling)   */
+#define WELM_ROPE_DEV_WAIT_TIMEOUT 32  /* a bounded barrier wait gave up (TMA ceiling, attention) */
+#define WELM_ROPE_DEV_BAD_PAGE 64      /* a block table names a block outside the cache */
 
 /* Fixed model contract (bench_welmv4_inplace_rope_npu.py:48-58): head_dim 256, rope_dim 64, 6 Q heads,
  * 1 K head, 64-token work tiles. */
@@ -329,6 +330,124 @@ int welm_rope_ceiling_tma_slices(void* q, void* k, int64_t n_tokens, int64_t q_t
                                  int64_t k_token_stride, int32_t ctas, int32_t stages, int32_t* device_status,
                                  void* stream);
 
+/*
+ * Rotary embedding with one position per axis (time, height, width, ...).
+ * Pair i (lanes 192 + i and 224 + i, i < 32) of every head belongs to one axis
+ * a(i) and is rotated by cos_sin_cache[positions[a(i)][t]][i] (cos) and
+ * [32 + i] (sin), with the arithmetic and roundings given above.  `sections`
+ * (HOST memory, num_axes entries, at most WELM_ROPE_MAX_AXES) holds the pairs
+ * of each axis, 32 in all: interleaved == 0 gives axis 0 the first
+ * sections[0] pairs, axis 1 the next, and so on; interleaved == 1 deals the
+ * pairs out in turn over the axes that still have some left.  sections = {32}
+ * is the ordinary embedding.  inverse == 1 negates the sines: the inverse
+ * rotation, which also takes the gradient of the outputs to the gradient of
+ * the inputs.
+ *
+ * q [n_tokens, num_q_heads, 256] and k [n_tokens, num_k_heads, 256] have token
+ * and head strides of their own (either count may be 0, then its pointers may
+ * be NULL).  q_out == q and k_out == k (with equal strides) rotates in place
+ * and moves only the rotated lanes; otherwise whole heads are copied.  The
+ * outputs' rows must be apart from one another and, unless in place, from the
+ * inputs; input strides may be 0.  positions is [num_axes][n_tokens] with rows
+ * position_stride apart; an axis of no pairs is not read.  A token with a
+ * position outside [0, max_position) on a used axis is left (or copied)
+ * unrotated and raises WELM_ROPE_DEV_BAD_POSITION.  Pointers to heads and the
+ * cache must be 16-byte aligned and strides multiples of 8 elements
+ * (WELM_ROPE_ERR_BAD_STRIDE otherwise).
+ */
+#define WELM_ROPE_MAX_AXES 4
+int welm_rope_multi_axis(const void* q, void* q_out, const void* k, void* k_out,
+                         const int64_t* positions, const float* cos_sin_cache,
+                         const int32_t* sections, int64_t num_axes, int64_t interleaved,
+                         int64_t inverse, int64_t n_tokens, int64_t num_q_heads,
+                         int64_t num_k_heads, int64_t q_token_stride, int64_t q_head_stride,
+                         int64_t q_out_token_stride, int64_t q_out_head_stride,
+                         int64_t k_token_stride, int64_t k_head_stride,
+                         int64_t k_out_token_stride, int64_t k_out_head_stride,
+                         int64_t position_stride, int64_t max_position,
+                         int32_t* device_status, void* stream);
+
+/*
+ * Ordinary prefill / decode fused with the append to a paged KV cache:
+ *   q[t]                 = rope(q[t])  in place, rotated lanes only
+ *   key_cache[slot[t]]   = rope(k[t])  all 256 lanes of every KV head
+ *   value_cache[slot[t]] = v[t]
+ * with slot = slot_mapping[t], block slot / block_size, place slot %
+ * block_size.  k and v are read only.  A token with a negative slot is
+ * padding and is left alone altogether, its q too; slot >= num_blocks *
+ * block_size raises WELM_ROPE_DEV_BAD_SLOT and a position outside the cos/sin
+ * cache WELM_ROPE_DEV_BAD_POSITION, and the token is left alone.  Two tokens of
+ * one call must not name the same slot: which of them it then holds, lane by
+ * lane, is open.  positions, sections, num_axes and interleaved as for
+ * welm_rope_multi_axis (num_axes 1, sections {32}: one position per token).
+ * num_q_heads may be 0.  The caches are [num_blocks, block_size, num_k_heads,
+ * 256]; key_cache_strides and value_cache_strides (HOST memory) give the
+ * elements between blocks, between slots of a block and between heads, so a
+ * [num_blocks, num_k_heads, block_size, 256] cache is the same call with its
+ * strides in that order.  Pointers must be 16-byte aligned and strides
+ * multiples of 8 elements.
+ */
+int welm_rope_kv_append(void* q, const void* k, const void* v, const int64_t* positions,
+                        const float* cos_sin_cache, const int32_t* sections, int64_t num_axes,
+                        int64_t interleaved, const int64_t* slot_mapping, void* key_cache,
+                        void* value_cache, int64_t n_tokens, int64_t num_q_heads,
+                        int64_t num_k_heads, int64_t q_token_stride, int64_t q_head_stride,
+                        int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
+                        int64_t v_head_stride, int64_t num_blocks, int64_t block_size,
+                        const int64_t* key_cache_strides, const int64_t* value_cache_strides,
+                        int64_t position_stride, int64_t max_position, int32_t* device_status,
+                        void* stream);
+
+/*
+ * Attention over a paged KV cache for a batch whose requests share a prefix:
+ *   out[t, h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * q[t, h] . k_j)
+ * over the prefix's keys and the request's own keys; query head h reads KV
+ * head h / (num_q_heads / num_k_heads).  Prefix key j < prefix_len lies in
+ * block prefix_table[j / block_size] at place j % block_size, and is read once
+ * for the whole batch; own key j < seq_lens[b] of request b in block
+ * block_table[b * table_stride + j / block_size].  Request b's query tokens are
+ * rows query_starts[b] .. query_starts[b + 1] of q, n of them, at its last n
+ * own keys: token i sees the prefix and its own keys 0 .. seq_lens[b] - n + i.
+ * query_starts == NULL gives every request one token (n_tokens == batch_size).
+ * A row that sees no key becomes zeros, its lse minus infinity.  lse (may be
+ * NULL, [n_tokens, num_q_heads] FP32) receives log sum_j p_j.  Rows of no
+ * request are left as they were (fill_unused == 0), or become such rows too
+ * (fill_unused == 1).
+ *
+ * The tables, lengths and starts are read on the device, so a captured launch
+ * follows their contents.  A length below 0 or above table_width * block_size,
+ * and starts that decrease or leave [0, n_tokens], are clamped and raise
+ * WELM_ROPE_DEV_BAD_LENGTH; a block outside [0, num_blocks) reads as zeros
+ * (keys and values) and raises WELM_ROPE_DEV_BAD_PAGE.  What a page holds
+ * behind the last key does not matter, no numbers included; a key that some
+ * rows of a request's tile do not see yet must be finite.
+ *
+ * Products take BF16 operands (p rounded to BF16) with FP32 sums; maxima, sums
+ * and partial results are FP32; out is rounded once.  Results do not depend on
+ * timing.  scale must be positive and finite (WELM_ROPE_ERR_BAD_MODE).
+ * block_size must be a multiple of 8.  The caches' strides as for
+ * welm_rope_kv_append; q may repeat rows (stride 0), out may not, and out must
+ * not overlap q.  Pointers must be 16-byte aligned, strides multiples of 8.
+ *
+ * The call allocates nothing: `workspace` is device memory of at least the
+ * bytes that welm_rope_attend_workspace gives for the same sizes on the current
+ * device.  It needs no initial contents and keeps nothing for the next call,
+ * but belongs to one call at a time: calls that may overlap on the GPU, replays
+ * of two captured graphs among them, need a workspace each.
+ */
+int welm_rope_attend_workspace(int64_t n_tokens, int64_t batch_size, int64_t num_q_heads,
+                               int64_t num_k_heads, int64_t prefix_len, int64_t* bytes);
+int welm_rope_attend(const void* q, void* out, float* lse, const void* key_cache,
+                     const void* value_cache, const int32_t* block_table,
+                     const int64_t* seq_lens, const int64_t* query_starts,
+                     const int32_t* prefix_table, int64_t prefix_len, int64_t n_tokens,
+                     int64_t batch_size, int64_t num_q_heads, int64_t num_k_heads,
+                     int64_t q_token_stride, int64_t q_head_stride, int64_t out_token_stride,
+                     int64_t out_head_stride, int64_t table_width, int64_t table_stride,
+                     int64_t num_blocks, int64_t block_size, const int64_t* key_cache_strides,
+                     const int64_t* value_cache_strides, float scale, int64_t fill_unused,
+                     void* workspace, int64_t workspace_bytes, int32_t* device_status, void* stream);
+
 /* Human-readable name of a welm_rope_status code (static storage). */
 const char* welm_rope_status_string(int status);
 
@@ -337,8 +456,10 @@ const char* welm_rope_status_string(int status);
  * 1.1 added welm_rope_ordinary_mapped and WELM_ROPE_ERR_NOT_MAPPED; 1.2 the
  * two measurement kernels welm_rope_ceiling_copy and welm_rope_ceiling_slices;
  * 1.3 the measurement kernel welm_rope_ceiling_gather; 1.4 the measurement
- * kernel welm_rope_ceiling_tma_slices and WELM_ROPE_DEV_WAIT_TIMEOUT. */
-#define WELM_ROPE_ABI_VERSION ((1 << 16) | 4)
+ * kernel welm_rope_ceiling_tma_slices and WELM_ROPE_DEV_WAIT_TIMEOUT; 1.5
+ * welm_rope_multi_axis, welm_rope_kv_append, welm_rope_attend,
+ * welm_rope_attend_workspace and WELM_ROPE_DEV_BAD_PAGE. */
+#define WELM_ROPE_ABI_VERSION ((1 << 16) | 5)
 int welm_rope_abi_version(void);
 
 #ifdef __cplusplus

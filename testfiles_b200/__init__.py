@@ -24,6 +24,13 @@ from .ops import (  # noqa: F401
     welmv4_inplace_rope,
     welmv4_inplace_rope_npu,
 )
+from .paged import (  # noqa: F401,E402
+    attend_shared_prefix,
+    attend_workspace_bytes,
+    rope_kv_append,
+    rope_multi_axis,
+    rope_multi_axis_inplace,
+)
 from .host import welmv4_inplace_rope_host  # noqa: F401,E402
 from .harness import Harness, providers_for_case  # noqa: F401,E402
 

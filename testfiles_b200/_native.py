@@ -25,6 +25,7 @@ ERR_TOO_MANY_TOKENS = 7
 ERR_NOT_MAPPED = 8
 STATIC_MAX_TOKENS = 2048
 LENS_MAX_BATCH = 2048
+MAX_AXES = 4
 
 # Device status bits.
 DEV_BAD_POSITION = 1
@@ -33,9 +34,11 @@ DEV_BAD_TILE = 4
 DEV_BAD_LENGTH = 8
 DEV_BAD_SLOT = 16
 DEV_WAIT_TIMEOUT = 32
+DEV_BAD_PAGE = 64
 
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
+_F32 = ctypes.c_float
 
 # name -> (restype, argtypes); every symbol declared in include/welm_rope.h.
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
@@ -53,6 +56,11 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "welm_rope_ceiling_gather": (ctypes.c_int, [_P, _P, _I64, _I64, _P, _P]),
     "welm_rope_ceiling_tma_slices": (ctypes.c_int, [_P, _P, _I64, _I64, _I64, ctypes.c_int32, ctypes.c_int32, _P,
                                                     _P]),
+    "welm_rope_multi_axis": (ctypes.c_int, [_P] * 7 + [_I64] * 16 + [_P, _P]),
+    "welm_rope_kv_append": (ctypes.c_int, [_P] * 6 + [_I64] * 2 + [_P] * 3 + [_I64] * 11 + [_P] * 2 + [_I64] * 2 +
+                            [_P, _P]),
+    "welm_rope_attend_workspace": (ctypes.c_int, [_I64] * 5 + [_P]),
+    "welm_rope_attend": (ctypes.c_int, [_P] * 9 + [_I64] * 13 + [_P] * 2 + [_F32, _I64, _P, _I64, _P, _P]),
     "welm_rope_count_tiles_host": (ctypes.c_int, [_P, _I64, _P]),
     "welm_rope_build_tiles_host": (ctypes.c_int, [_P, _I64, _P, _I64, _P, _P]),
     "welm_rope_status_string": (ctypes.c_char_p, [ctypes.c_int]),

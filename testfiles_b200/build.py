@@ -21,8 +21,9 @@ CSRC = PACKAGE_DIR / "csrc"
 # one translation unit per kernel family; the .cuh headers hold what they share
 SOURCES = tuple(CSRC / name for name in (
     "rope_ordinary.cu", "rope_mirror.cu", "rope_kv_write.cu", "rope_tiles.cu", "rope_host_memory.cu",
-    "rope_ceiling.cu", "rope_abi.cu"))
-HEADERS = (REPO_ROOT / "include" / "welm_rope.h", CSRC / "rope_device.cuh", CSRC / "rope_host.cuh")
+    "rope_ceiling.cu", "rope_multi_axis.cu", "rope_kv_append.cu", "rope_attend.cu", "rope_abi.cu"))
+HEADERS = (REPO_ROOT / "include" / "welm_rope.h", *(CSRC / name for name in (
+    "rope_device.cuh", "rope_host.cuh", "rope_axes.cuh", "rope_tma.cuh")))
 LIBRARY = PACKAGE_DIR / "libwelm_rope_b200.so"
 
 NVCC_FLAGS = (

@@ -1,0 +1,1088 @@
+// rope_attend.cu — attention of a batch over a paged KV cache whose requests
+// share a prefix, and its C entries welm_rope_attend and
+// welm_rope_attend_workspace.
+//
+// Query row (token t, head): o = sum_j p_j v_j / sum_j p_j with p_j =
+// exp(scale q.k_j - max) over the prefix's keys and the request's own keys up
+// to the token's position.  Both parts are exact softmax partial results (m,
+// l, O) with m the maximum, l = sum p and O = sum p v; two of them join as
+//     m = max(m1, m2), l = l1 2^(m1 - m) + l2 2^(m2 - m), O likewise.
+//
+// Work.  An item is 128 query rows (tokens x the query heads of one KV head)
+// against a run of keys.  The prefix's items take their rows from all requests
+// together, so a prefix key is read once for every 128 rows instead of once
+// for every request; a request's own items hold its own rows.  All items'
+// 64-key tiles form one line, cut into equal runs, one for each CTA; a CTA
+// walks the pieces of items in its run.  An item that is cut, or whose rows
+// also have the other part, leaves FP32 partial results in the workspace, and
+// a second kernel joins them row by row in the order of the keys, so results
+// do not depend on timing.  Lengths stay on the device: every CTA adds the
+// requests' tiles up for itself, and a captured launch follows new lengths.
+//
+// One CTA on an SM, eight warps:
+//   0     TMA producer: K and V tiles (64 keys, 32 KB each) into a ring of five
+//   1     issues tcgen05.mma: S = Q K^T (128 x 64) and O += P V (128 x 256)
+//   2     brings the piece's Q rows into shared memory (64 KB)
+//   3     lists the CTA's pieces
+//   4..7  softmax, one row a thread; rescaling of O; the results
+// S, P (BF16) and O live in TMEM (S and P twice, so that the softmax of one
+// tile runs beside the products of its neighbours).  P is rounded to BF16
+// because the product with the BF16 values takes both operands in one type;
+// l sums the unrounded p, and S, m, l and O are FP32.
+
+#include "rope_tma.cuh"
+
+namespace {
+
+constexpr int kRows = 128;             // query rows of an item
+constexpr int kKeys = 64;              // keys of a tile
+constexpr int kStages = 5;             // ring of K and V tiles
+constexpr int kStageBytes = kKeys * kHeadDim * 2;
+constexpr int kQChunkBytes = kRows * 128;  // 64 lanes of 128 rows
+constexpr int kQBytes = kRows * kHeadDim * 2;
+constexpr int kPieces = 4;             // ring of piece descriptors
+constexpr int kThreads = 256;
+constexpr int kSoftmaxWarp0 = 4;
+constexpr int kPieceReaders = 3 + 4;   // producer, issuer, Q warp, four softmax warps
+constexpr uint32_t kColS = 0, kColP = 128, kColO = 256;  // TMEM columns
+constexpr long long kWaitClocks = 1ll << 32;  // about two seconds
+constexpr float kRescaleStep = 8.0f;   // O is rescaled when the maximum grows by more than 2^8
+
+struct AttendArgs {
+  const uint16_t* q;
+  uint16_t* out;
+  float* lse;  // may be null
+  int64_t q_token, q_head, out_token, out_head;
+  const int32_t* prefix_table;
+  const int32_t* block_table;
+  int64_t table_stride;
+  const int64_t* seq_lens;
+  const int64_t* query_starts;  // may be null: one token a request
+  int32_t tokens, batch, q_heads, k_heads, group;
+  int32_t prefix_len, max_len;  // max_len: keys that a row of block_table can name
+  int32_t block_size, num_blocks;
+  int32_t slot_rows;            // rows of a workspace slot
+  int32_t grid;
+  int32_t fill;                 // 1: rows of no request become zeros
+  float scale;                  // times log2(e)
+  int64_t* units_before;        // [batch + 1] tiles of the items before each request
+  float* slot_ml;               // [2 grid][slot_rows][2]
+  float* slot_o;                // [2 grid][slot_rows][256]
+  float* part_ml;               // [2][tokens * q_heads][2]: whole items' rows, prefix and own
+  float* part_o;                // [2][tokens * q_heads][256]
+  int32_t* status;
+};
+
+__device__ __forceinline__ int div_up(int a, int b) { return (a + b - 1) / b; }
+__device__ __forceinline__ int64_t clamp64(int64_t v, int64_t lo, int64_t hi) {
+  return v < lo ? lo : v > hi ? hi : v;
+}
+
+// One request's own part: `count` query tokens from token `first`, the last of
+// them at the last of `len` keys.
+struct Request {
+  int first, count, len;
+  __device__ __forceinline__ int row_tiles(int group) const { return div_up(count * group, kRows); }
+  // Keys that the last row of row tile rt sees: every row of it sees at most these.
+  __device__ __forceinline__ int seen(int group, int rt) const {
+    int last = (rt * kRows + kRows - 1) / group;
+    if (last > count - 1) last = count - 1;
+    const int keys = len - count + last + 1;
+    return keys < 0 ? 0 : keys;
+  }
+  __device__ __forceinline__ int tiles(int group, int rt) const { return div_up(seen(group, rt), kKeys); }
+};
+
+__device__ __forceinline__ Request load_request(const AttendArgs& a, int b, bool tell) {
+  Request r;
+  int64_t lo = b, hi = b + 1;
+  bool good = true;
+  if (a.query_starts != nullptr) {
+    const int64_t s0 = __ldg(a.query_starts + b), s1 = __ldg(a.query_starts + b + 1);
+    lo = clamp64(s0, 0, a.tokens);
+    hi = clamp64(s1, lo, a.tokens);
+    good = lo == s0 && hi == s1;
+  }
+  const int64_t n = __ldg(a.seq_lens + b);
+  r.first = int(lo);
+  r.count = int(hi - lo);
+  r.len = int(clamp64(n, 0, a.max_len));
+  if (tell && !(good && r.len == n)) raise_status(a.status, WELM_ROPE_DEV_BAD_LENGTH);
+  return r;
+}
+
+// Query tokens in use: those behind the last request are left alone.
+__device__ __forceinline__ int used_tokens(const AttendArgs& a) {
+  return a.query_starts != nullptr ? int(clamp64(__ldg(a.query_starts + a.batch), 0, a.tokens)) : a.tokens;
+}
+
+// The line of tiles, cut into `grid` runs: CTA c has [begin(c), begin(c + 1)).
+// No run is empty: a line of fewer tiles than CTAs keeps only as many busy.
+struct Line {
+  int64_t units;
+  int grid;
+  __device__ __forceinline__ Line(int64_t n, int ctas) : units(n), grid(n < ctas ? int(n) : ctas) {}
+  __device__ __forceinline__ int64_t begin(int c) const { return units * c / grid; }
+  __device__ __forceinline__ int cta_of(int64_t u) const { return int(((u + 1) * grid - 1) / units); }
+};
+
+__device__ __forceinline__ int64_t prefix_units(const AttendArgs& a, int used) {
+  return int64_t(div_up(used * a.group, kRows)) * a.k_heads * div_up(a.prefix_len, kKeys);
+}
+
+enum Destination { kToOutput, kToSlot, kToPart };
+
+// A piece of an item, as the warps of a CTA read it.
+struct Piece {
+  int32_t tiles;       // 0: no more pieces
+  int32_t first_tile;
+  int32_t keys;        // keys that some row of the item sees
+  int32_t head;        // KV head
+  int32_t row0;        // first row, as (token - first) * group + query head in the group
+  int32_t rows;
+  int32_t first;       // token that rows are counted from
+  int32_t seen0;       // keys that token `first` sees; a later token sees one more each, or `keys` in the prefix
+  int32_t own;         // 1: a request's own keys; 0: the prefix
+  int32_t table_row;   // row of block_table
+  int32_t to;          // Destination
+  int32_t slot;
+};
+
+struct Control {
+  uint64_t full[kStages], empty[kStages];
+  uint64_t s_full[2], s_empty[2], p_full[2], pv_done[2];
+  uint64_t q_full, q_empty, o_free, drained;
+  uint64_t piece_full[kPieces], piece_empty[kPieces];
+  Piece piece[kPieces];
+  int64_t scan[kThreads / 32];
+  int64_t start_units;
+  int32_t start_request;
+  uint32_t tmem;
+  int32_t failed;
+};
+
+constexpr int kSmemBytes = 1024 + kQBytes + kStages * kStageBytes + 1024;
+static_assert(sizeof(Control) <= 1024, "control block");
+static_assert(kSmemBytes <= 227 * 1024, "shared memory of one CTA");
+
+// Waits for a phase of `bar`; false once any warp of the CTA has given up.
+__device__ __forceinline__ bool mbar_wait(Control& ctl, uint64_t* bar, uint32_t parity) {
+  if (mbar_poll(bar, parity)) return true;
+  const long long t0 = clock64();
+  while (!mbar_poll(bar, parity)) {
+    if (*reinterpret_cast<volatile int32_t*>(&ctl.failed)) return false;
+    if (clock64() - t0 > kWaitClocks) {
+      *reinterpret_cast<volatile int32_t*>(&ctl.failed) = 1;
+      return false;
+    }
+  }
+  return true;
+}
+
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// ---------------------------------------------------------------------------
+// tcgen05: descriptors, products, TMEM reads and writes.
+// ---------------------------------------------------------------------------
+// Shared-memory operand descriptor, 128-byte swizzle.  K-major (Q and K: lanes
+// are the contraction): `stride` is the step between groups of eight rows.
+// MN-major (V: keys are the contraction): `lead` steps between 64-lane chunks
+// and `stride` between groups of eight keys.
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr, uint32_t lead, uint32_t stride) {
+  return uint64_t((addr & 0x3ffffu) >> 4) | uint64_t(lead >> 4) << 16 | uint64_t(stride >> 4) << 32 |
+         uint64_t(1) << 46 | uint64_t(2) << 61;
+}
+
+// Instruction descriptor: FP32 accumulator, BF16 operands, M = 128.
+__host__ __device__ constexpr uint32_t instr_desc(int n, bool b_mn_major) {
+  return 1u << 4 | 1u << 7 | 1u << 10 | uint32_t(b_mn_major) << 16 | uint32_t(n / 8) << 17 | uint32_t(kRows / 16) << 24;
+}
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+      "r"(uint32_t(add))
+      : "memory");
+}
+
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a), "l"(b), "r"(idesc),
+      "r"(uint32_t(add))
+      : "memory");
+}
+
+// Arrives on `bar` when every product issued so far is done.
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
+
+__device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// 32 columns of the thread's TMEM lane.
+__device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+      "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+      "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
+      "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
+      "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),
+      "r"(r[31]), "r"(addr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_load_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Eight FP32 values to 32 aligned bytes.
+__device__ __forceinline__ void store8f(float* p, const float* v) {
+  asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]),
+               "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
+}
+
+// ---------------------------------------------------------------------------
+// The roles.
+// ---------------------------------------------------------------------------
+// Every warp that walks the pieces: next piece, or false at the end (or when
+// the CTA has given up).  Called by whole warps or by one thread.
+struct PieceReader {
+  int n = 0;
+  template <bool kWarp>
+  __device__ __forceinline__ bool next(Control& ctl, Piece& p) {
+    const int s = n % kPieces;
+    bool ok = mbar_wait(ctl, &ctl.piece_full[s], (n / kPieces) & 1);
+    if (kWarp) ok = __all_sync(0xffffffffu, ok);
+    if (!ok) return false;
+    p = ctl.piece[s];
+    if (kWarp) __syncwarp();
+    if (!kWarp || (threadIdx.x & 31) == 0) mbar_arrive(&ctl.piece_empty[s]);
+    ++n;
+    return p.tiles > 0;
+  }
+};
+
+// Lists the pieces of this CTA's run of tiles.
+__device__ void list_pieces(const AttendArgs& a, Control& ctl, const Line& line, int cta, int used, int64_t pre) {
+  const int lane = threadIdx.x & 31;
+  int n = 0;
+  // every lane holds the piece; lane 0 writes it
+  auto emit = [&](const Piece& p) {
+    const int s = n % kPieces;
+    const bool ok = __all_sync(0xffffffffu, mbar_wait(ctl, &ctl.piece_empty[s], ((n / kPieces) & 1) ^ 1));
+    if (!ok) return false;
+    if (lane == 0) {
+      ctl.piece[s] = p;
+      mbar_arrive(&ctl.piece_full[s]);
+    }
+    ++n;
+    return true;
+  };
+  int64_t u = line.begin(cta);
+  const int64_t end = line.begin(cta + 1);
+  const int key_tiles = div_up(a.prefix_len, kKeys);
+  const int row_tiles = div_up(used * a.group, kRows);
+  while (u < end && u < pre) {
+    const int item = int(u / key_tiles);
+    Piece p;
+    p.first_tile = int(u - int64_t(item) * key_tiles);
+    p.tiles = int(clamp64(end - u, 0, key_tiles - p.first_tile));
+    p.keys = a.prefix_len;
+    p.head = item / row_tiles;
+    p.row0 = (item - p.head * row_tiles) * kRows;
+    p.rows = used * a.group - p.row0 < kRows ? used * a.group - p.row0 : kRows;
+    p.first = 0;
+    p.seen0 = a.prefix_len;
+    p.own = 0;
+    p.table_row = 0;
+    p.to = p.tiles == key_tiles ? kToPart : kToSlot;
+    p.slot = 2 * cta + (p.first_tile > 0 ? 0 : 1);
+    if (!emit(p)) return;
+    u += p.tiles;
+  }
+  int64_t base = ctl.start_units + pre;  // of request `start_request`
+  for (int b0 = ctl.start_request; u < end && b0 < a.batch; b0 += 32) {
+    Request mine{0, 0, 0};
+    if (b0 + lane < a.batch) mine = load_request(a, b0 + lane, false);
+    for (int i = 0; i < 32 && u < end && b0 + i < a.batch; ++i) {
+      const Request r{__shfl_sync(0xffffffffu, mine.first, i), __shfl_sync(0xffffffffu, mine.count, i),
+                      __shfl_sync(0xffffffffu, mine.len, i)};
+      const int rts = r.row_tiles(a.group);
+      for (int rt = 0; rt < rts && u < end; ++rt) {
+        const int t = r.tiles(a.group, rt);
+        for (int h = 0; h < a.k_heads && u < end; ++h, base += t) {
+          if (u >= base + t) continue;
+          Piece p;
+          p.first_tile = int(u - base);
+          p.tiles = int(clamp64(end - u, 0, t - p.first_tile));
+          p.keys = r.seen(a.group, rt);
+          p.head = h;
+          p.row0 = rt * kRows;
+          p.rows = r.count * a.group - p.row0 < kRows ? r.count * a.group - p.row0 : kRows;
+          p.first = r.first;
+          p.seen0 = r.len - r.count + 1;
+          p.own = 1;
+          p.table_row = b0 + i;
+          p.to = p.tiles < t ? kToSlot : a.prefix_len > 0 ? kToPart : kToOutput;
+          p.slot = 2 * cta + (p.first_tile > 0 ? 0 : 1);
+          if (!emit(p)) return;
+          u += p.tiles;
+        }
+      }
+    }
+  }
+  Piece last{};
+  emit(last);
+}
+
+// Order of a piece's tiles in the ring: K0, K1, V0, K2, V1, ..., V(n-1).
+__device__ __forceinline__ int ring_k(int j) { return j == 0 ? 0 : 2 * j - 1; }
+__device__ __forceinline__ int ring_v(int j, int n) { return j + 1 < n ? 2 * j + 2 : 2 * n - 1; }
+
+// kWide: pages hold whole 64-key tiles, one TMA box each, laid out [4 chunks
+// of 64 lanes][64 keys]; otherwise pages are multiples of eight keys and a
+// tile is eight boxes, laid out [8 groups][4 chunks][8 keys].
+template <bool kWide>
+__device__ __forceinline__ void load_tile(const AttendArgs& a, const CUtensorMap* map, const int32_t* table, int tile,
+                                          int keys, int head, uint32_t dst, uint64_t* bar) {
+  constexpr int kBoxes = kWide ? 1 : kKeys / 8;
+  mbar_arm(bar, kStageBytes);
+#pragma unroll 1
+  for (int g = 0; g < kBoxes; ++g) {
+    const int key = tile * kKeys + g * 8;
+    int block = a.num_blocks, place = 0;  // past the cache: the box is filled with zeros
+    if (key < keys) {
+      const int page = key / a.block_size;
+      place = key - page * a.block_size;
+      block = __ldg(table + page);
+      if (block < 0 || block >= a.num_blocks) {
+        raise_status(a.status, WELM_ROPE_DEV_BAD_PAGE);
+        block = a.num_blocks;
+      }
+    }
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, "
+        "%6}], [%7];" ::"r"(dst + g * (8 * kHeadDim * 2)),
+        "l"(map), "r"(0), "r"(place), "r"(0), "r"(head), "r"(block), "r"(smem_u32(bar))
+        : "memory");
+  }
+}
+
+template <bool kWide>
+__device__ void produce(const AttendArgs& a, Control& ctl, const CUtensorMap* kmap, const CUtensorMap* vmap,
+                        uint32_t ring) {
+  PieceReader pieces;
+  Piece p;
+  uint32_t n = 0;  // tiles put into the ring
+  while (pieces.next<false>(ctl, p)) {
+    const int32_t* table = p.own ? a.block_table + p.table_row * a.table_stride : a.prefix_table;
+    for (int i = 0; i < 2 * p.tiles; ++i, ++n) {
+      // entry i: K0, K1, V0, K2, V1, ...
+      const bool is_v = i == 2 * p.tiles - 1 || (i >= 2 && (i & 1) == 0);
+      const int j = is_v ? (i == 2 * p.tiles - 1 ? p.tiles - 1 : i / 2 - 1) : (i + 1) / 2;
+      const uint32_t s = n % kStages;
+      if (!mbar_wait(ctl, &ctl.empty[s], ((n / kStages) & 1) ^ 1)) goto out;
+      load_tile<kWide>(a, is_v ? vmap : kmap, table, p.first_tile + j, p.keys, p.head, ring + s * kStageBytes,
+                       &ctl.full[s]);
+    }
+  }
+out:
+  // after a failed wait, the copies in flight still have to land
+  if (*reinterpret_cast<volatile int32_t*>(&ctl.failed)) {
+    for (uint32_t i = n > kStages ? n - kStages : 0; i < n; ++i) {
+      const long long t0 = clock64();
+      while (!mbar_poll(&ctl.full[i % kStages], (i / kStages) & 1) && clock64() - t0 < kWaitClocks) {
+      }
+    }
+  }
+}
+
+template <bool kWide>
+__device__ void issue_products(Control& ctl, uint32_t q, uint32_t ring, uint32_t tmem) {
+  // chunks of 64 lanes and groups of eight keys, in bytes apart in a K or V tile
+  constexpr uint32_t kChunk = kWide ? kKeys * 128 : 8 * 128, kGroup = kWide ? 8 * 128 : 8 * kHeadDim * 2;
+  constexpr uint32_t kIdescS = instr_desc(kKeys, false), kIdescO = instr_desc(kHeadDim, true);
+  PieceReader pieces;
+  Piece p;
+  uint32_t base = 0;   // ring entries before this piece
+  uint32_t tile = 0;   // tiles before this piece
+  for (uint32_t np = 0; pieces.next<false>(ctl, p); ++np) {
+    if (!mbar_wait(ctl, &ctl.q_full, np & 1)) break;
+    // the Q rows came by ordinary asynchronous copies
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    bool ok = true;
+    for (int j = 0; j <= p.tiles && ok; ++j) {
+      if (j < p.tiles) {  // S(j) = Q K(j)^T
+        const uint32_t e = base + ring_k(j), s = e % kStages, t = tile + j, buf = t & 1;
+        ok = mbar_wait(ctl, &ctl.full[s], (e / kStages) & 1) &&
+             mbar_wait(ctl, &ctl.s_empty[buf], ((t >> 1) & 1) ^ 1);
+        if (!ok) break;
+        tmem_fence_after();
+        const uint32_t k = ring + s * kStageBytes;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            mma_ss(tmem + kColS + buf * kKeys, operand_desc(q + c * kQChunkBytes + kk * 32, 16, 1024),
+                   operand_desc(k + c * kChunk + kk * 32, 16, kGroup), kIdescS, c + kk > 0);
+        mma_commit(&ctl.s_full[buf]);
+        mma_commit(&ctl.empty[s]);
+        if (j == p.tiles - 1) mma_commit(&ctl.q_empty);
+      }
+      if (j > 0) {  // O += P(j-1) V(j-1)
+        const int jv = j - 1;
+        const uint32_t e = base + ring_v(jv, p.tiles), s = e % kStages, t = tile + jv, buf = t & 1;
+        ok = mbar_wait(ctl, &ctl.full[s], (e / kStages) & 1) && mbar_wait(ctl, &ctl.p_full[buf], (t >> 1) & 1) &&
+             (jv > 0 || mbar_wait(ctl, &ctl.o_free, (np & 1) ^ 1));
+        if (!ok) break;
+        tmem_fence_after();
+        const uint32_t v = ring + s * kStageBytes;
+#pragma unroll
+        for (int ks = 0; ks < kKeys / 16; ++ks)
+          mma_ts(tmem + kColO, tmem + kColP + buf * (kKeys / 2) + ks * 8,
+                 operand_desc(v + ks * 2 * kGroup, kChunk, kGroup), kIdescO, jv > 0 || ks > 0);
+        mma_commit(&ctl.pv_done[buf]);
+        mma_commit(&ctl.empty[s]);
+      }
+    }
+    if (!ok) break;
+    base += 2 * p.tiles;
+    tile += p.tiles;
+  }
+  // no product may outlive the TMEM or the shared memory it works on
+  mma_commit(&ctl.drained);
+  const long long t0 = clock64();
+  while (!mbar_poll(&ctl.drained, 0) && clock64() - t0 < kWaitClocks) {
+  }
+}
+
+// Q rows of each piece: one row of 512 bytes a warp instruction, into the
+// 128-byte swizzle that the products read.  Rows past the item's stay as they
+// are: a row of S and O depends on its own Q row alone.
+__device__ void load_queries(const AttendArgs& a, Control& ctl, uint32_t q) {
+  const int lane = threadIdx.x & 31;
+  PieceReader pieces;
+  Piece p;
+  for (uint32_t np = 0; pieces.next<true>(ctl, p); ++np) {
+    if (!__all_sync(0xffffffffu, mbar_wait(ctl, &ctl.q_empty, (np & 1) ^ 1))) break;
+    int tok = p.row0 / a.group;
+    int g = p.row0 - tok * a.group;
+    for (int r = 0; r < p.rows; ++r) {
+      const uint16_t* src = a.q + (p.first + tok) * a.q_token + (p.head * a.group + g) * a.q_head + lane * 8;
+      const uint32_t dst = q + (lane >> 3) * kQChunkBytes + r * 128 + (((lane & 7) ^ (r & 7)) << 4);
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+      if (++g == a.group) {
+        g = 0;
+        ++tok;
+      }
+    }
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&ctl.q_full)) : "memory");
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// Softmax of the tiles, rescaling of O, and the results.
+template <bool kWide>
+__device__ void softmax_rows(const AttendArgs& a, Control& ctl, uint8_t* ring, uint32_t tmem) {
+  const int lane = threadIdx.x & 31;
+  const int warp = (threadIdx.x >> 5) - kSoftmaxWarp0;
+  const int row = warp * 32 + lane;
+  const uint32_t mine = tmem + (uint32_t(warp * 32) << 16);
+  const float c = a.scale;
+  PieceReader pieces;
+  Piece p;
+  uint32_t base = 0, tile = 0;
+  for (; pieces.next<true>(ctl, p); base += 2 * p.tiles, tile += p.tiles) {
+    const bool busy = warp * 32 < p.rows;  // some lane of the warp has a row
+    const int in_item = p.row0 + row;
+    const int tok = in_item / a.group;
+    int seen = p.own ? p.seen0 + tok : p.seen0;
+    if (seen > p.keys) seen = p.keys;
+    float m = -INFINITY, l = 0.0f;
+    for (int j = 0; j < p.tiles; ++j) {
+      const uint32_t t = tile + j, buf = t & 1, ph = (t >> 1) & 1;
+      if (!__all_sync(0xffffffffu, mbar_wait(ctl, &ctl.s_full[buf], ph))) return;
+      tmem_fence_after();
+      uint32_t s[2][32];
+      if (busy) {
+        tmem_load32(mine + kColS + buf * kKeys, s[0]);
+        tmem_load32(mine + kColS + buf * kKeys + 32, s[1]);
+        tmem_load_wait();
+      }
+      tmem_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl.s_empty[buf]);
+      uint32_t pk[32];
+      if (busy) {
+        const int left = seen - (p.first_tile + j) * kKeys;  // keys of this tile that the row sees
+        if (left < kKeys) {
+#pragma unroll
+          for (int i = 0; i < kKeys; ++i)
+            if (i >= left) s[i >> 5][i & 31] = 0xff800000u;
+        }
+        float top = m;
+#pragma unroll
+        for (int i = 0; i < kKeys; ++i) top = fmaxf(top, __uint_as_float(s[i >> 5][i & 31]));
+        // The maximum in use only moves when it has grown enough to matter:
+        // until then p stays at or below 2^8, well inside BF16 and FP32.
+        const bool grown = (top - m) * c > kRescaleStep;
+        if (j > 0 && __any_sync(0xffffffffu, grown)) {
+          const uint32_t tp = t - 1;
+          if (!__all_sync(0xffffffffu, mbar_wait(ctl, &ctl.pv_done[tp & 1], (tp >> 1) & 1))) return;
+          tmem_fence_after();
+          const float f = grown ? exp2_approx((m - top) * c) : 1.0f;
+          l *= f;
+#pragma unroll 1
+          for (int g = 0; g < kHeadDim / 32; ++g) {
+            uint32_t o[32];
+            tmem_load32(mine + kColO + g * 32, o);
+            tmem_load_wait();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+            tmem_store32(mine + kColO + g * 32, o);
+          }
+          tmem_store_wait();
+          if (grown) m = top;
+        } else if (j == 0) {
+          m = top;
+        }
+        const float mc = m == -INFINITY ? 0.0f : m * c;  // nothing seen yet: every p is 0
+#pragma unroll
+        for (int i = 0; i < kKeys; i += 2) {
+          const float p0 = exp2_approx(fmaf(__uint_as_float(s[i >> 5][i & 31]), c, -mc));
+          const float p1 = exp2_approx(fmaf(__uint_as_float(s[i >> 5][(i & 31) + 1]), c, -mc));
+          l += p0 + p1;
+          pk[i / 2] = pack_bf16x2(p0, p1);
+        }
+      }
+      if (t >= 2) {  // P(t - 2) has been read
+        if (!__all_sync(0xffffffffu, mbar_wait(ctl, &ctl.pv_done[buf], ph ^ 1))) return;
+        tmem_fence_after();
+      }
+      __syncwarp();
+      if (busy) {
+        tmem_store32(mine + kColP + buf * (kKeys / 2), pk);
+        tmem_store_wait();
+      }
+      // V rows past the keys weigh nothing, but what their page holds may be
+      // no number, and 0 times that is none either: they are cleared.
+      const int whole = p.keys - (p.first_tile + j) * kKeys;
+      if (whole < kKeys) {
+        const uint32_t e = base + ring_v(j, p.tiles), st = e % kStages;
+        if (!__all_sync(0xffffffffu, mbar_wait(ctl, &ctl.full[st], (e / kStages) & 1))) return;
+        uint8_t* v = ring + st * kStageBytes;
+        const int end = kWide ? kKeys : (whole + 7) & ~7;  // later groups were filled with zeros
+        for (int i = whole * 32 + row; i < end * 32; i += kRows) {
+          const int key = i >> 5, chunk = (i >> 3) & 3, unit = i & 7;
+          const int at = kWide ? chunk * (kKeys * 128) + key * 128
+                               : (key >> 3) * (8 * kHeadDim * 2) + chunk * 1024 + (key & 7) * 128;
+          *reinterpret_cast<uint4*>(v + at + unit * 16) = make_uint4(0, 0, 0, 0);
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      }
+      tmem_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&ctl.p_full[buf]);
+    }
+    // O of the piece
+    const uint32_t tl = tile + p.tiles - 1;
+    if (!__all_sync(0xffffffffu, mbar_wait(ctl, &ctl.pv_done[tl & 1], (tl >> 1) & 1))) return;
+    tmem_fence_after();
+    if (busy) {
+      const bool live = row < p.rows;
+      const int64_t token = p.first + tok;
+      const int head = p.head * a.group + (in_item - tok * a.group);
+      const int64_t flat = token * a.q_heads + head;
+      float* ml = nullptr;
+      float* to = nullptr;
+      uint16_t* out = nullptr;
+      float scale_out = 1.0f;
+      if (p.to == kToOutput) {
+        out = a.out + token * a.out_token + head * a.out_head;
+        scale_out = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+        if (live && a.lse != nullptr) a.lse[flat] = l > 0.0f || l != l ? (m * c + log2f(l)) * 0.6931471805599453f : -INFINITY;
+      } else if (p.to == kToSlot) {
+        ml = a.slot_ml + (int64_t(p.slot) * a.slot_rows + row) * 2;
+        to = a.slot_o + (int64_t(p.slot) * a.slot_rows + row) * kHeadDim;
+      } else {
+        const int64_t at = int64_t(p.own) * a.tokens * a.q_heads + flat;
+        ml = a.part_ml + at * 2;
+        to = a.part_o + at * kHeadDim;
+      }
+      if (live && ml != nullptr) *reinterpret_cast<float2*>(ml) = make_float2(m == -INFINITY ? m : m * c, l);
+#pragma unroll 1
+      for (int g = 0; g < kHeadDim / 32; ++g) {
+        uint32_t o[32];
+        __syncwarp();
+        tmem_load32(mine + kColO + g * 32, o);
+        tmem_load_wait();
+        if (!live) {
+          // a lane past the item's rows only takes part in the load
+        } else if (p.to == kToOutput) {
+          uint4* dst = reinterpret_cast<uint4*>(out + g * 32);
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            float f[8];
+#pragma unroll
+            for (int x = 0; x < 8; ++x) f[x] = l == 0.0f ? 0.0f : __uint_as_float(o[i + x]) * scale_out;
+            dst[i / 8] = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
+                                    pack_bf16x2(f[6], f[7]));
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            float f[8];
+#pragma unroll
+            for (int x = 0; x < 8; ++x) f[x] = __uint_as_float(o[i + x]);
+            store8f(to + g * 32 + i, f);
+          }
+        }
+      }
+    }
+    tmem_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&ctl.o_free);
+  }
+}
+
+// Tiles of the own items of requests [b0, b1).
+__device__ __forceinline__ int64_t request_units(const AttendArgs& a, int b, bool tell) {
+  const Request r = load_request(a, b, tell);
+  const int rts = r.row_tiles(a.group);
+  int64_t sum = 0;
+  for (int rt = 0; rt < rts; ++rt) sum += r.tiles(a.group, rt);
+  return sum * a.k_heads;
+}
+
+template <bool kWide>
+__global__ void __launch_bounds__(kThreads, 1)
+    rope_attend_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
+                       const __grid_constant__ AttendArgs a) {
+  extern __shared__ uint8_t raw[];
+  uint8_t* smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+  uint8_t* ring = smem + kQBytes;
+  Control& ctl = *reinterpret_cast<Control*>(ring + kStages * kStageBytes);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&ctl.full[s], 1);
+      mbar_init(&ctl.empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&ctl.s_full[i], 1);
+      mbar_init(&ctl.s_empty[i], 4);
+      mbar_init(&ctl.p_full[i], 4);
+      mbar_init(&ctl.pv_done[i], 1);
+    }
+    mbar_init(&ctl.q_full, 32);
+    mbar_init(&ctl.q_empty, 1);
+    mbar_init(&ctl.o_free, 4);
+    mbar_init(&ctl.drained, 1);
+    for (int i = 0; i < kPieces; ++i) {
+      mbar_init(&ctl.piece_full[i], 1);
+      mbar_init(&ctl.piece_empty[i], kPieceReaders);
+    }
+    ctl.failed = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&ctl.tmem))
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tmem_fence_before();
+  __syncthreads();
+  tmem_fence_after();
+  pdl_enter();
+  // Where this CTA's run begins: each thread adds up a stretch of requests.
+  const int used = used_tokens(a);
+  const int64_t pre = prefix_units(a, used);
+  const int stretch = div_up(a.batch, kThreads);
+  const int b0 = tid * stretch < a.batch ? tid * stretch : a.batch;
+  const int b1 = b0 + stretch < a.batch ? b0 + stretch : a.batch;
+  const bool writer = blockIdx.x == 0;
+  int64_t sum = 0;
+  for (int b = b0; b < b1; ++b) sum += request_units(a, b, writer);
+  int64_t incl = sum;
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t x = __shfl_up_sync(0xffffffffu, incl, d);
+    if (lane >= d) incl += x;
+  }
+  if (lane == 31) ctl.scan[warp] = incl;
+  if (tid == 0) {
+    ctl.start_request = a.batch;
+    ctl.start_units = 0;
+  }
+  __syncthreads();
+  int64_t before = incl - sum, total = 0;
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += ctl.scan[w];
+    total += ctl.scan[w];
+  }
+  const Line line(pre + total, a.grid);
+  const bool works = int(blockIdx.x) < line.grid;
+  if (works) {
+    const int64_t want = clamp64(line.begin(blockIdx.x) - pre, 0, total);
+    const bool find = want >= before && want < before + sum;
+    if (find || writer) {
+      int64_t u = before;
+      for (int b = b0; b < b1; ++b) {
+        const int64_t n = request_units(a, b, false);
+        if (find && want >= u && want < u + n) {
+          ctl.start_request = b;
+          ctl.start_units = u;
+        }
+        if (writer) a.units_before[b] = u;
+        u += n;
+      }
+    }
+  }
+  if (writer && tid == 0) a.units_before[a.batch] = total;
+  __syncthreads();
+  const uint32_t tmem = ctl.tmem;
+  if (works) {
+    const uint32_t q_at = smem_u32(smem), ring_at = smem_u32(ring);
+    if (warp == 0) {
+      if (lane == 0) produce<kWide>(a, ctl, &kmap, &vmap, ring_at);
+    } else if (warp == 1) {
+      if (lane == 0) issue_products<kWide>(ctl, q_at, ring_at, tmem);
+    } else if (warp == 2) {
+      load_queries(a, ctl, q_at);
+    } else if (warp == 3) {
+      list_pieces(a, ctl, line, blockIdx.x, used, pre);
+    } else {
+      softmax_rows<kWide>(a, ctl, ring, tmem);
+    }
+  }
+  tmem_fence_before();
+  __syncthreads();
+  if (tid == 0 && ctl.failed) raise_status(a.status, WELM_ROPE_DEV_WAIT_TIMEOUT);
+  if (warp == 1) {
+    tmem_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Joining the partial results of a row: kGroups x 64 threads a row, four lanes
+// of the head each; the groups take the row's partial results in turn.
+// ---------------------------------------------------------------------------
+struct Part {
+  int64_t ml, o;  // offsets into the workspace arrays
+};
+
+template <int kGroups>
+__global__ void __launch_bounds__(256) rope_attend_join_kernel(const __grid_constant__ AttendArgs a) {
+  constexpr int kRowThreads = 64 * kGroups, kRowsPerCta = 256 / kRowThreads;
+  __shared__ float4 s_o[kGroups > 1 ? 256 : 1];
+  __shared__ float2 s_ml[kGroups > 1 ? kGroups : 1];
+  const int part = threadIdx.x % kRowThreads;
+  const int grp = part >> 6, d4 = part & 63;
+  const int64_t flat = int64_t(blockIdx.x) * kRowsPerCta + threadIdx.x / kRowThreads;
+  pdl_enter();
+  const int used = used_tokens(a);
+  const int64_t rows = int64_t(a.tokens) * a.q_heads;
+  bool live = flat < rows;
+  const int token = live ? int(flat / a.q_heads) : 0;
+  const int hq = live ? int(flat - int64_t(token) * a.q_heads) : 0;
+  const int h = hq / a.group, g = hq - h * a.group;
+  // the row's request
+  int b = token;
+  if (a.query_starts != nullptr) {
+    int lo = 0, hi = a.batch;  // the last request that starts at or before the token
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (__ldg(a.query_starts + mid) <= token) lo = mid; else hi = mid;
+    }
+    b = lo;
+  }
+  Request r{0, 0, 0};
+  if (live && token < used) r = load_request(a, b, false);
+  const bool spare = live && (token < r.first || token >= r.first + r.count);  // a row of no request
+  if (spare) live = false;
+  const int64_t pre = prefix_units(a, used);
+  const int64_t total = a.units_before[a.batch];
+  const Line line(pre + total, a.grid);
+  // the two items of the row: [first unit, past the last), and its row in each
+  int64_t lo[2] = {0, 0}, hi[2] = {0, 0};
+  int in_tile[2] = {0, 0};
+  if (live) {
+    if (pre > 0) {
+      const int packed = token * a.group + g;
+      const int key_tiles = div_up(a.prefix_len, kKeys);
+      lo[0] = (int64_t(h) * div_up(used * a.group, kRows) + packed / kRows) * key_tiles;
+      hi[0] = lo[0] + key_tiles;
+      in_tile[0] = packed % kRows;
+    }
+    const int packed = (token - r.first) * a.group + g;
+    const int rt = packed / kRows;
+    int64_t u = pre + a.units_before[b];
+    for (int x = 0; x < rt; ++x) u += int64_t(r.tiles(a.group, x)) * a.k_heads;
+    const int t = r.tiles(a.group, rt);
+    lo[1] = u + int64_t(h) * t;
+    hi[1] = lo[1] + t;
+    in_tile[1] = packed % kRows;
+  }
+  int c0[2] = {0, 0}, n[2] = {0, 0};
+  for (int x = 0; x < 2; ++x) {
+    if (hi[x] == lo[x]) continue;
+    c0[x] = line.cta_of(lo[x]);
+    n[x] = line.cta_of(hi[x] - 1) - c0[x] + 1;
+  }
+  // written whole by the first kernel
+  if (pre == 0 && n[0] + n[1] == 1) live = false;
+  auto where = [&](int i) {
+    const int x = i >= n[0];
+    if (n[x] == 1) {
+      const int64_t at = int64_t(x) * rows + flat;
+      return Part{int64_t(a.part_ml - a.slot_ml) + at * 2, int64_t(a.part_o - a.slot_ml) + at * kHeadDim};
+    }
+    const int c = c0[x] + (x ? i - n[0] : i);
+    const int64_t at = int64_t(2 * c + (lo[x] < line.begin(c) ? 0 : 1)) * a.slot_rows + in_tile[x];
+    return Part{at * 2, int64_t(a.slot_o - a.slot_ml) + at * kHeadDim};
+  };
+  float m = -INFINITY, l = 0.0f;
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  const int count = live ? n[0] + n[1] : 0;
+  constexpr int kUnroll = 4;
+  for (int i0 = grp; i0 < count; i0 += kGroups * kUnroll) {
+    float2 ml[kUnroll];
+    float4 v[kUnroll];
+#pragma unroll
+    for (int x = 0; x < kUnroll; ++x) {
+      const int i = i0 + x * kGroups;
+      ml[x] = make_float2(-INFINITY, 0.0f);
+      v[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (i < count) {
+        const Part p = where(i);
+        ml[x] = *reinterpret_cast<const float2*>(a.slot_ml + p.ml);
+        v[x] = *reinterpret_cast<const float4*>(a.slot_ml + p.o + d4 * 4);
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < kUnroll; ++x) {
+      if (ml[x].x == -INFINITY && ml[x].y == 0.0f) continue;  // saw no key
+      const float top = fmaxf(m, ml[x].x);
+      const float base = top == -INFINITY ? 0.0f : top;
+      const float f0 = exp2_approx(m - base), f1 = exp2_approx(ml[x].x - base);
+      l = l * f0 + ml[x].y * f1;
+      o.x = o.x * f0 + v[x].x * f1;
+      o.y = o.y * f0 + v[x].y * f1;
+      o.z = o.z * f0 + v[x].z * f1;
+      o.w = o.w * f0 + v[x].w * f1;
+      m = top;
+    }
+  }
+  if (kGroups > 1) {
+    s_o[threadIdx.x] = o;
+    if (d4 == 0) s_ml[grp] = make_float2(m, l);
+    __syncthreads();
+    if (grp > 0) return;
+    for (int x = 1; x < kGroups; ++x) {
+      const float2 ml = s_ml[x];
+      if (ml.x == -INFINITY && ml.y == 0.0f) continue;
+      const float4 v = s_o[x * 64 + d4];
+      const float top = fmaxf(m, ml.x);
+      const float base = top == -INFINITY ? 0.0f : top;
+      const float f0 = exp2_approx(m - base), f1 = exp2_approx(ml.x - base);
+      l = l * f0 + ml.y * f1;
+      o.x = o.x * f0 + v.x * f1;
+      o.y = o.y * f0 + v.y * f1;
+      o.z = o.z * f0 + v.z * f1;
+      o.w = o.w * f0 + v.w * f1;
+      m = top;
+    }
+  }
+  if (!live && !(spare && a.fill)) return;
+  const bool none = l == 0.0f;
+  const float inv = none ? 0.0f : 1.0f / l;
+  uint2 packed = make_uint2(0, 0);
+  if (!none) packed = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+  *reinterpret_cast<uint2*>(a.out + token * a.out_token + hq * a.out_head + d4 * 4) = packed;
+  if (a.lse != nullptr && d4 == 0) a.lse[flat] = none ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+}
+
+// ---------------------------------------------------------------------------
+// Host side.
+// ---------------------------------------------------------------------------
+// Layout of the workspace, in bytes from its base.
+struct Workspace {
+  int64_t units, slot_ml, slot_o, part_ml, part_o, bytes;
+};
+
+Workspace attend_workspace(int64_t tokens, int64_t batch, int64_t q_heads, int64_t group, int64_t prefix_len,
+                           int64_t grid) {
+  auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
+  const int64_t rows = tokens * group < kRows ? tokens * group : kRows;
+  const int64_t slots = 2 * grid * rows;
+  const int64_t parts = prefix_len > 0 ? 2 * tokens * q_heads : 0;
+  Workspace w;
+  w.units = 0;
+  w.slot_ml = up((batch + 1) * 8);
+  w.slot_o = w.slot_ml + up(slots * 8);
+  w.part_ml = w.slot_o + up(slots * kHeadDim * 4);
+  w.part_o = w.part_ml + up(parts * 8);
+  w.bytes = w.part_o + up(parts * kHeadDim * 4);
+  return w;
+}
+
+// Tensor map of a cache as {64 lanes, slot, chunk of 64 lanes, head, block}.
+bool encode_cache_map(CUtensorMap& map, const void* base, int64_t blocks, int64_t block_size, int64_t heads,
+                      const int64_t* strides, int box_keys) {
+  const PFN_cuTensorMapEncodeTiled_v12000 encode = tensor_map_encoder();
+  if (encode == nullptr) return false;
+  const cuuint64_t dim[5] = {64, cuuint64_t(block_size), 4, cuuint64_t(heads), cuuint64_t(blocks)};
+  // the stride of a dimension of one is not used, but has to be one
+  auto step = [](int64_t extent, int64_t stride) { return cuuint64_t(extent > 1 ? stride : kHeadDim) * 2; };
+  const cuuint64_t stride[4] = {step(block_size, strides[1]), 128, step(heads, strides[2]), step(blocks, strides[0])};
+  const cuuint32_t box[5] = {64, cuuint32_t(box_keys), 4, 1, 1};
+  const cuuint32_t unit[5] = {1, 1, 1, 1, 1};
+  return encode(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(base), dim, stride, box, unit,
+                CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool attend_sizes_ok(int64_t tokens, int64_t batch, int64_t q_heads, int64_t k_heads, int64_t prefix_len) {
+  if (tokens < 0 || batch < 0 || q_heads < 1 || k_heads < 1 || prefix_len < 0) return false;
+  if (q_heads % k_heads != 0 || batch > kMaxItems || prefix_len > kMaxItems) return false;
+  return q_heads <= kMaxItems && tokens <= kMaxItems / q_heads;
+}
+
+template <bool kWide>
+int launch_attend(const CUtensorMap& kmap, const CUtensorMap& vmap, const AttendArgs& a, cudaStream_t stream) {
+  if (cudaFuncSetAttribute(rope_attend_kernel<kWide>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes) !=
+      cudaSuccess) {
+    cudaGetLastError();
+    return WELM_ROPE_ERR_CUDA;
+  }
+  int rc = launch(rope_attend_kernel<kWide>, unsigned(a.grid), kThreads, kSmemBytes, stream, kmap, vmap, a);
+  if (rc != WELM_ROPE_OK) return rc;
+  const int64_t rows = int64_t(a.tokens) * a.q_heads;
+  if (rows <= 1024) return launch(rope_attend_join_kernel<4>, unsigned(rows), 256, 0, stream, a);
+  return launch(rope_attend_join_kernel<1>, unsigned((rows + 3) / 4), 256, 0, stream, a);
+}
+
+}  // namespace
+
+extern "C" {
+
+int welm_rope_attend_workspace(int64_t n_tokens, int64_t batch_size, int64_t num_q_heads, int64_t num_k_heads,
+                               int64_t prefix_len, int64_t* bytes) {
+  if (!bytes) return WELM_ROPE_ERR_NULL_POINTER;
+  if (!attend_sizes_ok(n_tokens, batch_size, num_q_heads, num_k_heads, prefix_len)) return WELM_ROPE_ERR_BAD_SIZE;
+  const int sms = current_sm_count();
+  if (sms <= 0) {
+    cudaGetLastError();
+    return WELM_ROPE_ERR_CUDA;
+  }
+  *bytes = attend_workspace(n_tokens, batch_size, num_q_heads, num_q_heads / num_k_heads, prefix_len, sms).bytes;
+  return WELM_ROPE_OK;
+}
+
+int welm_rope_attend(const void* q, void* out, float* lse, const void* key_cache, const void* value_cache,
+                     const int32_t* block_table, const int64_t* seq_lens, const int64_t* query_starts,
+                     const int32_t* prefix_table, int64_t prefix_len, int64_t n_tokens, int64_t batch_size,
+                     int64_t num_q_heads, int64_t num_k_heads, int64_t q_token_stride, int64_t q_head_stride,
+                     int64_t out_token_stride, int64_t out_head_stride, int64_t table_width, int64_t table_stride,
+                     int64_t num_blocks, int64_t block_size, const int64_t* key_cache_strides,
+                     const int64_t* value_cache_strides, float scale, int64_t fill_unused, void* workspace,
+                     int64_t workspace_bytes, int32_t* device_status, void* stream) {
+  if (!attend_sizes_ok(n_tokens, batch_size, num_q_heads, num_k_heads, prefix_len)) return WELM_ROPE_ERR_BAD_SIZE;
+  if (num_blocks < 0 || block_size < 1 || table_width < 0 || num_blocks > kMaxItems || block_size > kMaxItems ||
+      table_width > kMaxItems / block_size)
+    return WELM_ROPE_ERR_BAD_SIZE;
+  if (!query_starts && n_tokens != batch_size) return WELM_ROPE_ERR_BAD_SIZE;
+  if (!(scale > 0.0f) || scale > 3.0e38f || (fill_unused != 0 && fill_unused != 1)) return WELM_ROPE_ERR_BAD_MODE;
+  if (n_tokens == 0 || batch_size == 0) return WELM_ROPE_OK;
+  if (block_size % 8 != 0 || num_blocks == 0) return WELM_ROPE_ERR_BAD_SIZE;
+  if (!q || !out || !key_cache || !value_cache || !seq_lens || !workspace || !key_cache_strides ||
+      !value_cache_strides || (table_width > 0 && !block_table) || (prefix_len > 0 && !prefix_table))
+    return WELM_ROPE_ERR_NULL_POINTER;
+  if (q_token_stride < 0 || q_head_stride < 0 || table_stride < 0 ||
+      !rows_apart<2>({n_tokens, num_q_heads}, {out_token_stride, out_head_stride}))
+    return WELM_ROPE_ERR_BAD_STRIDE;
+  int64_t bits = q_token_stride | q_head_stride | out_token_stride | out_head_stride;
+  const int64_t extent[3] = {num_blocks, block_size, num_k_heads};
+  for (const int64_t* s : {key_cache_strides, value_cache_strides}) {
+    for (int i = 0; i < 3; ++i) {
+      // tensor maps: steps of 16 bytes, below 2^40
+      if (extent[i] > 1 && (s[i] < kHeadDim || s[i] >= (int64_t(1) << 39))) return WELM_ROPE_ERR_BAD_STRIDE;
+      if (extent[i] > 1) bits |= s[i];
+    }
+  }
+  if (bits & 7) return WELM_ROPE_ERR_BAD_STRIDE;
+  for (const void* p : {q, static_cast<const void*>(out), key_cache, value_cache, static_cast<const void*>(workspace)})
+    if (!aligned16(p)) return WELM_ROPE_ERR_BAD_STRIDE;
+  const int sms = current_sm_count();
+  if (sms <= 0) {
+    cudaGetLastError();
+    return WELM_ROPE_ERR_CUDA;
+  }
+  const int64_t group = num_q_heads / num_k_heads;
+  const Workspace w = attend_workspace(n_tokens, batch_size, num_q_heads, group, prefix_len, sms);
+  if (workspace_bytes < w.bytes) return WELM_ROPE_ERR_CAPACITY;
+  const bool wide = block_size % kKeys == 0;
+  const int box = wide ? kKeys : 8;
+  CUtensorMap kmap, vmap;
+  if (!encode_cache_map(kmap, key_cache, num_blocks, block_size, num_k_heads, key_cache_strides, box) ||
+      !encode_cache_map(vmap, value_cache, num_blocks, block_size, num_k_heads, value_cache_strides, box))
+    return WELM_ROPE_ERR_CUDA;
+  AttendArgs a{};
+  a.q = static_cast<const uint16_t*>(q);
+  a.out = static_cast<uint16_t*>(out);
+  a.lse = lse;
+  a.q_token = q_token_stride;
+  a.q_head = q_head_stride;
+  a.out_token = out_token_stride;
+  a.out_head = out_head_stride;
+  a.prefix_table = prefix_table;
+  a.block_table = block_table;
+  a.table_stride = table_stride;
+  a.seq_lens = seq_lens;
+  a.query_starts = query_starts;
+  a.tokens = int32_t(n_tokens);
+  a.batch = int32_t(batch_size);
+  a.q_heads = int32_t(num_q_heads);
+  a.k_heads = int32_t(num_k_heads);
+  a.group = int32_t(group);
+  a.prefix_len = int32_t(prefix_len);
+  a.max_len = int32_t(table_width * block_size);
+  a.block_size = int32_t(block_size);
+  a.num_blocks = int32_t(num_blocks);
+  a.slot_rows = int32_t(n_tokens * group < kRows ? n_tokens * group : kRows);
+  a.grid = sms;
+  a.fill = int32_t(fill_unused);
+  a.scale = scale * 1.4426950408889634f;
+  char* base = static_cast<char*>(workspace);
+  a.units_before = reinterpret_cast<int64_t*>(base + w.units);
+  a.slot_ml = reinterpret_cast<float*>(base + w.slot_ml);
+  a.slot_o = reinterpret_cast<float*>(base + w.slot_o);
+  a.part_ml = reinterpret_cast<float*>(base + w.part_ml);
+  a.part_o = reinterpret_cast<float*>(base + w.part_o);
+  a.status = device_status;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return wide ? launch_attend<true>(kmap, vmap, a, s) : launch_attend<false>(kmap, vmap, a, s);
+}
+
+}  // extern "C"

@@ -24,9 +24,7 @@
 //   stores — so the register path can be compared with TMA staging on the
 //   op's own buffers.
 
-#include <cudaTypedefs.h>
-
-#include "rope_host.cuh"
+#include "rope_tma.cuh"
 
 namespace {
 
@@ -154,24 +152,6 @@ constexpr int kTmaKBytes = kRopeDim * 2 * kTmaTileTokens;
 constexpr int kTmaStageBytes = kTmaQBytes + kTmaKBytes;
 constexpr int kTmaWaitPolls = 1 << 22;
 
-__device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
-}
-
-__device__ __forceinline__ void mbar_arm(uint64_t* bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
-}
-
-__device__ __forceinline__ bool mbar_poll(uint64_t* bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
-      : "=r"(done)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return done != 0;
-}
-
 __device__ __forceinline__ void tma_tile_load(uint8_t* stage, const CUtensorMap* qmap, const CUtensorMap* kmap,
                                               int tile, uint64_t* bar) {
   const int z = tile * kTmaTileTokens;
@@ -244,21 +224,6 @@ __global__ void __launch_bounds__(kBlock) ceiling_tma_slices_kernel(const __grid
     }
   }
   asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-}
-
-// The driver's tensor-map encoder, looked up once through the runtime.
-PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
-  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult found;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found) != cudaSuccess ||
-        found != cudaDriverEntryPointSuccess) {
-      cudaGetLastError();
-      return static_cast<PFN_cuTensorMapEncodeTiled_v12000>(nullptr);
-    }
-    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-  }();
-  return fn;
 }
 
 // Tensor maps of Q ({256 lanes, 6 heads, N tokens}) and K ({256 lanes, N

@@ -150,6 +150,27 @@ int launch(void (*kernel)(Params...), unsigned grid, unsigned block, size_t smem
   return WELM_ROPE_OK;
 }
 
+// Whether the 256-lane rows of a tensor with these extents and strides are
+// apart from one another: from the smallest stride up, each steps over all
+// that the smaller ones span.  Every usual order of the dimensions passes.
+template <int N>
+bool rows_apart(const int64_t (&extent)[N], const int64_t (&stride)[N]) {
+  int order[N];
+  for (int i = 0; i < N; ++i) {
+    int at = i;
+    for (; at > 0 && stride[order[at - 1]] > stride[i]; --at) order[at] = order[at - 1];
+    order[at] = i;
+  }
+  __int128 span = kHeadDim;
+  for (int i = 0; i < N; ++i) {
+    const int64_t n = extent[order[i]], s = stride[order[i]];
+    if (n <= 1) continue;
+    if (s < span) return false;
+    span += __int128(s) * (n - 1);
+  }
+  return span <= __int128(INT64_MAX) / 2;
+}
+
 // How the token phase is laid out for one call (see Source).
 struct Plan {
   Source src;

@@ -1,0 +1,128 @@
+// rope_multi_axis.cu — rotary embedding with a position per axis (time,
+// height, width, ...), in place or into new tensors, forward or inverse, and
+// its C entry welm_rope_multi_axis.
+//
+// The rotation of a pair is orthogonal, so the gradient of the inputs is the
+// inverse rotation (sin negated) of the gradient of the outputs: the backward
+// pass is this kernel again.  Memory-bound: six FP32 operations a pair.  Work
+// item: (token, head, part), four threads a head as in the other kernels; the
+// Q heads of a token come first, then its K heads, so the threads of a warp
+// share the token's cos/sin lines in L1.
+
+#include "rope_axes.cuh"
+
+namespace {
+
+struct MultiAxisArgs {
+  const uint16_t* src[2];  // Q and K
+  uint16_t* dst[2];        // src in place, or the copies
+  int64_t src_token[2], src_head[2], dst_token[2], dst_head[2];
+  AxisArgs axes;
+  int32_t* status;
+  int32_t items, heads, q_heads;
+  float sign;  // +1 forward, -1 inverse
+};
+
+// kCopy: whole heads are read and written (lanes 0..191 copied); otherwise only
+// the rotated lanes move.  A token whose position is out of range is copied
+// unrotated, or left as it is, and flagged.
+template <bool kCopy>
+__global__ void __launch_bounds__(kBlock) rope_multi_axis_kernel(const MultiAxisArgs a) {
+  const int item = blockIdx.x * blockDim.x + threadIdx.x;
+  const int part = item & (kParts - 1);
+  const int row = item >> kPartShift;
+  const int tok = row / a.heads;
+  const int head = row - tok * a.heads;
+  const int x = head >= a.q_heads;
+  const int h = x ? head - a.q_heads : head;
+  const uint16_t* src = a.src[x] + tok * a.src_token[x] + h * a.src_head[x];
+  pdl_enter();
+  if (item >= a.items) return;
+  WholeHead piece;
+  if (kCopy) {
+    piece.load(src, part);
+  } else {
+    piece.x1 = *reinterpret_cast<const uint4*>(src + kRopeLane0 + part * kLanes);
+    piece.x2 = *reinterpret_cast<const uint4*>(src + kRopeLane0 + kHalf + part * kLanes);
+  }
+  AxisRows rows;
+  const bool ok = rows.load(a.axes, tok);
+  if (ok) {
+    CosSin cs;
+    rows.gather(a.axes.map, part, cs);
+#pragma unroll
+    for (int i = 0; i < kLanes; ++i) cs.s[i] *= a.sign;
+    rotate8(piece.x1, piece.x2, cs);
+  } else if (part == 0 && head == 0) {
+    raise_status(a.status, WELM_ROPE_DEV_BAD_POSITION);
+  }
+  uint16_t* dst = a.dst[x] + tok * a.dst_token[x] + h * a.dst_head[x];
+  if (kCopy) {
+    piece.store(dst, part);
+  } else if (ok) {
+    *reinterpret_cast<uint4*>(dst + kRopeLane0 + part * kLanes) = piece.x1;
+    *reinterpret_cast<uint4*>(dst + kRopeLane0 + kHalf + part * kLanes) = piece.x2;
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+int welm_rope_multi_axis(const void* q, void* q_out, const void* k, void* k_out, const int64_t* positions,
+                         const float* cos_sin_cache, const int32_t* sections, int64_t num_axes, int64_t interleaved,
+                         int64_t inverse, int64_t n_tokens, int64_t num_q_heads, int64_t num_k_heads,
+                         int64_t q_token_stride, int64_t q_head_stride, int64_t q_out_token_stride,
+                         int64_t q_out_head_stride, int64_t k_token_stride, int64_t k_head_stride,
+                         int64_t k_out_token_stride, int64_t k_out_head_stride, int64_t position_stride,
+                         int64_t max_position, int32_t* device_status, void* stream) {
+  if (num_axes < 1 || num_axes > kMaxAxes || (interleaved != 0 && interleaved != 1) || (inverse != 0 && inverse != 1))
+    return WELM_ROPE_ERR_BAD_MODE;
+  if (!sections) return WELM_ROPE_ERR_NULL_POINTER;
+  MultiAxisArgs a{};
+  if (!make_axis_map(sections, num_axes, interleaved, a.axes.map)) return WELM_ROPE_ERR_BAD_MODE;
+  if (n_tokens < 0 || num_q_heads < 0 || num_k_heads < 0 || max_position < 0) return WELM_ROPE_ERR_BAD_SIZE;
+  if (num_q_heads > kMaxItems || num_k_heads > kMaxItems) return WELM_ROPE_ERR_BAD_SIZE;
+  const int64_t heads = num_q_heads + num_k_heads;
+  if (n_tokens == 0 || heads == 0) return WELM_ROPE_OK;
+  if (n_tokens > kMaxItems / kParts / heads) return WELM_ROPE_ERR_BAD_SIZE;
+  if ((num_q_heads > 0 && (!q || !q_out)) || (num_k_heads > 0 && (!k || !k_out)) || !positions || !cos_sin_cache)
+    return WELM_ROPE_ERR_NULL_POINTER;
+  const void* src[2] = {q, k};
+  void* dst[2] = {q_out, k_out};
+  const int64_t count[2] = {num_q_heads, num_k_heads};
+  const int64_t strides[2][4] = {{q_token_stride, q_head_stride, q_out_token_stride, q_out_head_stride},
+                                 {k_token_stride, k_head_stride, k_out_token_stride, k_out_head_stride}};
+  bool in_place = true;
+  for (int x = 0; x < 2; ++x) {
+    if (count[x] == 0) continue;
+    const int64_t* s = strides[x];
+    // sources may repeat a row (stride 0); destinations may not
+    if (s[0] < 0 || s[1] < 0 || !rows_apart<2>({n_tokens, count[x]}, {s[2], s[3]})) return WELM_ROPE_ERR_BAD_STRIDE;
+    if (!aligned16(src[x]) || !aligned16(dst[x]) || ((s[0] | s[1] | s[2] | s[3]) & 7)) return WELM_ROPE_ERR_BAD_STRIDE;
+    if (src[x] != dst[x]) in_place = false;
+    else if (s[0] != s[2] || s[1] != s[3]) return WELM_ROPE_ERR_BAD_STRIDE;
+    a.src[x] = static_cast<const uint16_t*>(src[x]);
+    a.dst[x] = static_cast<uint16_t*>(dst[x]);
+    a.src_token[x] = s[0];
+    a.src_head[x] = s[1];
+    a.dst_token[x] = s[2];
+    a.dst_head[x] = s[3];
+  }
+  if (!aligned16(cos_sin_cache) || (num_axes > 1 && position_stride < 0)) return WELM_ROPE_ERR_BAD_STRIDE;
+  a.axes.positions = positions;
+  a.axes.pos_stride = position_stride;
+  a.axes.cache = cos_sin_cache;
+  a.axes.max_position = max_position;
+  a.status = device_status;
+  a.heads = int32_t(heads);
+  a.q_heads = int32_t(num_q_heads);
+  a.items = int32_t(n_tokens * heads * kParts);
+  a.sign = inverse ? -1.0f : 1.0f;
+  const unsigned grid = unsigned((int64_t(a.items) + kBlock - 1) / kBlock);
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return in_place ? launch(rope_multi_axis_kernel<false>, grid, kBlock, 0, s, a)
+                  : launch(rope_multi_axis_kernel<true>, grid, kBlock, 0, s, a);
+}
+
+}  // extern "C"

@@ -1,0 +1,197 @@
+"""CPU checks of the attention kernels' work division, restated from
+rope_attend.cu: the pieces that the CTAs list cover every 64-key tile of every
+item once, every workspace index lies inside its array, and the join kernel
+finds exactly the pieces that hold a row's partial results."""
+
+from __future__ import annotations
+
+import random
+
+import pytest
+
+ROWS, KEYS = 128, 64
+
+
+def div_up(a, b):
+    return (a + b - 1) // b
+
+
+class Plan:
+    def __init__(self, counts, lens, prefix, q_heads, k_heads, grid):
+        self.counts, self.lens, self.prefix = counts, lens, prefix
+        self.q_heads, self.k_heads, self.group = q_heads, k_heads, q_heads // k_heads
+        self.starts = [0]
+        for n in counts:
+            self.starts.append(self.starts[-1] + n)
+        self.tokens = self.starts[-1]
+        self.row_tiles = div_up(self.tokens * self.group, ROWS)
+        self.pre = self.row_tiles * k_heads * div_up(prefix, KEYS)
+        self.before = [0]
+        for b in range(len(counts)):
+            self.before.append(self.before[-1] + k_heads * sum(self.tiles(b, rt) for rt in range(self.own_tiles(b))))
+        self.units = self.pre + self.before[-1]
+        self.grid = min(grid, self.units)
+        self.slot_rows = min(ROWS, self.tokens * self.group)
+
+    def own_tiles(self, b):
+        return div_up(self.counts[b] * self.group, ROWS)
+
+    def seen(self, b, rt):
+        last = min((rt * ROWS + ROWS - 1) // self.group, self.counts[b] - 1)
+        return max(0, self.lens[b] - self.counts[b] + last + 1)
+
+    def tiles(self, b, rt):
+        return div_up(self.seen(b, rt), KEYS)
+
+    def begin(self, c):
+        return self.units * c // self.grid
+
+    def cta_of(self, u):
+        return ((u + 1) * self.grid - 1) // self.units
+
+    def pieces(self, cta):
+        """(item, first tile, tiles, destination) in the order of list_pieces."""
+        u, end = self.begin(cta), self.begin(cta + 1)
+        key_tiles = div_up(self.prefix, KEYS)
+        while u < end and u < self.pre:
+            item, first = divmod(u, key_tiles)
+            n = min(end - u, key_tiles - first)
+            head, tile = divmod(item, self.row_tiles)
+            to = ("part", 0) if n == key_tiles else ("slot", 2 * cta + (0 if first > 0 else 1))
+            yield ("prefix", head, tile), first, n, to
+            u += n
+        want = max(0, min(self.begin(cta) - self.pre, self.before[-1]))
+        start = next((b for b in range(len(self.counts)) if self.before[b] <= want < self.before[b + 1]),
+                     len(self.counts))
+        base = self.pre + (self.before[start] if start < len(self.counts) else 0)
+        for b in range(start, len(self.counts)):
+            for rt in range(self.own_tiles(b)):
+                t = self.tiles(b, rt)
+                for h in range(self.k_heads):
+                    if u < end and u < base + t:
+                        first = u - base
+                        assert first >= 0
+                        n = min(end - u, t - first)
+                        to = ("slot", 2 * cta + (0 if first > 0 else 1)) if n < t else (
+                            ("part", 1) if self.prefix else ("out", 0))
+                        yield ("own", b, rt, h), first, n, to
+                        u += n
+                    base += t
+        assert u == end
+
+    def join(self, token, hq):
+        """The places of a row's partial results in the order of the keys, or None where the first kernel wrote it."""
+        h, g = divmod(hq, self.group)
+        b = max(i for i in range(len(self.counts)) if self.starts[i] <= token and self.counts[i])
+        found = []
+        ranges = []
+        if self.pre:
+            packed = token * self.group + g
+            key_tiles = div_up(self.prefix, KEYS)
+            lo = (h * self.row_tiles + packed // ROWS) * key_tiles
+            ranges.append((0, lo, lo + key_tiles, packed % ROWS))
+        packed = (token - self.starts[b]) * self.group + g
+        rt = packed // ROWS
+        lo = self.pre + self.before[b] + self.k_heads * sum(self.tiles(b, x) for x in range(rt)) + h * self.tiles(b, rt)
+        ranges.append((1, lo, lo + self.tiles(b, rt), packed % ROWS))
+        for x, lo, hi, row in ranges:
+            if lo == hi:
+                continue
+            c0, c1 = self.cta_of(lo), self.cta_of(hi - 1)
+            if c0 == c1:
+                found.append(("part", x, token * self.q_heads + hq) if self.pre else None)
+            else:
+                found += [("slot", 2 * c + (0 if lo < self.begin(c) else 1), row) for c in range(c0, c1 + 1)]
+        return None if found == [None] else found
+
+
+def check(plan):
+    held = {}  # (token, query head) -> places in the order of the pieces' CTAs
+    covered = {}
+    if plan.units:
+        for cta in range(plan.grid):
+            used = set()
+            for item, first, n, to in plan.pieces(cta):
+                assert n > 0
+                covered.setdefault(item, []).append((first, n))
+                if to[0] == "slot":
+                    assert 0 <= to[1] < 2 * plan.grid and to[1] not in used
+                    used.add(to[1])
+                if item[0] == "prefix":
+                    _, head, tile = item
+                    first_token, row0, limit = 0, tile * ROWS, plan.tokens * plan.group
+                else:
+                    _, b, rt, head = item
+                    first_token, row0, limit = plan.starts[b], rt * ROWS, plan.counts[b] * plan.group
+                for row in range(min(ROWS, limit - row0)):
+                    tok, g = divmod(row0 + row, plan.group)
+                    key = (first_token + tok, head * plan.group + g)
+                    assert row < plan.slot_rows and key[0] < plan.tokens
+                    place = None if to[0] == "out" else ("slot", to[1], row) if to[0] == "slot" else (
+                        "part", to[1], key[0] * plan.q_heads + key[1])
+                    held.setdefault(key, []).append(place)
+    expected = {}
+    if plan.prefix:
+        for h in range(plan.k_heads):
+            for t in range(plan.row_tiles):
+                expected["prefix", h, t] = div_up(plan.prefix, KEYS)
+    for b in range(len(plan.counts)):
+        for rt in range(plan.own_tiles(b)):
+            for h in range(plan.k_heads):
+                if plan.tiles(b, rt):
+                    expected["own", b, rt, h] = plan.tiles(b, rt)
+    assert covered.keys() == expected.keys()
+    for item, runs in covered.items():
+        runs.sort()
+        at = 0
+        for first, n in runs:
+            assert first == at
+            at += n
+        assert at == expected[item]
+    for token in range(plan.tokens):
+        for hq in range(plan.q_heads):
+            want = held.get((token, hq), [])
+            assert plan.join(token, hq) == (None if want == [None] else want), (token, hq)
+
+
+@pytest.mark.parametrize("counts,lens,prefix,heads,grid", [
+    ([1], [300], 0, (6, 1), 148), ([1], [0], 0, (6, 1), 148), ([1], [0], 1, (6, 1), 148),
+    ([1] * 40, [50] * 40, 1000, (6, 1), 148), ([5, 0, 3], [7, 9, 1], 65, (8, 2), 148),
+    ([100, 40], [100, 300], 200, (6, 1), 16), ([3], [5000], 0, (130, 1), 7), ([1] * 300, [1] * 300, 0, (6, 1), 148),
+])
+def test_pieces_cover_every_tile_and_the_join_finds_them(counts, lens, prefix, heads, grid):
+    check(Plan(counts, lens, prefix, *heads, grid))
+
+
+def test_random_batches():
+    rng = random.Random(5)
+    for _ in range(60):
+        batch = rng.randint(1, 20)
+        counts = [rng.choice([0, 1, 1, rng.randint(1, 60)]) for _ in range(batch)]
+        lens = [rng.choice([0, 1, 63, 64, 65, rng.randint(0, 2000)]) for _ in range(batch)]
+        prefix = rng.choice([0, 1, 64, rng.randint(1, 3000)])
+        heads = rng.choice([(6, 1), (8, 2), (4, 4), (12, 2)])
+        check(Plan(counts, lens, prefix, *heads, rng.choice([1, 5, 20, 148])))
+
+
+def test_ring_order_names_every_entry_once():
+    """K0, K1, V0, K2, V1, ...: what the producer loads at each entry is what the issuer looks for there."""
+    ring_k = lambda j: 0 if j == 0 else 2 * j - 1  # noqa: E731
+    ring_v = lambda j, n: 2 * j + 2 if j + 1 < n else 2 * n - 1  # noqa: E731
+    for n in range(1, 40):
+        produced = {}
+        for i in range(2 * n):
+            is_v = i == 2 * n - 1 or (i >= 2 and i % 2 == 0)
+            j = (n - 1 if i == 2 * n - 1 else i // 2 - 1) if is_v else (i + 1) // 2
+            produced[i] = (is_v, j)
+        assert sorted(produced.values()) == [(v, j) for v in (False, True) for j in range(n)]
+        for j in range(n):
+            assert produced[ring_k(j)] == (False, j) and produced[ring_v(j, n)] == (True, j)
+        # the order in which the products take them
+        taken = []
+        for j in range(n + 1):
+            if j < n:
+                taken.append(ring_k(j))
+            if j > 0:
+                taken.append(ring_v(j - 1, n))
+        assert taken == list(range(2 * n))
