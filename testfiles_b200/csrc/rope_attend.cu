@@ -12,39 +12,42 @@
 // against a run of keys.  The prefix's items take their rows from all requests
 // together, so a prefix key is read once for every 128 rows instead of once
 // for every request; a request's own items hold its own rows.  All items'
-// 64-key tiles form one line, cut into equal runs, one for each CTA; a CTA
+// 128-key tiles form one line, cut into equal runs, one for each CTA; a CTA
 // walks the pieces of items in its run.  An item that is cut, or whose rows
 // also have the other part, leaves FP32 partial results in the workspace, and
 // a second kernel joins them row by row in the order of the keys, so results
 // do not depend on timing.  Lengths stay on the device: every CTA adds the
 // requests' tiles up for itself, and a captured launch follows new lengths.
 //
-// One CTA on an SM, eight warps:
-//   0     TMA producer: K and V tiles (64 keys, 32 KB each) into a ring of five
-//   1     issues tcgen05.mma: S = Q K^T (128 x 64) and O += P V (128 x 256)
-//   2     brings the piece's Q rows into shared memory (64 KB)
-//   3     lists the CTA's pieces
-//   4..7  softmax, one row a thread; rescaling of O; the results
-// S, P (BF16) and O live in TMEM (S and P twice, so that the softmax of one
-// tile runs beside the products of its neighbours).  P is rounded to BF16
-// because the product with the BF16 values takes both operands in one type;
-// l sums the unrounded p, and S, m, l and O are FP32.
+// One CTA on an SM, twelve warps:
+//   0      TMA producer: K and V, half a tile (128 keys x 128 lanes, 32 KB) at
+//          a time, into a ring of five
+//   1      issues tcgen05.mma: S = Q K^T (128 x 128) and O += P V (128 x 256)
+//   2      brings the piece's Q rows into shared memory (64 KB)
+//   3      lists the CTA's pieces
+//   4..11  softmax: two threads a row, 64 keys each; rescaling of O; results
+// S and O live in TMEM, S twice, so that the softmax of one tile runs beside
+// the products of its neighbours; P (BF16) takes the place of S.  P is rounded
+// to BF16 because the product with the BF16 values takes both operands in one
+// type; l sums the unrounded p, and S, m, l and O are FP32.
 
 #include "rope_tma.cuh"
 
 namespace {
 
 constexpr int kRows = 128;             // query rows of an item
-constexpr int kKeys = 64;              // keys of a tile
-constexpr int kStages = 5;             // ring of K and V tiles
-constexpr int kStageBytes = kKeys * kHeadDim * 2;
+constexpr int kKeys = 128;             // keys of a tile
+constexpr int kHalfLanes = kHeadDim / 2;   // lanes of half a K or V tile
+constexpr int kStages = 5;             // ring of halves of K and V tiles
+constexpr int kChunkBytes = kKeys * 128;   // 64 lanes of 128 keys
+constexpr int kStageBytes = 2 * kChunkBytes;
 constexpr int kQChunkBytes = kRows * 128;  // 64 lanes of 128 rows
 constexpr int kQBytes = kRows * kHeadDim * 2;
 constexpr int kPieces = 4;             // ring of piece descriptors
-constexpr int kThreads = 256;
-constexpr int kSoftmaxWarp0 = 4;
-constexpr int kPieceReaders = 3 + 4;   // producer, issuer, Q warp, four softmax warps
-constexpr uint32_t kColS = 0, kColP = 128, kColO = 256;  // TMEM columns
+constexpr int kThreads = 384;
+constexpr int kSoftmaxWarp0 = 4, kSoftmaxWarps = 8;
+constexpr int kPieceReaders = 3 + kSoftmaxWarps;  // producer, issuer, Q warp, softmax warps
+constexpr uint32_t kColS = 0, kColO = 256;  // TMEM columns: S (and P) of even and odd tiles, then O
 constexpr long long kWaitClocks = 1ll << 32;  // about two seconds
 constexpr float kRescaleStep = 8.0f;   // O is rescaled when the maximum grows by more than 2^8
 
@@ -61,11 +64,12 @@ struct AttendArgs {
   int32_t tokens, batch, q_heads, k_heads, group;
   int32_t prefix_len, max_len;  // max_len: keys that a row of block_table can name
   int32_t block_size, num_blocks;
+  int32_t box_keys;             // keys of one TMA box: a power of two that divides block_size
   int32_t slot_rows;            // rows of a workspace slot
   int32_t grid;
   int32_t fill;                 // 1: rows of no request become zeros
   float scale;                  // times log2(e)
-  int64_t* units_before;        // [batch + 1] tiles of the items before each request
+  int32_t* units_before;        // [batch + 1] tiles of the items before each request
   float* slot_ml;               // [2 grid][slot_rows][2]
   float* slot_o;                // [2 grid][slot_rows][256]
   float* part_ml;               // [2][tokens * q_heads][2]: whole items' rows, prefix and own
@@ -119,15 +123,20 @@ __device__ __forceinline__ int used_tokens(const AttendArgs& a) {
 // The line of tiles, cut into `grid` runs: CTA c has [begin(c), begin(c + 1)).
 // No run is empty: a line of fewer tiles than CTAs keeps only as many busy.
 struct Line {
-  int64_t units;
-  int grid;
-  __device__ __forceinline__ Line(int64_t n, int ctas) : units(n), grid(n < ctas ? int(n) : ctas) {}
-  __device__ __forceinline__ int64_t begin(int c) const { return units * c / grid; }
-  __device__ __forceinline__ int cta_of(int64_t u) const { return int(((u + 1) * grid - 1) / units); }
+  int units, grid, each, more;  // the first `more` runs have each + 1 tiles
+  __device__ __forceinline__ Line(int n, int ctas) : units(n), grid(n < ctas ? n : ctas) {
+    each = grid > 0 ? n / grid : 0;
+    more = n - each * grid;
+  }
+  __device__ __forceinline__ int begin(int c) const { return each * c + (c < more ? c : more); }
+  __device__ __forceinline__ int cta_of(int u) const {
+    const int longer = more * (each + 1);
+    return u < longer ? u / (each + 1) : more + (u - longer) / each;
+  }
 };
 
-__device__ __forceinline__ int64_t prefix_units(const AttendArgs& a, int used) {
-  return int64_t(div_up(used * a.group, kRows)) * a.k_heads * div_up(a.prefix_len, kKeys);
+__device__ __forceinline__ int prefix_units(const AttendArgs& a, int used) {
+  return div_up(used * a.group, kRows) * a.k_heads * div_up(a.prefix_len, kKeys);
 }
 
 enum Destination { kToOutput, kToSlot, kToPart };
@@ -150,19 +159,26 @@ struct Piece {
 
 struct Control {
   uint64_t full[kStages], empty[kStages];
-  uint64_t s_full[2], s_empty[2], p_full[2], pv_done[2];
+  uint64_t s_full[2], p_full[2], pv_done[2];
   uint64_t q_full, q_empty, o_free, drained;
+  uint64_t swap[4];  // the two warps of 32 rows
   uint64_t piece_full[kPieces], piece_empty[kPieces];
   Piece piece[kPieces];
-  int64_t scan[kThreads / 32];
-  int64_t start_units;
+  int32_t scan[kThreads / 32];
+  int32_t start_units;
   int32_t start_request;
   uint32_t tmem;
   int32_t failed;
 };
 
-constexpr int kSmemBytes = 1024 + kQBytes + kStages * kStageBytes + 1024;
-static_assert(sizeof(Control) <= 1024, "control block");
+// The two halves of a row's keys swap their maxima (even and odd tiles apart)
+// and at last their sums through shared memory.
+struct Swap {
+  float value[2][2][kRows];  // [tile parity][half]
+};
+
+constexpr int kSmemBytes = kQBytes + kStages * kStageBytes + sizeof(Swap) + 768;
+static_assert(sizeof(Control) <= 768, "control block");
 static_assert(kSmemBytes <= 227 * 1024, "shared memory of one CTA");
 
 // Waits for a phase of `bar`; false once any warp of the CTA has given up.
@@ -284,7 +300,7 @@ struct PieceReader {
 };
 
 // Lists the pieces of this CTA's run of tiles.
-__device__ void list_pieces(const AttendArgs& a, Control& ctl, const Line& line, int cta, int used, int64_t pre) {
+__device__ void list_pieces(const AttendArgs& a, Control& ctl, const Line& line, int cta, int used, int pre) {
   const int lane = threadIdx.x & 31;
   int n = 0;
   // every lane holds the piece; lane 0 writes it
@@ -299,19 +315,19 @@ __device__ void list_pieces(const AttendArgs& a, Control& ctl, const Line& line,
     ++n;
     return true;
   };
-  int64_t u = line.begin(cta);
-  const int64_t end = line.begin(cta + 1);
+  int u = line.begin(cta);
+  const int end = line.begin(cta + 1);
   const int key_tiles = div_up(a.prefix_len, kKeys);
   const int row_tiles = div_up(used * a.group, kRows);
   while (u < end && u < pre) {
-    const int item = int(u / key_tiles);
+    const int item = u / key_tiles;
     Piece p;
-    p.first_tile = int(u - int64_t(item) * key_tiles);
-    p.tiles = int(clamp64(end - u, 0, key_tiles - p.first_tile));
+    p.first_tile = u - item * key_tiles;
+    p.tiles = min(end - u, key_tiles - p.first_tile);
     p.keys = a.prefix_len;
     p.head = item / row_tiles;
     p.row0 = (item - p.head * row_tiles) * kRows;
-    p.rows = used * a.group - p.row0 < kRows ? used * a.group - p.row0 : kRows;
+    p.rows = min(used * a.group - p.row0, kRows);
     p.first = 0;
     p.seen0 = a.prefix_len;
     p.own = 0;
@@ -321,7 +337,7 @@ __device__ void list_pieces(const AttendArgs& a, Control& ctl, const Line& line,
     if (!emit(p)) return;
     u += p.tiles;
   }
-  int64_t base = ctl.start_units + pre;  // of request `start_request`
+  int base = ctl.start_units + pre;  // of request `start_request`
   for (int b0 = ctl.start_request; u < end && b0 < a.batch; b0 += 32) {
     Request mine{0, 0, 0};
     if (b0 + lane < a.batch) mine = load_request(a, b0 + lane, false);
@@ -334,12 +350,12 @@ __device__ void list_pieces(const AttendArgs& a, Control& ctl, const Line& line,
         for (int h = 0; h < a.k_heads && u < end; ++h, base += t) {
           if (u >= base + t) continue;
           Piece p;
-          p.first_tile = int(u - base);
-          p.tiles = int(clamp64(end - u, 0, t - p.first_tile));
+          p.first_tile = u - base;
+          p.tiles = min(end - u, t - p.first_tile);
           p.keys = r.seen(a.group, rt);
           p.head = h;
           p.row0 = rt * kRows;
-          p.rows = r.count * a.group - p.row0 < kRows ? r.count * a.group - p.row0 : kRows;
+          p.rows = min(r.count * a.group - p.row0, kRows);
           p.first = r.first;
           p.seen0 = r.len - r.count + 1;
           p.own = 1;
@@ -356,23 +372,32 @@ __device__ void list_pieces(const AttendArgs& a, Control& ctl, const Line& line,
   emit(last);
 }
 
-// Order of a piece's tiles in the ring: K0, K1, V0, K2, V1, ..., V(n-1).
+// Order of a piece's tiles in the ring: K0, K1, V0, K2, V1, ..., V(n-1), each
+// as its lower and its upper 128 lanes.
 __device__ __forceinline__ int ring_k(int j) { return j == 0 ? 0 : 2 * j - 1; }
 __device__ __forceinline__ int ring_v(int j, int n) { return j + 1 < n ? 2 * j + 2 : 2 * n - 1; }
 
-// kWide: pages hold whole 64-key tiles, one TMA box each, laid out [4 chunks
-// of 64 lanes][64 keys]; otherwise pages are multiples of eight keys and a
-// tile is eight boxes, laid out [8 groups][4 chunks][8 keys].
-template <bool kWide>
-__device__ __forceinline__ void load_tile(const AttendArgs& a, const CUtensorMap* map, const int32_t* table, int tile,
-                                          int keys, int head, uint32_t dst, uint64_t* bar) {
-  constexpr int kBoxes = kWide ? 1 : kKeys / 8;
-  mbar_arm(bar, kStageBytes);
-#pragma unroll 1
-  for (int g = 0; g < kBoxes; ++g) {
-    const int key = tile * kKeys + g * 8;
-    int block = a.num_blocks, place = 0;  // past the cache: the box is filled with zeros
-    if (key < keys) {
+// The producer warp.  A half tile is [2 chunks of 64 lanes][128 keys][128
+// bytes], filled by boxes of 64 lanes x box_keys keys: pages need not hold
+// whole tiles.  Lane g of the warp looks up the block of the tile's g-th box
+// of keys, one tile ahead, and issues that box's copies.
+__device__ void produce(const AttendArgs& a, Control& ctl, const CUtensorMap* kmap, const CUtensorMap* vmap,
+                        uint32_t ring) {
+  const int lane = threadIdx.x & 31;
+  const int boxes = kKeys / a.box_keys;
+  PieceReader pieces;
+  Piece p;
+  uint32_t n = 0;  // half tiles put into the ring
+  bool ok = true;
+  while (ok && pieces.next<true>(ctl, p)) {
+    const int32_t* table = p.own ? a.block_table + p.table_row * a.table_stride : a.prefix_table;
+    // Block and place of this lane's box in tile j; behind the keys the block
+    // past the cache, whose box is filled with zeros.
+    auto look_up = [&](int j, int& block, int& place) {
+      const int key = (p.first_tile + j) * kKeys + lane * a.box_keys;
+      block = a.num_blocks;
+      place = 0;
+      if (j >= p.tiles || lane >= boxes || key >= p.keys) return;
       const int page = key / a.block_size;
       place = key - page * a.block_size;
       block = __ldg(table + page);
@@ -380,34 +405,39 @@ __device__ __forceinline__ void load_tile(const AttendArgs& a, const CUtensorMap
         raise_status(a.status, WELM_ROPE_DEV_BAD_PAGE);
         block = a.num_blocks;
       }
+    };
+    auto load = [&](const CUtensorMap* map, int block, int place) {
+#pragma unroll 1
+      for (int half = 0; half < 2; ++half, ++n) {
+        const uint32_t s = n % kStages;
+        if (!__all_sync(0xffffffffu, mbar_wait(ctl, &ctl.empty[s], ((n / kStages) & 1) ^ 1))) return false;
+        if (lane == 0) mbar_arm(&ctl.full[s], kStageBytes);
+        __syncwarp();
+        if (lane < boxes) {
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+            asm volatile(
+                "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
+                "%4, %5}], [%6];" ::"r"(ring + s * kStageBytes + c * kChunkBytes + lane * a.box_keys * 128),
+                "l"(map), "r"(half * kHalfLanes + c * 64), "r"(place), "r"(p.head), "r"(block),
+                "r"(smem_u32(&ctl.full[s]))
+                : "memory");
+        }
+      }
+      return true;
+    };
+    int block, place, block_v = 0, place_v = 0, block_next, place_next;
+    look_up(0, block, place);
+    for (int j = 0; j <= p.tiles && ok; ++j) {
+      look_up(j + 1, block_next, place_next);
+      if (j < p.tiles) ok = load(kmap, block, place);
+      if (ok && j > 0) ok = load(vmap, block_v, place_v);
+      block_v = block;
+      place_v = place;
+      block = block_next;
+      place = place_next;
     }
-    asm volatile(
-        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, "
-        "%6}], [%7];" ::"r"(dst + g * (8 * kHeadDim * 2)),
-        "l"(map), "r"(0), "r"(place), "r"(0), "r"(head), "r"(block), "r"(smem_u32(bar))
-        : "memory");
   }
-}
-
-template <bool kWide>
-__device__ void produce(const AttendArgs& a, Control& ctl, const CUtensorMap* kmap, const CUtensorMap* vmap,
-                        uint32_t ring) {
-  PieceReader pieces;
-  Piece p;
-  uint32_t n = 0;  // tiles put into the ring
-  while (pieces.next<false>(ctl, p)) {
-    const int32_t* table = p.own ? a.block_table + p.table_row * a.table_stride : a.prefix_table;
-    for (int i = 0; i < 2 * p.tiles; ++i, ++n) {
-      // entry i: K0, K1, V0, K2, V1, ...
-      const bool is_v = i == 2 * p.tiles - 1 || (i >= 2 && (i & 1) == 0);
-      const int j = is_v ? (i == 2 * p.tiles - 1 ? p.tiles - 1 : i / 2 - 1) : (i + 1) / 2;
-      const uint32_t s = n % kStages;
-      if (!mbar_wait(ctl, &ctl.empty[s], ((n / kStages) & 1) ^ 1)) goto out;
-      load_tile<kWide>(a, is_v ? vmap : kmap, table, p.first_tile + j, p.keys, p.head, ring + s * kStageBytes,
-                       &ctl.full[s]);
-    }
-  }
-out:
   // after a failed wait, the copies in flight still have to land
   if (*reinterpret_cast<volatile int32_t*>(&ctl.failed)) {
     for (uint32_t i = n > kStages ? n - kStages : 0; i < n; ++i) {
@@ -418,14 +448,11 @@ out:
   }
 }
 
-template <bool kWide>
 __device__ void issue_products(Control& ctl, uint32_t q, uint32_t ring, uint32_t tmem) {
-  // chunks of 64 lanes and groups of eight keys, in bytes apart in a K or V tile
-  constexpr uint32_t kChunk = kWide ? kKeys * 128 : 8 * 128, kGroup = kWide ? 8 * 128 : 8 * kHeadDim * 2;
-  constexpr uint32_t kIdescS = instr_desc(kKeys, false), kIdescO = instr_desc(kHeadDim, true);
+  constexpr uint32_t kIdescS = instr_desc(kKeys, false), kIdescO = instr_desc(kHalfLanes, true);
   PieceReader pieces;
   Piece p;
-  uint32_t base = 0;   // ring entries before this piece
+  uint32_t base = 0;   // ring entries before this piece, in whole tiles of K or V
   uint32_t tile = 0;   // tiles before this piece
   for (uint32_t np = 0; pieces.next<false>(ctl, p); ++np) {
     if (!mbar_wait(ctl, &ctl.q_full, np & 1)) break;
@@ -433,37 +460,49 @@ __device__ void issue_products(Control& ctl, uint32_t q, uint32_t ring, uint32_t
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     bool ok = true;
     for (int j = 0; j <= p.tiles && ok; ++j) {
-      if (j < p.tiles) {  // S(j) = Q K(j)^T
-        const uint32_t e = base + ring_k(j), s = e % kStages, t = tile + j, buf = t & 1;
-        ok = mbar_wait(ctl, &ctl.full[s], (e / kStages) & 1) &&
-             mbar_wait(ctl, &ctl.s_empty[buf], ((t >> 1) & 1) ^ 1);
+      if (j < p.tiles) {  // S(j) = Q K(j)^T, once P(j - 2) in its place has been used
+        const uint32_t t = tile + j, buf = t & 1;
+        ok = t < 2 || mbar_wait(ctl, &ctl.pv_done[buf], ((t >> 1) & 1) ^ 1);
+#pragma unroll
+        for (int half = 0; half < 2 && ok; ++half) {
+          const uint32_t e = 2 * (base + ring_k(j)) + half, s = e % kStages;
+          ok = mbar_wait(ctl, &ctl.full[s], (e / kStages) & 1);
+          if (!ok) break;
+          tmem_fence_after();
+          const uint32_t k = ring + s * kStageBytes;
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              mma_ss(tmem + kColS + buf * kKeys, operand_desc(q + (2 * half + c) * kQChunkBytes + kk * 32, 16, 1024),
+                     operand_desc(k + c * kChunkBytes + kk * 32, 16, 1024), kIdescS, half + c + kk > 0);
+          mma_commit(&ctl.empty[s]);
+        }
         if (!ok) break;
-        tmem_fence_after();
-        const uint32_t k = ring + s * kStageBytes;
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            mma_ss(tmem + kColS + buf * kKeys, operand_desc(q + c * kQChunkBytes + kk * 32, 16, 1024),
-                   operand_desc(k + c * kChunk + kk * 32, 16, kGroup), kIdescS, c + kk > 0);
         mma_commit(&ctl.s_full[buf]);
-        mma_commit(&ctl.empty[s]);
         if (j == p.tiles - 1) mma_commit(&ctl.q_empty);
       }
       if (j > 0) {  // O += P(j-1) V(j-1)
         const int jv = j - 1;
-        const uint32_t e = base + ring_v(jv, p.tiles), s = e % kStages, t = tile + jv, buf = t & 1;
-        ok = mbar_wait(ctl, &ctl.full[s], (e / kStages) & 1) && mbar_wait(ctl, &ctl.p_full[buf], (t >> 1) & 1) &&
+        const uint32_t t = tile + jv, buf = t & 1;
+        ok = mbar_wait(ctl, &ctl.p_full[buf], (t >> 1) & 1) &&
              (jv > 0 || mbar_wait(ctl, &ctl.o_free, (np & 1) ^ 1));
-        if (!ok) break;
-        tmem_fence_after();
-        const uint32_t v = ring + s * kStageBytes;
 #pragma unroll
-        for (int ks = 0; ks < kKeys / 16; ++ks)
-          mma_ts(tmem + kColO, tmem + kColP + buf * (kKeys / 2) + ks * 8,
-                 operand_desc(v + ks * 2 * kGroup, kChunk, kGroup), kIdescO, jv > 0 || ks > 0);
+        for (int half = 0; half < 2 && ok; ++half) {
+          const uint32_t e = 2 * (base + ring_v(jv, p.tiles)) + half, s = e % kStages;
+          ok = mbar_wait(ctl, &ctl.full[s], (e / kStages) & 1);
+          if (!ok) break;
+          tmem_fence_after();
+          const uint32_t v = ring + s * kStageBytes;
+          // P: keys 0..63 in the first 32 columns of S, keys 64..127 in those from column 64
+#pragma unroll
+          for (int ks = 0; ks < kKeys / 16; ++ks)
+            mma_ts(tmem + kColO + half * kHalfLanes, tmem + kColS + buf * kKeys + (ks >> 2) * 64 + (ks & 3) * 8,
+                   operand_desc(v + ks * 16 * 128, kChunkBytes, 1024), kIdescO, jv > 0 || ks > 0);
+          mma_commit(&ctl.empty[s]);
+        }
+        if (!ok) break;
         mma_commit(&ctl.pv_done[buf]);
-        mma_commit(&ctl.empty[s]);
       }
     }
     if (!ok) break;
@@ -502,17 +541,31 @@ __device__ void load_queries(const AttendArgs& a, Control& ctl, uint32_t q) {
   asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// Softmax of the tiles, rescaling of O, and the results.
-template <bool kWide>
-__device__ void softmax_rows(const AttendArgs& a, Control& ctl, uint8_t* ring, uint32_t tmem) {
+// Softmax of the tiles, rescaling of O, and the results.  Two threads hold a
+// row: the first four warps its keys 0..63 of a tile and lanes 0..127 of O,
+// the others the rest; they swap maxima, so both come to the same ones.
+__device__ void softmax_rows(const AttendArgs& a, Control& ctl, Swap& swap, uint8_t* ring, uint32_t tmem) {
   const int lane = threadIdx.x & 31;
-  const int warp = (threadIdx.x >> 5) - kSoftmaxWarp0;
+  const int warp = ((threadIdx.x >> 5) - kSoftmaxWarp0) & 3;
+  const int half = (threadIdx.x >> 5) >= kSoftmaxWarp0 + 4;
   const int row = warp * 32 + lane;
   const uint32_t mine = tmem + (uint32_t(warp * 32) << 16);
+  const uint32_t my_s = mine + kColS + half * 64, my_o = mine + kColO + half * kHalfLanes;
   const float c = a.scale;
   PieceReader pieces;
   Piece p;
-  uint32_t base = 0, tile = 0;
+  uint32_t base = 0, tile = 0, swaps = 0;
+  // hands `value` to the row's other thread and returns that thread's
+  auto trade = [&](float value, float& other) {
+    const uint32_t parity = swaps & 1;
+    swap.value[parity][half][row] = value;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&ctl.swap[warp]);
+    if (!__all_sync(0xffffffffu, mbar_wait(ctl, &ctl.swap[warp], parity))) return false;
+    other = swap.value[parity][half ^ 1][row];
+    ++swaps;
+    return true;
+  };
   for (; pieces.next<true>(ctl, p); base += 2 * p.tiles, tile += p.tiles) {
     const bool busy = warp * 32 < p.rows;  // some lane of the warp has a row
     const int in_item = p.row0 + row;
@@ -524,26 +577,23 @@ __device__ void softmax_rows(const AttendArgs& a, Control& ctl, uint8_t* ring, u
       const uint32_t t = tile + j, buf = t & 1, ph = (t >> 1) & 1;
       if (!__all_sync(0xffffffffu, mbar_wait(ctl, &ctl.s_full[buf], ph))) return;
       tmem_fence_after();
-      uint32_t s[2][32];
       if (busy) {
-        tmem_load32(mine + kColS + buf * kKeys, s[0]);
-        tmem_load32(mine + kColS + buf * kKeys + 32, s[1]);
+        uint32_t s[2][32];
+        tmem_load32(my_s + buf * kKeys, s[0]);
+        tmem_load32(my_s + buf * kKeys + 32, s[1]);
         tmem_load_wait();
-      }
-      tmem_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&ctl.s_empty[buf]);
-      uint32_t pk[32];
-      if (busy) {
-        const int left = seen - (p.first_tile + j) * kKeys;  // keys of this tile that the row sees
-        if (left < kKeys) {
+        const int left = seen - (p.first_tile + j) * kKeys - half * 64;  // of these 64 keys, those that the row sees
+        if (left < 64) {
 #pragma unroll
-          for (int i = 0; i < kKeys; ++i)
+          for (int i = 0; i < 64; ++i)
             if (i >= left) s[i >> 5][i & 31] = 0xff800000u;
         }
-        float top = m;
+        float tops[4] = {m, m, m, m};
 #pragma unroll
-        for (int i = 0; i < kKeys; ++i) top = fmaxf(top, __uint_as_float(s[i >> 5][i & 31]));
+        for (int i = 0; i < 64; ++i) tops[i & 3] = fmaxf(tops[i & 3], __uint_as_float(s[i >> 5][i & 31]));
+        float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), other;
+        if (!trade(top, other)) return;
+        top = fmaxf(top, other);
         // The maximum in use only moves when it has grown enough to matter:
         // until then p stays at or below 2^8, well inside BF16 and FP32.
         const bool grown = (top - m) * c > kRescaleStep;
@@ -554,13 +604,13 @@ __device__ void softmax_rows(const AttendArgs& a, Control& ctl, uint8_t* ring, u
           const float f = grown ? exp2_approx((m - top) * c) : 1.0f;
           l *= f;
 #pragma unroll 1
-          for (int g = 0; g < kHeadDim / 32; ++g) {
+          for (int g = 0; g < kHalfLanes / 32; ++g) {
             uint32_t o[32];
-            tmem_load32(mine + kColO + g * 32, o);
+            tmem_load32(my_o + g * 32, o);
             tmem_load_wait();
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-            tmem_store32(mine + kColO + g * 32, o);
+            tmem_store32(my_o + g * 32, o);
           }
           tmem_store_wait();
           if (grown) m = top;
@@ -568,37 +618,33 @@ __device__ void softmax_rows(const AttendArgs& a, Control& ctl, uint8_t* ring, u
           m = top;
         }
         const float mc = m == -INFINITY ? 0.0f : m * c;  // nothing seen yet: every p is 0
+        uint32_t pk[32];
+        float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < kKeys; i += 2) {
+        for (int i = 0; i < 64; i += 2) {
           const float p0 = exp2_approx(fmaf(__uint_as_float(s[i >> 5][i & 31]), c, -mc));
           const float p1 = exp2_approx(fmaf(__uint_as_float(s[i >> 5][(i & 31) + 1]), c, -mc));
-          l += p0 + p1;
+          sums[i & 2] += p0;
+          sums[(i & 2) + 1] += p1;
           pk[i / 2] = pack_bf16x2(p0, p1);
         }
-      }
-      if (t >= 2) {  // P(t - 2) has been read
-        if (!__all_sync(0xffffffffu, mbar_wait(ctl, &ctl.pv_done[buf], ph ^ 1))) return;
-        tmem_fence_after();
-      }
-      __syncwarp();
-      if (busy) {
-        tmem_store32(mine + kColP + buf * (kKeys / 2), pk);
+        l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+        __syncwarp();
+        tmem_store32(my_s + buf * kKeys, pk);
         tmem_store_wait();
       }
       // V rows past the keys weigh nothing, but what their page holds may be
-      // no number, and 0 times that is none either: they are cleared.
+      // no number, and 0 times that is none either: they are cleared.  Boxes
+      // that begin behind the keys were filled with zeros.
       const int whole = p.keys - (p.first_tile + j) * kKeys;
       if (whole < kKeys) {
-        const uint32_t e = base + ring_v(j, p.tiles), st = e % kStages;
+        const uint32_t e = 2 * (base + ring_v(j, p.tiles)) + half, st = e % kStages;
         if (!__all_sync(0xffffffffu, mbar_wait(ctl, &ctl.full[st], (e / kStages) & 1))) return;
         uint8_t* v = ring + st * kStageBytes;
-        const int end = kWide ? kKeys : (whole + 7) & ~7;  // later groups were filled with zeros
-        for (int i = whole * 32 + row; i < end * 32; i += kRows) {
-          const int key = i >> 5, chunk = (i >> 3) & 3, unit = i & 7;
-          const int at = kWide ? chunk * (kKeys * 128) + key * 128
-                               : (key >> 3) * (8 * kHeadDim * 2) + chunk * 1024 + (key & 7) * 128;
-          *reinterpret_cast<uint4*>(v + at + unit * 16) = make_uint4(0, 0, 0, 0);
-        }
+        const int end = div_up(whole, a.box_keys) * a.box_keys;
+        for (int i = whole * 16 + row; i < end * 16; i += kRows)
+          *reinterpret_cast<uint4*>(v + ((i >> 3) & 1) * kChunkBytes + (i >> 4) * 128 + (i & 7) * 16) =
+              make_uint4(0, 0, 0, 0);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
       tmem_fence_before();
@@ -610,6 +656,9 @@ __device__ void softmax_rows(const AttendArgs& a, Control& ctl, uint8_t* ring, u
     if (!__all_sync(0xffffffffu, mbar_wait(ctl, &ctl.pv_done[tl & 1], (tl >> 1) & 1))) return;
     tmem_fence_after();
     if (busy) {
+      float other;
+      if (!trade(l, other)) return;
+      l = half ? other + l : l + other;
       const bool live = row < p.rows;
       const int64_t token = p.first + tok;
       const int head = p.head * a.group + (in_item - tok * a.group);
@@ -619,23 +668,25 @@ __device__ void softmax_rows(const AttendArgs& a, Control& ctl, uint8_t* ring, u
       uint16_t* out = nullptr;
       float scale_out = 1.0f;
       if (p.to == kToOutput) {
-        out = a.out + token * a.out_token + head * a.out_head;
-        scale_out = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-        if (live && a.lse != nullptr) a.lse[flat] = l > 0.0f || l != l ? (m * c + log2f(l)) * 0.6931471805599453f : -INFINITY;
+        out = a.out + token * a.out_token + head * a.out_head + half * kHalfLanes;
+        scale_out = l == 0.0f ? 0.0f : 1.0f / l;
+        if (live && half == 0 && a.lse != nullptr)
+          a.lse[flat] = l == 0.0f ? -INFINITY : (m * c + log2f(l)) * 0.6931471805599453f;
       } else if (p.to == kToSlot) {
         ml = a.slot_ml + (int64_t(p.slot) * a.slot_rows + row) * 2;
-        to = a.slot_o + (int64_t(p.slot) * a.slot_rows + row) * kHeadDim;
+        to = a.slot_o + (int64_t(p.slot) * a.slot_rows + row) * kHeadDim + half * kHalfLanes;
       } else {
         const int64_t at = int64_t(p.own) * a.tokens * a.q_heads + flat;
         ml = a.part_ml + at * 2;
-        to = a.part_o + at * kHeadDim;
+        to = a.part_o + at * kHeadDim + half * kHalfLanes;
       }
-      if (live && ml != nullptr) *reinterpret_cast<float2*>(ml) = make_float2(m == -INFINITY ? m : m * c, l);
+      if (live && half == 0 && ml != nullptr)
+        *reinterpret_cast<float2*>(ml) = make_float2(m == -INFINITY ? m : m * c, l);
 #pragma unroll 1
-      for (int g = 0; g < kHeadDim / 32; ++g) {
+      for (int g = 0; g < kHalfLanes / 32; ++g) {
         uint32_t o[32];
         __syncwarp();
-        tmem_load32(mine + kColO + g * 32, o);
+        tmem_load32(my_o + g * 32, o);
         tmem_load_wait();
         if (!live) {
           // a lane past the item's rows only takes part in the load
@@ -666,23 +717,22 @@ __device__ void softmax_rows(const AttendArgs& a, Control& ctl, uint8_t* ring, u
   }
 }
 
-// Tiles of the own items of requests [b0, b1).
-__device__ __forceinline__ int64_t request_units(const AttendArgs& a, int b, bool tell) {
+// Tiles of a request's own items.
+__device__ __forceinline__ int request_units(const AttendArgs& a, int b, bool tell) {
   const Request r = load_request(a, b, tell);
   const int rts = r.row_tiles(a.group);
-  int64_t sum = 0;
+  int sum = 0;
   for (int rt = 0; rt < rts; ++rt) sum += r.tiles(a.group, rt);
   return sum * a.k_heads;
 }
 
-template <bool kWide>
 __global__ void __launch_bounds__(kThreads, 1)
     rope_attend_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                        const __grid_constant__ AttendArgs a) {
-  extern __shared__ uint8_t raw[];
-  uint8_t* smem = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
+  extern __shared__ __align__(1024) uint8_t smem[];  // the 128-byte swizzle repeats every 1024 bytes
   uint8_t* ring = smem + kQBytes;
-  Control& ctl = *reinterpret_cast<Control*>(ring + kStages * kStageBytes);
+  Swap& swap = *reinterpret_cast<Swap*>(ring + kStages * kStageBytes);
+  Control& ctl = *reinterpret_cast<Control*>(&swap + 1);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     for (int s = 0; s < kStages; ++s) {
@@ -691,14 +741,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&ctl.s_full[i], 1);
-      mbar_init(&ctl.s_empty[i], 4);
-      mbar_init(&ctl.p_full[i], 4);
+      mbar_init(&ctl.p_full[i], kSoftmaxWarps);
       mbar_init(&ctl.pv_done[i], 1);
     }
     mbar_init(&ctl.q_full, 32);
     mbar_init(&ctl.q_empty, 1);
-    mbar_init(&ctl.o_free, 4);
+    mbar_init(&ctl.o_free, kSoftmaxWarps);
     mbar_init(&ctl.drained, 1);
+    for (int i = 0; i < 4; ++i) mbar_init(&ctl.swap[i], 2);
     for (int i = 0; i < kPieces; ++i) {
       mbar_init(&ctl.piece_full[i], 1);
       mbar_init(&ctl.piece_empty[i], kPieceReaders);
@@ -717,16 +767,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   pdl_enter();
   // Where this CTA's run begins: each thread adds up a stretch of requests.
   const int used = used_tokens(a);
-  const int64_t pre = prefix_units(a, used);
+  const int pre = prefix_units(a, used);
   const int stretch = div_up(a.batch, kThreads);
-  const int b0 = tid * stretch < a.batch ? tid * stretch : a.batch;
-  const int b1 = b0 + stretch < a.batch ? b0 + stretch : a.batch;
+  const int b0 = min(tid * stretch, a.batch), b1 = min(b0 + stretch, a.batch);
   const bool writer = blockIdx.x == 0;
-  int64_t sum = 0;
+  int sum = 0;
   for (int b = b0; b < b1; ++b) sum += request_units(a, b, writer);
-  int64_t incl = sum;
+  int incl = sum;
   for (int d = 1; d < 32; d <<= 1) {
-    const int64_t x = __shfl_up_sync(0xffffffffu, incl, d);
+    const int x = __shfl_up_sync(0xffffffffu, incl, d);
     if (lane >= d) incl += x;
   }
   if (lane == 31) ctl.scan[warp] = incl;
@@ -735,7 +784,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     ctl.start_units = 0;
   }
   __syncthreads();
-  int64_t before = incl - sum, total = 0;
+  int before = incl - sum, total = 0;
   for (int w = 0; w < kThreads / 32; ++w) {
     if (w < warp) before += ctl.scan[w];
     total += ctl.scan[w];
@@ -743,12 +792,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   const Line line(pre + total, a.grid);
   const bool works = int(blockIdx.x) < line.grid;
   if (works) {
-    const int64_t want = clamp64(line.begin(blockIdx.x) - pre, 0, total);
+    const int want = max(line.begin(blockIdx.x) - pre, 0);
     const bool find = want >= before && want < before + sum;
     if (find || writer) {
-      int64_t u = before;
+      int u = before;
       for (int b = b0; b < b1; ++b) {
-        const int64_t n = request_units(a, b, false);
+        const int n = request_units(a, b, false);
         if (find && want >= u && want < u + n) {
           ctl.start_request = b;
           ctl.start_units = u;
@@ -764,15 +813,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (works) {
     const uint32_t q_at = smem_u32(smem), ring_at = smem_u32(ring);
     if (warp == 0) {
-      if (lane == 0) produce<kWide>(a, ctl, &kmap, &vmap, ring_at);
+      produce(a, ctl, &kmap, &vmap, ring_at);
     } else if (warp == 1) {
-      if (lane == 0) issue_products<kWide>(ctl, q_at, ring_at, tmem);
+      if (lane == 0) issue_products(ctl, q_at, ring_at, tmem);
     } else if (warp == 2) {
       load_queries(a, ctl, q_at);
     } else if (warp == 3) {
       list_pieces(a, ctl, line, blockIdx.x, used, pre);
     } else {
-      softmax_rows<kWide>(a, ctl, ring, tmem);
+      softmax_rows(a, ctl, swap, ring, tmem);
     }
   }
   tmem_fence_before();
@@ -786,85 +835,95 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 // ---------------------------------------------------------------------------
 // Joining the partial results of a row: kGroups x 64 threads a row, four lanes
-// of the head each; the groups take the row's partial results in turn.
+// of the head each; the groups take the row's partial results in turn.  The
+// row's first warp works out where they are.
 // ---------------------------------------------------------------------------
-struct Part {
-  int64_t ml, o;  // offsets into the workspace arrays
+struct RowParts {
+  int cta[2], count[2], in_tile[2];  // prefix and own item: first CTA, CTAs, row of the item
+  int spare;                         // 1: a row of no request
+  int live;                          // 1: this kernel writes the row
+};
+
+__device__ __forceinline__ void find_parts(const AttendArgs& a, int64_t flat, RowParts& to) {
+  const int lane = threadIdx.x & 31;
+  const int used = used_tokens(a);
+  RowParts r{};
+  if (flat < int64_t(a.tokens) * a.q_heads) {
+    const int token = int(flat / a.q_heads), hq = int(flat - int64_t(token) * a.q_heads);
+    const int h = hq / a.group, g = hq - h * a.group;
+    int b = token;  // the row's request: the last that starts at or before the token
+    if (a.query_starts != nullptr) {
+      int lo = 0, hi = a.batch;
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (__ldg(a.query_starts + mid) <= token) lo = mid; else hi = mid;
+      }
+      b = lo;
+    }
+    Request q{0, 0, 0};
+    if (token < used) q = load_request(a, b, false);
+    r.spare = token < q.first || token >= q.first + q.count;
+    if (!r.spare) {
+      const int pre = prefix_units(a, used);
+      const Line line(pre + a.units_before[a.batch], a.grid);
+      auto place = [&](int x, int first, int tiles, int in_tile) {
+        r.in_tile[x] = in_tile;
+        if (tiles == 0) return;
+        r.cta[x] = line.cta_of(first);
+        r.count[x] = line.cta_of(first + tiles - 1) - r.cta[x] + 1;
+      };
+      if (pre > 0) {
+        const int packed = token * a.group + g, key_tiles = div_up(a.prefix_len, kKeys);
+        place(0, (h * div_up(used * a.group, kRows) + packed / kRows) * key_tiles, key_tiles, packed % kRows);
+      }
+      const int packed = (token - q.first) * a.group + g, rt = packed / kRows;
+      int u = 0;  // tiles of the request's earlier rows
+      for (int x = lane; x < rt; x += 32) u += q.tiles(a.group, x);
+      u = __reduce_add_sync(0xffffffffu, u);
+      const int t = q.tiles(a.group, rt);
+      place(1, pre + a.units_before[b] + u * a.k_heads + h * t, t, packed % kRows);
+      r.live = pre > 0 || r.count[1] != 1;  // otherwise the first kernel wrote the row
+    } else {
+      r.live = a.fill;
+    }
+  }
+  if (lane == 0) to = r;
+}
+
+// Running join of partial results (m, l, four lanes of O).
+struct Joined {
+  float m = -INFINITY, l = 0.0f;
+  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  __device__ __forceinline__ void add(float2 ml, float4 v) {
+    if (ml.x == -INFINITY && ml.y == 0.0f) return;  // saw no key
+    const float top = fmaxf(m, ml.x);
+    const float base = top == -INFINITY ? 0.0f : top;
+    const float f0 = exp2_approx(m - base), f1 = exp2_approx(ml.x - base);
+    l = l * f0 + ml.y * f1;
+    o.x = o.x * f0 + v.x * f1;
+    o.y = o.y * f0 + v.y * f1;
+    o.z = o.z * f0 + v.z * f1;
+    o.w = o.w * f0 + v.w * f1;
+    m = top;
+  }
 };
 
 template <int kGroups>
 __global__ void __launch_bounds__(256) rope_attend_join_kernel(const __grid_constant__ AttendArgs a) {
   constexpr int kRowThreads = 64 * kGroups, kRowsPerCta = 256 / kRowThreads;
+  __shared__ RowParts parts[kRowsPerCta];
   __shared__ float4 s_o[kGroups > 1 ? 256 : 1];
-  __shared__ float2 s_ml[kGroups > 1 ? kGroups : 1];
-  const int part = threadIdx.x % kRowThreads;
+  __shared__ float2 s_ml[kGroups];
+  const int in_cta = threadIdx.x / kRowThreads, part = threadIdx.x % kRowThreads;
   const int grp = part >> 6, d4 = part & 63;
-  const int64_t flat = int64_t(blockIdx.x) * kRowsPerCta + threadIdx.x / kRowThreads;
+  const int64_t flat = int64_t(blockIdx.x) * kRowsPerCta + in_cta;
   pdl_enter();
-  const int used = used_tokens(a);
+  if (part < 32) find_parts(a, flat, parts[in_cta]);
+  __syncthreads();
+  const RowParts r = parts[in_cta];
   const int64_t rows = int64_t(a.tokens) * a.q_heads;
-  bool live = flat < rows;
-  const int token = live ? int(flat / a.q_heads) : 0;
-  const int hq = live ? int(flat - int64_t(token) * a.q_heads) : 0;
-  const int h = hq / a.group, g = hq - h * a.group;
-  // the row's request
-  int b = token;
-  if (a.query_starts != nullptr) {
-    int lo = 0, hi = a.batch;  // the last request that starts at or before the token
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (__ldg(a.query_starts + mid) <= token) lo = mid; else hi = mid;
-    }
-    b = lo;
-  }
-  Request r{0, 0, 0};
-  if (live && token < used) r = load_request(a, b, false);
-  const bool spare = live && (token < r.first || token >= r.first + r.count);  // a row of no request
-  if (spare) live = false;
-  const int64_t pre = prefix_units(a, used);
-  const int64_t total = a.units_before[a.batch];
-  const Line line(pre + total, a.grid);
-  // the two items of the row: [first unit, past the last), and its row in each
-  int64_t lo[2] = {0, 0}, hi[2] = {0, 0};
-  int in_tile[2] = {0, 0};
-  if (live) {
-    if (pre > 0) {
-      const int packed = token * a.group + g;
-      const int key_tiles = div_up(a.prefix_len, kKeys);
-      lo[0] = (int64_t(h) * div_up(used * a.group, kRows) + packed / kRows) * key_tiles;
-      hi[0] = lo[0] + key_tiles;
-      in_tile[0] = packed % kRows;
-    }
-    const int packed = (token - r.first) * a.group + g;
-    const int rt = packed / kRows;
-    int64_t u = pre + a.units_before[b];
-    for (int x = 0; x < rt; ++x) u += int64_t(r.tiles(a.group, x)) * a.k_heads;
-    const int t = r.tiles(a.group, rt);
-    lo[1] = u + int64_t(h) * t;
-    hi[1] = lo[1] + t;
-    in_tile[1] = packed % kRows;
-  }
-  int c0[2] = {0, 0}, n[2] = {0, 0};
-  for (int x = 0; x < 2; ++x) {
-    if (hi[x] == lo[x]) continue;
-    c0[x] = line.cta_of(lo[x]);
-    n[x] = line.cta_of(hi[x] - 1) - c0[x] + 1;
-  }
-  // written whole by the first kernel
-  if (pre == 0 && n[0] + n[1] == 1) live = false;
-  auto where = [&](int i) {
-    const int x = i >= n[0];
-    if (n[x] == 1) {
-      const int64_t at = int64_t(x) * rows + flat;
-      return Part{int64_t(a.part_ml - a.slot_ml) + at * 2, int64_t(a.part_o - a.slot_ml) + at * kHeadDim};
-    }
-    const int c = c0[x] + (x ? i - n[0] : i);
-    const int64_t at = int64_t(2 * c + (lo[x] < line.begin(c) ? 0 : 1)) * a.slot_rows + in_tile[x];
-    return Part{at * 2, int64_t(a.slot_o - a.slot_ml) + at * kHeadDim};
-  };
-  float m = -INFINITY, l = 0.0f;
-  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  const int count = live ? n[0] + n[1] : 0;
+  const int count = r.live ? r.count[0] + r.count[1] : 0;
+  Joined sum;
   constexpr int kUnroll = 4;
   for (int i0 = grp; i0 < count; i0 += kGroups * kUnroll) {
     float2 ml[kUnroll];
@@ -875,52 +934,43 @@ __global__ void __launch_bounds__(256) rope_attend_join_kernel(const __grid_cons
       ml[x] = make_float2(-INFINITY, 0.0f);
       v[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       if (i < count) {
-        const Part p = where(i);
-        ml[x] = *reinterpret_cast<const float2*>(a.slot_ml + p.ml);
-        v[x] = *reinterpret_cast<const float4*>(a.slot_ml + p.o + d4 * 4);
+        const bool own = i >= r.count[0];
+        const int at = own ? i - r.count[0] : i;
+        const float* pml;
+        const float* po;
+        if ((own ? r.count[1] : r.count[0]) == 1) {  // the whole item's rows
+          const int64_t place = (own ? rows : 0) + flat;
+          pml = a.part_ml + place * 2;
+          po = a.part_o + place * kHeadDim;
+        } else {  // a CTA's first piece where the item began earlier, else its last
+          const int slot = 2 * ((own ? r.cta[1] : r.cta[0]) + at) + (at == 0);
+          const int64_t place = int64_t(slot) * a.slot_rows + (own ? r.in_tile[1] : r.in_tile[0]);
+          pml = a.slot_ml + place * 2;
+          po = a.slot_o + place * kHeadDim;
+        }
+        ml[x] = *reinterpret_cast<const float2*>(pml);
+        v[x] = *reinterpret_cast<const float4*>(po + d4 * 4);
       }
     }
 #pragma unroll
-    for (int x = 0; x < kUnroll; ++x) {
-      if (ml[x].x == -INFINITY && ml[x].y == 0.0f) continue;  // saw no key
-      const float top = fmaxf(m, ml[x].x);
-      const float base = top == -INFINITY ? 0.0f : top;
-      const float f0 = exp2_approx(m - base), f1 = exp2_approx(ml[x].x - base);
-      l = l * f0 + ml[x].y * f1;
-      o.x = o.x * f0 + v[x].x * f1;
-      o.y = o.y * f0 + v[x].y * f1;
-      o.z = o.z * f0 + v[x].z * f1;
-      o.w = o.w * f0 + v[x].w * f1;
-      m = top;
-    }
+    for (int x = 0; x < kUnroll; ++x) sum.add(ml[x], v[x]);
   }
   if (kGroups > 1) {
-    s_o[threadIdx.x] = o;
-    if (d4 == 0) s_ml[grp] = make_float2(m, l);
+    s_o[threadIdx.x] = sum.o;
+    if (d4 == 0) s_ml[grp] = make_float2(sum.m, sum.l);
     __syncthreads();
     if (grp > 0) return;
-    for (int x = 1; x < kGroups; ++x) {
-      const float2 ml = s_ml[x];
-      if (ml.x == -INFINITY && ml.y == 0.0f) continue;
-      const float4 v = s_o[x * 64 + d4];
-      const float top = fmaxf(m, ml.x);
-      const float base = top == -INFINITY ? 0.0f : top;
-      const float f0 = exp2_approx(m - base), f1 = exp2_approx(ml.x - base);
-      l = l * f0 + ml.y * f1;
-      o.x = o.x * f0 + v.x * f1;
-      o.y = o.y * f0 + v.y * f1;
-      o.z = o.z * f0 + v.z * f1;
-      o.w = o.w * f0 + v.w * f1;
-      m = top;
-    }
+#pragma unroll
+    for (int x = 1; x < kGroups; ++x) sum.add(s_ml[x], s_o[x * 64 + d4]);
   }
-  if (!live && !(spare && a.fill)) return;
-  const bool none = l == 0.0f;
-  const float inv = none ? 0.0f : 1.0f / l;
+  if (!r.live) return;
+  const int token = int(flat / a.q_heads), hq = int(flat - int64_t(token) * a.q_heads);
+  const bool none = sum.l == 0.0f;
+  const float inv = none ? 0.0f : 1.0f / sum.l;
   uint2 packed = make_uint2(0, 0);
-  if (!none) packed = make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv));
+  if (!none) packed = make_uint2(pack_bf16x2(sum.o.x * inv, sum.o.y * inv), pack_bf16x2(sum.o.z * inv, sum.o.w * inv));
   *reinterpret_cast<uint2*>(a.out + token * a.out_token + hq * a.out_head + d4 * 4) = packed;
-  if (a.lse != nullptr && d4 == 0) a.lse[flat] = none ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+  if (a.lse != nullptr && d4 == 0) a.lse[flat] = none ? -INFINITY : (sum.m + log2f(sum.l)) * 0.6931471805599453f;
 }
 
 // ---------------------------------------------------------------------------
@@ -939,7 +989,7 @@ Workspace attend_workspace(int64_t tokens, int64_t batch, int64_t q_heads, int64
   const int64_t parts = prefix_len > 0 ? 2 * tokens * q_heads : 0;
   Workspace w;
   w.units = 0;
-  w.slot_ml = up((batch + 1) * 8);
+  w.slot_ml = up((batch + 1) * 4);
   w.slot_o = w.slot_ml + up(slots * 8);
   w.part_ml = w.slot_o + up(slots * kHeadDim * 4);
   w.part_o = w.part_ml + up(parts * 8);
@@ -947,18 +997,19 @@ Workspace attend_workspace(int64_t tokens, int64_t batch, int64_t q_heads, int64
   return w;
 }
 
-// Tensor map of a cache as {64 lanes, slot, chunk of 64 lanes, head, block}.
+// Tensor map of a cache as {256 lanes, slot, head, block}, boxes of 64 lanes
+// and `box_keys` slots.
 bool encode_cache_map(CUtensorMap& map, const void* base, int64_t blocks, int64_t block_size, int64_t heads,
                       const int64_t* strides, int box_keys) {
   const PFN_cuTensorMapEncodeTiled_v12000 encode = tensor_map_encoder();
   if (encode == nullptr) return false;
-  const cuuint64_t dim[5] = {64, cuuint64_t(block_size), 4, cuuint64_t(heads), cuuint64_t(blocks)};
+  const cuuint64_t dim[4] = {kHeadDim, cuuint64_t(block_size), cuuint64_t(heads), cuuint64_t(blocks)};
   // the stride of a dimension of one is not used, but has to be one
   auto step = [](int64_t extent, int64_t stride) { return cuuint64_t(extent > 1 ? stride : kHeadDim) * 2; };
-  const cuuint64_t stride[4] = {step(block_size, strides[1]), 128, step(heads, strides[2]), step(blocks, strides[0])};
-  const cuuint32_t box[5] = {64, cuuint32_t(box_keys), 4, 1, 1};
-  const cuuint32_t unit[5] = {1, 1, 1, 1, 1};
-  return encode(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(base), dim, stride, box, unit,
+  const cuuint64_t stride[3] = {step(block_size, strides[1]), step(heads, strides[2]), step(blocks, strides[0])};
+  const cuuint32_t box[4] = {64, cuuint32_t(box_keys), 1, 1};
+  const cuuint32_t unit[4] = {1, 1, 1, 1};
+  return encode(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dim, stride, box, unit,
                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -969,14 +1020,13 @@ bool attend_sizes_ok(int64_t tokens, int64_t batch, int64_t q_heads, int64_t k_h
   return q_heads <= kMaxItems && tokens <= kMaxItems / q_heads;
 }
 
-template <bool kWide>
 int launch_attend(const CUtensorMap& kmap, const CUtensorMap& vmap, const AttendArgs& a, cudaStream_t stream) {
-  if (cudaFuncSetAttribute(rope_attend_kernel<kWide>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes) !=
+  if (cudaFuncSetAttribute(rope_attend_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes) !=
       cudaSuccess) {
     cudaGetLastError();
     return WELM_ROPE_ERR_CUDA;
   }
-  int rc = launch(rope_attend_kernel<kWide>, unsigned(a.grid), kThreads, kSmemBytes, stream, kmap, vmap, a);
+  int rc = launch(rope_attend_kernel, unsigned(a.grid), kThreads, kSmemBytes, stream, kmap, vmap, a);
   if (rc != WELM_ROPE_OK) return rc;
   const int64_t rows = int64_t(a.tokens) * a.q_heads;
   if (rows <= 1024) return launch(rope_attend_join_kernel<4>, unsigned(rows), 256, 0, stream, a);
@@ -1013,6 +1063,11 @@ int welm_rope_attend(const void* q, void* out, float* lse, const void* key_cache
       table_width > kMaxItems / block_size)
     return WELM_ROPE_ERR_BAD_SIZE;
   if (!query_starts && n_tokens != batch_size) return WELM_ROPE_ERR_BAD_SIZE;
+  // tiles are counted in 32 bits
+  const __int128 row_tiles = (n_tokens * (num_q_heads / num_k_heads) + kRows - 1) / kRows;
+  if ((row_tiles * ((prefix_len + kKeys - 1) / kKeys) +
+       (row_tiles + batch_size) * ((table_width * block_size + kKeys - 1) / kKeys)) * num_k_heads >= INT32_MAX)
+    return WELM_ROPE_ERR_BAD_SIZE;
   if (!(scale > 0.0f) || scale > 3.0e38f || (fill_unused != 0 && fill_unused != 1)) return WELM_ROPE_ERR_BAD_MODE;
   if (n_tokens == 0 || batch_size == 0) return WELM_ROPE_OK;
   if (block_size % 8 != 0 || num_blocks == 0) return WELM_ROPE_ERR_BAD_SIZE;
@@ -1042,8 +1097,8 @@ int welm_rope_attend(const void* q, void* out, float* lse, const void* key_cache
   const int64_t group = num_q_heads / num_k_heads;
   const Workspace w = attend_workspace(n_tokens, batch_size, num_q_heads, group, prefix_len, sms);
   if (workspace_bytes < w.bytes) return WELM_ROPE_ERR_CAPACITY;
-  const bool wide = block_size % kKeys == 0;
-  const int box = wide ? kKeys : 8;
+  int box = 8;
+  while (box < kKeys && block_size % (2 * box) == 0) box *= 2;
   CUtensorMap kmap, vmap;
   if (!encode_cache_map(kmap, key_cache, num_blocks, block_size, num_k_heads, key_cache_strides, box) ||
       !encode_cache_map(vmap, value_cache, num_blocks, block_size, num_k_heads, value_cache_strides, box))
@@ -1070,19 +1125,20 @@ int welm_rope_attend(const void* q, void* out, float* lse, const void* key_cache
   a.max_len = int32_t(table_width * block_size);
   a.block_size = int32_t(block_size);
   a.num_blocks = int32_t(num_blocks);
+  a.box_keys = box;
   a.slot_rows = int32_t(n_tokens * group < kRows ? n_tokens * group : kRows);
   a.grid = sms;
   a.fill = int32_t(fill_unused);
   a.scale = scale * 1.4426950408889634f;
   char* base = static_cast<char*>(workspace);
-  a.units_before = reinterpret_cast<int64_t*>(base + w.units);
+  a.units_before = reinterpret_cast<int32_t*>(base + w.units);
   a.slot_ml = reinterpret_cast<float*>(base + w.slot_ml);
   a.slot_o = reinterpret_cast<float*>(base + w.slot_o);
   a.part_ml = reinterpret_cast<float*>(base + w.part_ml);
   a.part_o = reinterpret_cast<float*>(base + w.part_o);
   a.status = device_status;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return wide ? launch_attend<true>(kmap, vmap, a, s) : launch_attend<false>(kmap, vmap, a, s);
+  return launch_attend(kmap, vmap, a, s);
 }
 
 }  // extern "C"

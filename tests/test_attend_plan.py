@@ -1,5 +1,5 @@
 """CPU checks of the attention kernels' work division, restated from
-rope_attend.cu: the pieces that the CTAs list cover every 64-key tile of every
+rope_attend.cu: the pieces that the CTAs list cover every 128-key tile of every
 item once, every workspace index lies inside its array, and the join kernel
 finds exactly the pieces that hold a row's partial results."""
 
@@ -9,7 +9,7 @@ import random
 
 import pytest
 
-ROWS, KEYS = 128, 64
+ROWS = KEYS = 128
 
 
 def div_up(a, b):
@@ -44,10 +44,13 @@ class Plan:
         return div_up(self.seen(b, rt), KEYS)
 
     def begin(self, c):
-        return self.units * c // self.grid
+        each, more = divmod(self.units, self.grid)
+        return each * c + min(c, more)
 
     def cta_of(self, u):
-        return ((u + 1) * self.grid - 1) // self.units
+        each, more = divmod(self.units, self.grid)
+        longer = more * (each + 1)
+        return u // (each + 1) if u < longer else more + (u - longer) // each
 
     def pieces(self, cta):
         """(item, first tile, tiles, destination) in the order of list_pieces."""
@@ -101,7 +104,7 @@ class Plan:
             if c0 == c1:
                 found.append(("part", x, token * self.q_heads + hq) if self.pre else None)
             else:
-                found += [("slot", 2 * c + (0 if lo < self.begin(c) else 1), row) for c in range(c0, c1 + 1)]
+                found += [("slot", 2 * c + (c == c0), row) for c in range(c0, c1 + 1)]
         return None if found == [None] else found
 
 

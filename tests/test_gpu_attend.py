@@ -83,14 +83,14 @@ def agree(batch, got, want=None):
     assert (out[:n][none] == 0).all()
 
 
-@pytest.mark.parametrize("lens", [[1], [63], [64], [65], [300], [0], [5000], [0, 1, 64, 129, 1000], [17] * 150])
+@pytest.mark.parametrize("lens", [[1], [63], [64], [65], [127], [128], [129], [300], [0], [5000], [0, 1, 64, 129, 1000], [17] * 150])
 def test_decode_without_prefix(lens):
     batch = Batch(lens)
     agree(batch, batch.run())
     assert batch.status.item() == 0
 
 
-@pytest.mark.parametrize("prefix", [1, 63, 64, 65, 1000, 4097])
+@pytest.mark.parametrize("prefix", [1, 63, 64, 65, 127, 128, 129, 1000, 4097])
 @pytest.mark.parametrize("lens", [[1], [0], [0, 1, 64, 129, 700], [30] * 40])
 def test_decode_with_prefix(prefix, lens):
     batch = Batch(lens, prefix=prefix)
