@@ -431,7 +431,7 @@ int welm_rope_kv_append(void* q, const void* k, const void* v, const int64_t* po
  *
  * The call allocates nothing: `workspace` is device memory of at least the
  * bytes that welm_rope_attend_workspace gives for the same sizes on the current
- * device.  It needs no initial contents and keeps nothing for the next call,
+ * device, 32-byte aligned.  It needs no initial contents and keeps nothing for the next call,
  * but belongs to one call at a time: calls that may overlap on the GPU, replays
  * of two captured graphs among them, need a workspace each.
  */

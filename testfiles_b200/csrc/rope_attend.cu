@@ -51,6 +51,22 @@ constexpr uint32_t kColS = 0, kColO = 256;  // TMEM columns: S (and P) of even a
 constexpr long long kWaitClocks = 1ll << 32;  // about two seconds
 constexpr float kRescaleStep = 8.0f;   // O is rescaled when the maximum grows by more than 2^8
 
+// Division by a number that the host knows: x / d for 0 <= x < 2^31 as one
+// multiplication and a shift.  mul = ceil(2^(31 + L) / d) with L = ceil(log2 d)
+// is less than d <= 2^L over 2^(31 + L) / d, too little to reach the next quotient.
+struct Divisor {
+  uint32_t mul = 0;
+  int32_t shift = 0, d = 1;
+  Divisor() = default;
+  explicit Divisor(int64_t by) : d(int32_t(by)) {
+    int log = 0;
+    while ((int64_t(1) << log) < by) ++log;
+    shift = 31 + log;
+    mul = uint32_t(((uint64_t(1) << shift) + uint64_t(by) - 1) / uint64_t(by));
+  }
+  __device__ __forceinline__ int of(int x) const { return int((uint64_t(uint32_t(x)) * mul) >> shift); }
+};
+
 struct AttendArgs {
   const uint16_t* q;
   uint16_t* out;
@@ -62,6 +78,7 @@ struct AttendArgs {
   const int64_t* seq_lens;
   const int64_t* query_starts;  // may be null: one token a request
   int32_t tokens, batch, q_heads, k_heads, group;
+  Divisor by_group, by_block, by_q_heads;
   int32_t prefix_len, max_len;  // max_len: keys that a row of block_table can name
   int32_t block_size, num_blocks;
   int32_t box_keys;             // keys of one TMA box: a power of two that divides block_size
@@ -70,10 +87,12 @@ struct AttendArgs {
   int32_t fill;                 // 1: rows of no request become zeros
   float scale;                  // times log2(e)
   int32_t* units_before;        // [batch + 1] tiles of the items before each request
+  // Partial results.  O is laid out [32][rows][8 lanes]: the threads of a warp,
+  // a row each, then write (and a row's reader reads) whole 32-byte sectors.
   float* slot_ml;               // [2 grid][slot_rows][2]
-  float* slot_o;                // [2 grid][slot_rows][256]
-  float* part_ml;               // [2][tokens * q_heads][2]: whole items' rows, prefix and own
-  float* part_o;                // [2][tokens * q_heads][256]
+  float* slot_o;                // [2 grid][32][slot_rows][8]
+  float* part_ml;               // [2][k_heads * tokens * group][2]: whole items' rows, prefix and own
+  float* part_o;                // [2][32][k_heads * tokens * group][8]
   int32_t* status;
 };
 
@@ -86,15 +105,32 @@ __device__ __forceinline__ int64_t clamp64(int64_t v, int64_t lo, int64_t hi) {
 // them at the last of `len` keys.
 struct Request {
   int first, count, len;
-  __device__ __forceinline__ int row_tiles(int group) const { return div_up(count * group, kRows); }
+  __device__ __forceinline__ int row_tiles(const AttendArgs& a) const { return div_up(count * a.group, kRows); }
   // Keys that the last row of row tile rt sees: every row of it sees at most these.
-  __device__ __forceinline__ int seen(int group, int rt) const {
-    int last = (rt * kRows + kRows - 1) / group;
-    if (last > count - 1) last = count - 1;
-    const int keys = len - count + last + 1;
-    return keys < 0 ? 0 : keys;
+  __device__ __forceinline__ int seen(const AttendArgs& a, int rt) const {
+    const int last = min(a.by_group.of(rt * kRows + kRows - 1), count - 1);
+    return max(len - count + last + 1, 0);
   }
-  __device__ __forceinline__ int tiles(int group, int rt) const { return div_up(seen(group, rt), kKeys); }
+  __device__ __forceinline__ int tiles(const AttendArgs& a, int rt) const { return div_up(seen(a, rt), kKeys); }
+  // Key tiles of one head's row tiles before rt, rt below row_tiles.  Row tile x
+  // (not the last) has ceil((b + floor((128 x + 127) / G)) / 128) of them, b =
+  // len - count + 1; nested floors make that floor((x + c) / G) with c = floor((127
+  // + G (b + 127)) / 128), or none if negative, and sums of floor(i / G) are
+  // triangular numbers.
+  __device__ __forceinline__ int tiles_before(const AttendArgs& a, int rt) const {
+    if (rt == 0) return 0;
+    const int c = int((127 + int64_t(a.group) * (len - count + 128)) >> 7);
+    auto sum = [&](int x) {  // of floor(i / G) over 0 <= i < x
+      if (x <= 0) return 0;
+      const int q = a.by_group.of(x);
+      return int(int64_t(a.group) * q * (q - 1) / 2) + q * (x - q * a.group);
+    };
+    return sum(rt + c) - sum(c);
+  }
+  __device__ __forceinline__ int all_tiles(const AttendArgs& a) const {
+    const int n = row_tiles(a);
+    return n == 0 ? 0 : tiles_before(a, n - 1) + div_up(len, kKeys);
+  }
 };
 
 __device__ __forceinline__ Request load_request(const AttendArgs& a, int b, bool tell) {
@@ -238,6 +274,15 @@ __device__ __forceinline__ void mma_commit(uint64_t* bar) {
                : "memory");
 }
 
+// One lane of a whole warp.  What the lane's products take is computed by the
+// warp, alike in every lane, so that it can stay in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(one));
+  return one != 0;
+}
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
+
 __device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
@@ -282,18 +327,15 @@ __device__ __forceinline__ void store8f(float* p, const float* v) {
 // The roles.
 // ---------------------------------------------------------------------------
 // Every warp that walks the pieces: next piece, or false at the end (or when
-// the CTA has given up).  Called by whole warps or by one thread.
+// the CTA has given up).
 struct PieceReader {
   int n = 0;
-  template <bool kWarp>
   __device__ __forceinline__ bool next(Control& ctl, Piece& p) {
     const int s = n % kPieces;
-    bool ok = mbar_wait(ctl, &ctl.piece_full[s], (n / kPieces) & 1);
-    if (kWarp) ok = __all_sync(0xffffffffu, ok);
-    if (!ok) return false;
+    if (!__all_sync(0xffffffffu, mbar_wait(ctl, &ctl.piece_full[s], (n / kPieces) & 1))) return false;
     p = ctl.piece[s];
-    if (kWarp) __syncwarp();
-    if (!kWarp || (threadIdx.x & 31) == 0) mbar_arrive(&ctl.piece_empty[s]);
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(&ctl.piece_empty[s]);
     ++n;
     return p.tiles > 0;
   }
@@ -344,15 +386,24 @@ __device__ void list_pieces(const AttendArgs& a, Control& ctl, const Line& line,
     for (int i = 0; i < 32 && u < end && b0 + i < a.batch; ++i) {
       const Request r{__shfl_sync(0xffffffffu, mine.first, i), __shfl_sync(0xffffffffu, mine.count, i),
                       __shfl_sync(0xffffffffu, mine.len, i)};
-      const int rts = r.row_tiles(a.group);
-      for (int rt = 0; rt < rts && u < end; ++rt) {
-        const int t = r.tiles(a.group, rt);
+      const int rts = r.row_tiles(a);
+      int rt = 0;
+      if (rts > 1 && u > base) {  // the last row tile that begins at or before u
+        int hi = rts;
+        while (hi - rt > 1) {
+          const int mid = (rt + hi) >> 1;
+          if (base + a.k_heads * r.tiles_before(a, mid) <= u) rt = mid; else hi = mid;
+        }
+        base += a.k_heads * r.tiles_before(a, rt);
+      }
+      for (; rt < rts && u < end; ++rt) {
+        const int t = r.tiles(a, rt);
         for (int h = 0; h < a.k_heads && u < end; ++h, base += t) {
           if (u >= base + t) continue;
           Piece p;
           p.first_tile = u - base;
           p.tiles = min(end - u, t - p.first_tile);
-          p.keys = r.seen(a.group, rt);
+          p.keys = r.seen(a, rt);
           p.head = h;
           p.row0 = rt * kRows;
           p.rows = min(r.count * a.group - p.row0, kRows);
@@ -389,7 +440,7 @@ __device__ void produce(const AttendArgs& a, Control& ctl, const CUtensorMap* km
   Piece p;
   uint32_t n = 0;  // half tiles put into the ring
   bool ok = true;
-  while (ok && pieces.next<true>(ctl, p)) {
+  while (ok && pieces.next(ctl, p)) {
     const int32_t* table = p.own ? a.block_table + p.table_row * a.table_stride : a.prefix_table;
     // Block and place of this lane's box in tile j; behind the keys the block
     // past the cache, whose box is filled with zeros.
@@ -398,7 +449,7 @@ __device__ void produce(const AttendArgs& a, Control& ctl, const CUtensorMap* km
       block = a.num_blocks;
       place = 0;
       if (j >= p.tiles || lane >= boxes || key >= p.keys) return;
-      const int page = key / a.block_size;
+      const int page = a.by_block.of(key);
       place = key - page * a.block_size;
       block = __ldg(table + page);
       if (block < 0 || block >= a.num_blocks) {
@@ -450,90 +501,117 @@ __device__ void produce(const AttendArgs& a, Control& ctl, const CUtensorMap* km
 
 __device__ void issue_products(Control& ctl, uint32_t q, uint32_t ring, uint32_t tmem) {
   constexpr uint32_t kIdescS = instr_desc(kKeys, false), kIdescO = instr_desc(kHalfLanes, true);
+  constexpr uint32_t kFull = 0xffffffffu;
+  const uint64_t q_desc = operand_desc(q, 16, 1024);
   PieceReader pieces;
   Piece p;
   uint32_t base = 0;   // ring entries before this piece, in whole tiles of K or V
   uint32_t tile = 0;   // tiles before this piece
-  for (uint32_t np = 0; pieces.next<false>(ctl, p); ++np) {
-    if (!mbar_wait(ctl, &ctl.q_full, np & 1)) break;
+  for (uint32_t np = 0; pieces.next(ctl, p); ++np) {
+    if (!__all_sync(kFull, mbar_wait(ctl, &ctl.q_full, np & 1))) break;
     // the Q rows came by ordinary asynchronous copies
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    const int tiles = int(uniform(p.tiles));
     bool ok = true;
-    for (int j = 0; j <= p.tiles && ok; ++j) {
-      if (j < p.tiles) {  // S(j) = Q K(j)^T, once P(j - 2) in its place has been used
-        const uint32_t t = tile + j, buf = t & 1;
-        ok = t < 2 || mbar_wait(ctl, &ctl.pv_done[buf], ((t >> 1) & 1) ^ 1);
+    // Both halves of a tile of K or V; what the ring already holds is waited for
+    // before what the products before it decide.
+    auto landed = [&](uint32_t e) {
+      return mbar_wait(ctl, &ctl.full[e % kStages], (e / kStages) & 1) &&
+             mbar_wait(ctl, &ctl.full[(e + 1) % kStages], ((e + 1) / kStages) & 1);
+    };
+    for (int j = 0; j <= tiles; ++j) {
+      if (j < tiles) {  // S(j) = Q K(j)^T, once P(j - 2) in its place has been used
+        const uint32_t t = tile + j, buf = t & 1, e = 2 * (base + ring_k(j));
+        ok = landed(e) && (t < 2 || mbar_wait(ctl, &ctl.pv_done[buf], ((t >> 1) & 1) ^ 1));
+        if (!__all_sync(kFull, ok)) break;
+        tmem_fence_after();
+        const uint32_t s0 = uniform(e % kStages), s1 = uniform((e + 1) % kStages);
+        const uint64_t k_desc[2] = {operand_desc(ring + s0 * kStageBytes, 16, 1024),
+                                    operand_desc(ring + s1 * kStageBytes, 16, 1024)};
+        const uint32_t d = tmem + kColS + buf * kKeys;
+        if (elect_one()) {
 #pragma unroll
-        for (int half = 0; half < 2 && ok; ++half) {
-          const uint32_t e = 2 * (base + ring_k(j)) + half, s = e % kStages;
-          ok = mbar_wait(ctl, &ctl.full[s], (e / kStages) & 1);
-          if (!ok) break;
-          tmem_fence_after();
-          const uint32_t k = ring + s * kStageBytes;
+          for (int half = 0; half < 2; ++half) {
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
+            for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              mma_ss(tmem + kColS + buf * kKeys, operand_desc(q + (2 * half + c) * kQChunkBytes + kk * 32, 16, 1024),
-                     operand_desc(k + c * kChunkBytes + kk * 32, 16, 1024), kIdescS, half + c + kk > 0);
-          mma_commit(&ctl.empty[s]);
+              for (int kk = 0; kk < 4; ++kk)
+                mma_ss(d, q_desc + (((2 * half + c) * kQChunkBytes + kk * 32) >> 4),
+                       k_desc[half] + ((c * kChunkBytes + kk * 32) >> 4), kIdescS, half + c + kk > 0);
+            mma_commit(&ctl.empty[half == 0 ? s0 : s1]);
+          }
+          mma_commit(&ctl.s_full[buf]);
+          if (j == tiles - 1) mma_commit(&ctl.q_empty);
         }
-        if (!ok) break;
-        mma_commit(&ctl.s_full[buf]);
-        if (j == p.tiles - 1) mma_commit(&ctl.q_empty);
+        __syncwarp();
       }
       if (j > 0) {  // O += P(j-1) V(j-1)
         const int jv = j - 1;
-        const uint32_t t = tile + jv, buf = t & 1;
-        ok = mbar_wait(ctl, &ctl.p_full[buf], (t >> 1) & 1) &&
-             (jv > 0 || mbar_wait(ctl, &ctl.o_free, (np & 1) ^ 1));
+        const uint32_t t = tile + jv, buf = t & 1, e = 2 * (base + ring_v(jv, tiles));
+        ok = landed(e) && (jv > 0 || mbar_wait(ctl, &ctl.o_free, (np & 1) ^ 1)) &&
+             mbar_wait(ctl, &ctl.p_full[buf], (t >> 1) & 1);
+        if (!__all_sync(kFull, ok)) break;
+        tmem_fence_after();
+        const uint32_t s0 = uniform(e % kStages), s1 = uniform((e + 1) % kStages);
+        const uint64_t v_desc[2] = {operand_desc(ring + s0 * kStageBytes, kChunkBytes, 1024),
+                                    operand_desc(ring + s1 * kStageBytes, kChunkBytes, 1024)};
+        // P: keys 0..63 in the first 32 columns of S, keys 64..127 in those from column 64
+        const uint32_t p_at = tmem + kColS + buf * kKeys;
+        if (elect_one()) {
 #pragma unroll
-        for (int half = 0; half < 2 && ok; ++half) {
-          const uint32_t e = 2 * (base + ring_v(jv, p.tiles)) + half, s = e % kStages;
-          ok = mbar_wait(ctl, &ctl.full[s], (e / kStages) & 1);
-          if (!ok) break;
-          tmem_fence_after();
-          const uint32_t v = ring + s * kStageBytes;
-          // P: keys 0..63 in the first 32 columns of S, keys 64..127 in those from column 64
+          for (int half = 0; half < 2; ++half) {
 #pragma unroll
-          for (int ks = 0; ks < kKeys / 16; ++ks)
-            mma_ts(tmem + kColO + half * kHalfLanes, tmem + kColS + buf * kKeys + (ks >> 2) * 64 + (ks & 3) * 8,
-                   operand_desc(v + ks * 16 * 128, kChunkBytes, 1024), kIdescO, jv > 0 || ks > 0);
-          mma_commit(&ctl.empty[s]);
+            for (int ks = 0; ks < kKeys / 16; ++ks)
+              mma_ts(tmem + kColO + half * kHalfLanes, p_at + (ks >> 2) * 64 + (ks & 3) * 8,
+                     v_desc[half] + ((ks * 16 * 128) >> 4), kIdescO, jv > 0 || ks > 0);
+            mma_commit(&ctl.empty[half == 0 ? s0 : s1]);
+          }
+          mma_commit(&ctl.pv_done[buf]);
         }
-        if (!ok) break;
-        mma_commit(&ctl.pv_done[buf]);
+        __syncwarp();
       }
     }
+    ok = __all_sync(kFull, ok);
     if (!ok) break;
-    base += 2 * p.tiles;
-    tile += p.tiles;
+    base += 2 * tiles;
+    tile += tiles;
   }
   // no product may outlive the TMEM or the shared memory it works on
-  mma_commit(&ctl.drained);
+  if (elect_one()) mma_commit(&ctl.drained);
+  __syncwarp();
   const long long t0 = clock64();
   while (!mbar_poll(&ctl.drained, 0) && clock64() - t0 < kWaitClocks) {
   }
 }
 
 // Q rows of each piece: one row of 512 bytes a warp instruction, into the
-// 128-byte swizzle that the products read.  Rows past the item's stay as they
-// are: a row of S and O depends on its own Q row alone.
+// 128-byte swizzle that the products read.  Each lane works out the addresses
+// of four rows beforehand.  Rows past the item's stay as they are: a row of S
+// and O depends on its own Q row alone.
 __device__ void load_queries(const AttendArgs& a, Control& ctl, uint32_t q) {
   const int lane = threadIdx.x & 31;
   PieceReader pieces;
   Piece p;
-  for (uint32_t np = 0; pieces.next<true>(ctl, p); ++np) {
+  for (uint32_t np = 0; pieces.next(ctl, p); ++np) {
+    const uint16_t* mine[kRows / 32];
+#pragma unroll
+    for (int i = 0; i < kRows / 32; ++i) {
+      const int in_item = p.row0 + min(i * 32 + lane, p.rows - 1);
+      const int tok = a.by_group.of(in_item);
+      mine[i] = a.q + (p.first + tok) * a.q_token + (p.head * a.group + in_item - tok * a.group) * a.q_head;
+    }
     if (!__all_sync(0xffffffffu, mbar_wait(ctl, &ctl.q_empty, (np & 1) ^ 1))) break;
-    int tok = p.row0 / a.group;
-    int g = p.row0 - tok * a.group;
-    for (int r = 0; r < p.rows; ++r) {
-      const uint16_t* src = a.q + (p.first + tok) * a.q_token + (p.head * a.group + g) * a.q_head + lane * 8;
-      const uint32_t dst = q + (lane >> 3) * kQChunkBytes + r * 128 + (((lane & 7) ^ (r & 7)) << 4);
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-      if (++g == a.group) {
-        g = 0;
-        ++tok;
+    const uint32_t to = q + (lane >> 3) * kQChunkBytes;
+#pragma unroll
+    for (int i = 0; i < kRows / 32; ++i) {
+      const int rows = min(p.rows - i * 32, 32);
+#pragma unroll 8
+      for (int r = 0; r < rows; ++r) {
+        const uint64_t src = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(mine[i]), r) + lane * 16;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + (i * 32 + r) * 128 +
+                                                                       (((lane & 7) ^ (r & 7)) << 4)),
+                     "l"(src)
+                     : "memory");
       }
     }
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&ctl.q_full)) : "memory");
@@ -566,10 +644,10 @@ __device__ void softmax_rows(const AttendArgs& a, Control& ctl, Swap& swap, uint
     ++swaps;
     return true;
   };
-  for (; pieces.next<true>(ctl, p); base += 2 * p.tiles, tile += p.tiles) {
+  for (; pieces.next(ctl, p); base += 2 * p.tiles, tile += p.tiles) {
     const bool busy = warp * 32 < p.rows;  // some lane of the warp has a row
     const int in_item = p.row0 + row;
-    const int tok = in_item / a.group;
+    const int tok = a.by_group.of(in_item);
     int seen = p.own ? p.seen0 + tok : p.seen0;
     if (seen > p.keys) seen = p.keys;
     float m = -INFINITY, l = 0.0f;
@@ -662,35 +740,18 @@ __device__ void softmax_rows(const AttendArgs& a, Control& ctl, Swap& swap, uint
       const bool live = row < p.rows;
       const int64_t token = p.first + tok;
       const int head = p.head * a.group + (in_item - tok * a.group);
-      const int64_t flat = token * a.q_heads + head;
-      float* ml = nullptr;
-      float* to = nullptr;
-      uint16_t* out = nullptr;
-      float scale_out = 1.0f;
       if (p.to == kToOutput) {
-        out = a.out + token * a.out_token + head * a.out_head + half * kHalfLanes;
-        scale_out = l == 0.0f ? 0.0f : 1.0f / l;
+        uint16_t* out = a.out + token * a.out_token + head * a.out_head + half * kHalfLanes;
+        const float scale_out = l == 0.0f ? 0.0f : 1.0f / l;
         if (live && half == 0 && a.lse != nullptr)
-          a.lse[flat] = l == 0.0f ? -INFINITY : (m * c + log2f(l)) * 0.6931471805599453f;
-      } else if (p.to == kToSlot) {
-        ml = a.slot_ml + (int64_t(p.slot) * a.slot_rows + row) * 2;
-        to = a.slot_o + (int64_t(p.slot) * a.slot_rows + row) * kHeadDim + half * kHalfLanes;
-      } else {
-        const int64_t at = int64_t(p.own) * a.tokens * a.q_heads + flat;
-        ml = a.part_ml + at * 2;
-        to = a.part_o + at * kHeadDim + half * kHalfLanes;
-      }
-      if (live && half == 0 && ml != nullptr)
-        *reinterpret_cast<float2*>(ml) = make_float2(m == -INFINITY ? m : m * c, l);
+          a.lse[token * a.q_heads + head] = l == 0.0f ? -INFINITY : (m * c + log2f(l)) * 0.6931471805599453f;
 #pragma unroll 1
-      for (int g = 0; g < kHalfLanes / 32; ++g) {
-        uint32_t o[32];
-        __syncwarp();
-        tmem_load32(my_o + g * 32, o);
-        tmem_load_wait();
-        if (!live) {
-          // a lane past the item's rows only takes part in the load
-        } else if (p.to == kToOutput) {
+        for (int g = 0; g < kHalfLanes / 32; ++g) {
+          uint32_t o[32];
+          __syncwarp();
+          tmem_load32(my_o + g * 32, o);
+          tmem_load_wait();
+          if (!live) continue;
           uint4* dst = reinterpret_cast<uint4*>(out + g * 32);
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
@@ -700,16 +761,36 @@ __device__ void softmax_rows(const AttendArgs& a, Control& ctl, Swap& swap, uint
             dst[i / 8] = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
                                     pack_bf16x2(f[6], f[7]));
           }
-        } else {
+        }
+      } else {
+        const int64_t all = int64_t(a.tokens) * a.q_heads;
+        const int64_t at = p.to == kToSlot ? int64_t(p.slot) * a.slot_rows + row
+                                           : (p.own * a.k_heads + p.head) * (int64_t(a.tokens) * a.group) +
+                                                 p.first * int64_t(a.group) + in_item;
+        const int64_t rows = p.to == kToSlot ? a.slot_rows : all;  // from one group of eight lanes to the next
+        float* to = p.to == kToSlot ? a.slot_o + (int64_t(p.slot) * 32 * a.slot_rows + row) * 8
+                                    : a.part_o + (p.own * 32 * all + at - p.own * all) * 8;
+        to += half * 16 * rows * 8;
+        if (live && half == 0)
+          *reinterpret_cast<float2*>((p.to == kToSlot ? a.slot_ml : a.part_ml) + at * 2) =
+              make_float2(m == -INFINITY ? m : m * c, l);
+#pragma unroll 1
+        for (int g = 0; g < kHalfLanes / 32; ++g) {
+          uint32_t o[32];
+          __syncwarp();
+          tmem_load32(my_o + g * 32, o);
+          tmem_load_wait();
+          if (!live) continue;
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
             float f[8];
 #pragma unroll
             for (int x = 0; x < 8; ++x) f[x] = __uint_as_float(o[i + x]);
-            store8f(to + g * 32 + i, f);
+            store8f(to + (g * 4 + i / 8) * rows * 8, f);
           }
         }
       }
+      __syncwarp();
     }
     tmem_fence_before();
     __syncwarp();
@@ -719,11 +800,7 @@ __device__ void softmax_rows(const AttendArgs& a, Control& ctl, Swap& swap, uint
 
 // Tiles of a request's own items.
 __device__ __forceinline__ int request_units(const AttendArgs& a, int b, bool tell) {
-  const Request r = load_request(a, b, tell);
-  const int rts = r.row_tiles(a.group);
-  int sum = 0;
-  for (int rt = 0; rt < rts; ++rt) sum += r.tiles(a.group, rt);
-  return sum * a.k_heads;
+  return load_request(a, b, tell).all_tiles(a) * a.k_heads;
 }
 
 __global__ void __launch_bounds__(kThreads, 1)
@@ -815,7 +892,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 0) {
       produce(a, ctl, &kmap, &vmap, ring_at);
     } else if (warp == 1) {
-      if (lane == 0) issue_products(ctl, q_at, ring_at, tmem);
+      issue_products(ctl, q_at, ring_at, uniform(tmem));
     } else if (warp == 2) {
       load_queries(a, ctl, q_at);
     } else if (warp == 3) {
@@ -834,143 +911,160 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // ---------------------------------------------------------------------------
-// Joining the partial results of a row: kGroups x 64 threads a row, four lanes
-// of the head each; the groups take the row's partial results in turn.  The
-// row's first warp works out where they are.
+// Joining the partial results of a row, eight lanes of the head a thread.  128
+// threads hold four neighbouring rows, four of them a 128-byte line of the
+// partial results' layout.  With kGroups > 1 a CTA joins four rows and its
+// groups of 128 threads take the rows' partial results in turn (few rows, which
+// may have many); with kGroups == 1 a CTA of two such groups joins 32 rows.
+// The first threads work out where the parts of the CTA's rows are, a row each.
 // ---------------------------------------------------------------------------
 struct RowParts {
   int cta[2], count[2], in_tile[2];  // prefix and own item: first CTA, CTAs, row of the item
-  int spare;                         // 1: a row of no request
   int live;                          // 1: this kernel writes the row
+  int token, head;
 };
 
-__device__ __forceinline__ void find_parts(const AttendArgs& a, int64_t flat, RowParts& to) {
-  const int lane = threadIdx.x & 31;
+__device__ __forceinline__ RowParts find_parts(const AttendArgs& a, int flat) {
   const int used = used_tokens(a);
   RowParts r{};
-  if (flat < int64_t(a.tokens) * a.q_heads) {
-    const int token = int(flat / a.q_heads), hq = int(flat - int64_t(token) * a.q_heads);
-    const int h = hq / a.group, g = hq - h * a.group;
-    int b = token;  // the row's request: the last that starts at or before the token
-    if (a.query_starts != nullptr) {
-      int lo = 0, hi = a.batch;
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (__ldg(a.query_starts + mid) <= token) lo = mid; else hi = mid;
-      }
-      b = lo;
+  if (flat >= a.tokens * a.q_heads) return r;
+  const int token = a.by_q_heads.of(flat), hq = flat - token * a.q_heads;
+  const int h = a.by_group.of(hq), g = hq - h * a.group;
+  r.token = token;
+  r.head = hq;
+  int b = token;  // the row's request: the last that starts at or before the token
+  if (a.query_starts != nullptr) {
+    int lo = 0, hi = a.batch;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (__ldg(a.query_starts + mid) <= token) lo = mid; else hi = mid;
     }
-    Request q{0, 0, 0};
-    if (token < used) q = load_request(a, b, false);
-    r.spare = token < q.first || token >= q.first + q.count;
-    if (!r.spare) {
-      const int pre = prefix_units(a, used);
-      const Line line(pre + a.units_before[a.batch], a.grid);
-      auto place = [&](int x, int first, int tiles, int in_tile) {
-        r.in_tile[x] = in_tile;
-        if (tiles == 0) return;
-        r.cta[x] = line.cta_of(first);
-        r.count[x] = line.cta_of(first + tiles - 1) - r.cta[x] + 1;
-      };
-      if (pre > 0) {
-        const int packed = token * a.group + g, key_tiles = div_up(a.prefix_len, kKeys);
-        place(0, (h * div_up(used * a.group, kRows) + packed / kRows) * key_tiles, key_tiles, packed % kRows);
-      }
-      const int packed = (token - q.first) * a.group + g, rt = packed / kRows;
-      int u = 0;  // tiles of the request's earlier rows
-      for (int x = lane; x < rt; x += 32) u += q.tiles(a.group, x);
-      u = __reduce_add_sync(0xffffffffu, u);
-      const int t = q.tiles(a.group, rt);
-      place(1, pre + a.units_before[b] + u * a.k_heads + h * t, t, packed % kRows);
-      r.live = pre > 0 || r.count[1] != 1;  // otherwise the first kernel wrote the row
-    } else {
-      r.live = a.fill;
-    }
+    b = lo;
   }
-  if (lane == 0) to = r;
+  Request q{0, 0, 0};
+  if (token < used) q = load_request(a, b, false);
+  if (token < q.first || token >= q.first + q.count) {  // a row of no request
+    r.live = a.fill;
+    return r;
+  }
+  const int pre = prefix_units(a, used);
+  const Line line(pre + a.units_before[a.batch], a.grid);
+  auto place = [&](int x, int first, int tiles, int in_tile) {
+    r.in_tile[x] = in_tile;
+    if (tiles == 0) return;
+    r.cta[x] = line.cta_of(first);
+    r.count[x] = line.cta_of(first + tiles - 1) - r.cta[x] + 1;
+  };
+  if (pre > 0) {
+    const int packed = token * a.group + g, key_tiles = div_up(a.prefix_len, kKeys);
+    place(0, (h * div_up(used * a.group, kRows) + packed / kRows) * key_tiles, key_tiles, packed % kRows);
+  }
+  const int packed = (token - q.first) * a.group + g, rt = packed / kRows;
+  const int t = q.tiles(a, rt);
+  place(1, pre + a.units_before[b] + q.tiles_before(a, rt) * a.k_heads + h * t, t, packed % kRows);
+  r.live = pre > 0 || r.count[1] != 1;  // otherwise the first kernel wrote the row
+  return r;
 }
 
-// Running join of partial results (m, l, four lanes of O).
+// Running join of partial results (m, l, eight lanes of O).
 struct Joined {
   float m = -INFINITY, l = 0.0f;
-  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  __device__ __forceinline__ void add(float2 ml, float4 v) {
-    if (ml.x == -INFINITY && ml.y == 0.0f) return;  // saw no key
-    const float top = fmaxf(m, ml.x);
+  float o[8] = {};
+  __device__ __forceinline__ void add(float m1, float l1, const float (&v)[8]) {
+    if (m1 == -INFINITY && l1 == 0.0f) return;  // saw no key
+    const float top = fmaxf(m, m1);
     const float base = top == -INFINITY ? 0.0f : top;
-    const float f0 = exp2_approx(m - base), f1 = exp2_approx(ml.x - base);
-    l = l * f0 + ml.y * f1;
-    o.x = o.x * f0 + v.x * f1;
-    o.y = o.y * f0 + v.y * f1;
-    o.z = o.z * f0 + v.z * f1;
-    o.w = o.w * f0 + v.w * f1;
+    const float f0 = exp2_approx(m - base), f1 = exp2_approx(m1 - base);
+    l = l * f0 + l1 * f1;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = o[i] * f0 + v[i] * f1;
     m = top;
   }
 };
 
+__device__ __forceinline__ void load8f(const float* p, float (&v)[8]) {
+  asm volatile("ld.global.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+               : "l"(p)
+               : "memory");
+}
+
 template <int kGroups>
-__global__ void __launch_bounds__(256) rope_attend_join_kernel(const __grid_constant__ AttendArgs a) {
-  constexpr int kRowThreads = 64 * kGroups, kRowsPerCta = 256 / kRowThreads;
+__global__ void __launch_bounds__(kGroups == 1 ? 256 : 128 * kGroups)
+    rope_attend_join_kernel(const __grid_constant__ AttendArgs a) {
+  constexpr int kRowsPerCta = kGroups == 1 ? 32 : 4, kUnroll = 4;
   __shared__ RowParts parts[kRowsPerCta];
-  __shared__ float4 s_o[kGroups > 1 ? 256 : 1];
-  __shared__ float2 s_ml[kGroups];
-  const int in_cta = threadIdx.x / kRowThreads, part = threadIdx.x % kRowThreads;
-  const int grp = part >> 6, d4 = part & 63;
-  const int64_t flat = int64_t(blockIdx.x) * kRowsPerCta + in_cta;
+  __shared__ float s_o[kGroups == 1 ? 1 : kGroups - 1][kGroups == 1 ? 1 : 10][128];
+  const int grp = threadIdx.x >> 7, in_grp = threadIdx.x & 127;
+  const int lanes8 = in_grp >> 2;  // eight lanes of the head
   pdl_enter();
-  if (part < 32) find_parts(a, flat, parts[in_cta]);
+  if (threadIdx.x < kRowsPerCta) parts[threadIdx.x] = find_parts(a, blockIdx.x * kRowsPerCta + threadIdx.x);
   __syncthreads();
-  const RowParts r = parts[in_cta];
-  const int64_t rows = int64_t(a.tokens) * a.q_heads;
-  const int count = r.live ? r.count[0] + r.count[1] : 0;
-  Joined sum;
-  constexpr int kUnroll = 4;
-  for (int i0 = grp; i0 < count; i0 += kGroups * kUnroll) {
-    float2 ml[kUnroll];
-    float4 v[kUnroll];
+  const int64_t all = int64_t(a.tokens) * a.q_heads;
+  for (int row = (kGroups == 1 ? 4 * grp : 0) + (in_grp & 3); row < kRowsPerCta; row += 8) {
+    const RowParts r = parts[row];
+    const int count = r.live ? r.count[0] + r.count[1] : 0;
+    const int h = a.by_group.of(r.head);
+    // the row among the whole items' rows
+    const int64_t packed = int64_t(h) * a.tokens * a.group + int64_t(r.token) * a.group + (r.head - h * a.group);
+    Joined sum;
+    for (int i0 = kGroups == 1 ? 0 : grp; i0 < count; i0 += kGroups * kUnroll) {
+      float2 ml[kUnroll];
+      float v[kUnroll][8];
 #pragma unroll
-    for (int x = 0; x < kUnroll; ++x) {
-      const int i = i0 + x * kGroups;
-      ml[x] = make_float2(-INFINITY, 0.0f);
-      v[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (i < count) {
-        const bool own = i >= r.count[0];
-        const int at = own ? i - r.count[0] : i;
-        const float* pml;
-        const float* po;
-        if ((own ? r.count[1] : r.count[0]) == 1) {  // the whole item's rows
-          const int64_t place = (own ? rows : 0) + flat;
-          pml = a.part_ml + place * 2;
-          po = a.part_o + place * kHeadDim;
-        } else {  // a CTA's first piece where the item began earlier, else its last
-          const int slot = 2 * ((own ? r.cta[1] : r.cta[0]) + at) + (at == 0);
-          const int64_t place = int64_t(slot) * a.slot_rows + (own ? r.in_tile[1] : r.in_tile[0]);
-          pml = a.slot_ml + place * 2;
-          po = a.slot_o + place * kHeadDim;
+      for (int x = 0; x < kUnroll; ++x) {
+        const int i = i0 + x * kGroups;
+        ml[x] = make_float2(-INFINITY, 0.0f);
+        if (i < count) {
+          const bool own = i >= r.count[0];
+          if ((own ? r.count[1] : r.count[0]) == 1) {
+            ml[x] = *reinterpret_cast<const float2*>(a.part_ml + ((own ? all : 0) + packed) * 2);
+            load8f(a.part_o + ((own ? 32 * all : 0) + lanes8 * all + packed) * 8, v[x]);
+          } else {  // a CTA's first piece where the item began earlier, else its last
+            const int at = own ? i - r.count[0] : i;
+            const int64_t slot = 2 * ((own ? r.cta[1] : r.cta[0]) + at) + (at == 0);
+            const int in_tile = own ? r.in_tile[1] : r.in_tile[0];
+            ml[x] = *reinterpret_cast<const float2*>(a.slot_ml + (slot * a.slot_rows + in_tile) * 2);
+            load8f(a.slot_o + ((slot * 32 + lanes8) * a.slot_rows + in_tile) * 8, v[x]);
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) v[x][k] = 0.0f;
         }
-        ml[x] = *reinterpret_cast<const float2*>(pml);
-        v[x] = *reinterpret_cast<const float4*>(po + d4 * 4);
+      }
+#pragma unroll
+      for (int x = 0; x < kUnroll; ++x) sum.add(ml[x].x, ml[x].y, v[x]);
+    }
+    if (kGroups > 1) {
+      if (grp > 0) {
+        float(&to)[kGroups == 1 ? 1 : 10][128] = s_o[grp - 1];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) to[k][in_grp] = sum.o[k];
+        to[8][in_grp] = sum.m;
+        to[9][in_grp] = sum.l;
+      }
+      __syncthreads();
+      if (grp > 0) return;
+#pragma unroll 1
+      for (int w = 0; w < kGroups - 1; ++w) {
+        float v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = s_o[w][k][in_grp];
+        sum.add(s_o[w][8][in_grp], s_o[w][9][in_grp], v);
       }
     }
-#pragma unroll
-    for (int x = 0; x < kUnroll; ++x) sum.add(ml[x], v[x]);
+    if (!r.live) continue;
+    const bool none = sum.l == 0.0f;
+    const float inv = none ? 0.0f : 1.0f / sum.l;
+    uint4 packed_out = make_uint4(0, 0, 0, 0);
+    if (!none)
+      packed_out = make_uint4(pack_bf16x2(sum.o[0] * inv, sum.o[1] * inv), pack_bf16x2(sum.o[2] * inv, sum.o[3] * inv),
+                              pack_bf16x2(sum.o[4] * inv, sum.o[5] * inv), pack_bf16x2(sum.o[6] * inv, sum.o[7] * inv));
+    *reinterpret_cast<uint4*>(a.out + r.token * a.out_token + r.head * a.out_head + lanes8 * 8) = packed_out;
+    if (a.lse != nullptr && lanes8 == 0)
+      a.lse[int64_t(r.token) * a.q_heads + r.head] =
+          none ? -INFINITY : (sum.m + log2f(sum.l)) * 0.6931471805599453f;
   }
-  if (kGroups > 1) {
-    s_o[threadIdx.x] = sum.o;
-    if (d4 == 0) s_ml[grp] = make_float2(sum.m, sum.l);
-    __syncthreads();
-    if (grp > 0) return;
-#pragma unroll
-    for (int x = 1; x < kGroups; ++x) sum.add(s_ml[x], s_o[x * 64 + d4]);
-  }
-  if (!r.live) return;
-  const int token = int(flat / a.q_heads), hq = int(flat - int64_t(token) * a.q_heads);
-  const bool none = sum.l == 0.0f;
-  const float inv = none ? 0.0f : 1.0f / sum.l;
-  uint2 packed = make_uint2(0, 0);
-  if (!none) packed = make_uint2(pack_bf16x2(sum.o.x * inv, sum.o.y * inv), pack_bf16x2(sum.o.z * inv, sum.o.w * inv));
-  *reinterpret_cast<uint2*>(a.out + token * a.out_token + hq * a.out_head + d4 * 4) = packed;
-  if (a.lse != nullptr && d4 == 0) a.lse[flat] = none ? -INFINITY : (sum.m + log2f(sum.l)) * 0.6931471805599453f;
 }
 
 // ---------------------------------------------------------------------------
@@ -1029,8 +1123,9 @@ int launch_attend(const CUtensorMap& kmap, const CUtensorMap& vmap, const Attend
   int rc = launch(rope_attend_kernel, unsigned(a.grid), kThreads, kSmemBytes, stream, kmap, vmap, a);
   if (rc != WELM_ROPE_OK) return rc;
   const int64_t rows = int64_t(a.tokens) * a.q_heads;
-  if (rows <= 1024) return launch(rope_attend_join_kernel<4>, unsigned(rows), 256, 0, stream, a);
-  return launch(rope_attend_join_kernel<1>, unsigned((rows + 3) / 4), 256, 0, stream, a);
+  if (rows <= 4 * a.grid) return launch(rope_attend_join_kernel<4>, unsigned((rows + 3) / 4), 512, 0, stream, a);
+  if (rows <= 4096) return launch(rope_attend_join_kernel<2>, unsigned((rows + 3) / 4), 256, 0, stream, a);
+  return launch(rope_attend_join_kernel<1>, unsigned((rows + 31) / 32), 256, 0, stream, a);
 }
 
 }  // namespace
@@ -1063,7 +1158,9 @@ int welm_rope_attend(const void* q, void* out, float* lse, const void* key_cache
       table_width > kMaxItems / block_size)
     return WELM_ROPE_ERR_BAD_SIZE;
   if (!query_starts && n_tokens != batch_size) return WELM_ROPE_ERR_BAD_SIZE;
-  // tiles are counted in 32 bits
+  // tiles are counted in 32 bits, and a request's rows against its keys too
+  if (num_q_heads / num_k_heads > (int64_t(1) << 36) / (table_width * block_size + n_tokens + 256))
+    return WELM_ROPE_ERR_BAD_SIZE;
   const __int128 row_tiles = (n_tokens * (num_q_heads / num_k_heads) + kRows - 1) / kRows;
   if ((row_tiles * ((prefix_len + kKeys - 1) / kKeys) +
        (row_tiles + batch_size) * ((table_width * block_size + kKeys - 1) / kKeys)) * num_k_heads >= INT32_MAX)
@@ -1087,8 +1184,9 @@ int welm_rope_attend(const void* q, void* out, float* lse, const void* key_cache
     }
   }
   if (bits & 7) return WELM_ROPE_ERR_BAD_STRIDE;
-  for (const void* p : {q, static_cast<const void*>(out), key_cache, value_cache, static_cast<const void*>(workspace)})
+  for (const void* p : {q, static_cast<const void*>(out), key_cache, value_cache})
     if (!aligned16(p)) return WELM_ROPE_ERR_BAD_STRIDE;
+  if (reinterpret_cast<uintptr_t>(workspace) & 31u) return WELM_ROPE_ERR_BAD_STRIDE;
   const int sms = current_sm_count();
   if (sms <= 0) {
     cudaGetLastError();
@@ -1121,6 +1219,9 @@ int welm_rope_attend(const void* q, void* out, float* lse, const void* key_cache
   a.q_heads = int32_t(num_q_heads);
   a.k_heads = int32_t(num_k_heads);
   a.group = int32_t(group);
+  a.by_group = Divisor(group);
+  a.by_block = Divisor(block_size);
+  a.by_q_heads = Divisor(num_q_heads);
   a.prefix_len = int32_t(prefix_len);
   a.max_len = int32_t(table_width * block_size);
   a.block_size = int32_t(block_size);

@@ -384,7 +384,7 @@ def attend_shared_prefix(
     is zeros, its logarithm minus infinity; so are rows of no request in an
     ``out`` that the call allocates, while a given ``out`` keeps them.
 
-    ``workspace``: device memory of :func:`attend_workspace_bytes`, 16-byte
+    ``workspace``: device memory of :func:`attend_workspace_bytes`, 32-byte
     aligned, for one call at a time; by default the call takes it from torch's
     allocator.  Lengths, starts and tables are read on the device, so a captured
     call follows them; ``prefix_len`` is part of the capture.  There is no
@@ -447,8 +447,8 @@ def attend_shared_prefix(
         elif not isinstance(workspace, torch.Tensor) or workspace.get_device() != index:
             raise ValueError("workspace must be a tensor on the device of q")
         size = workspace.numel() * workspace.element_size()
-        if size < need or not workspace.is_contiguous() or workspace.data_ptr() & 15:
-            raise ValueError(f"workspace must be contiguous, 16-byte aligned and hold {need} bytes")
+        if size < need or not workspace.is_contiguous() or workspace.data_ptr() & 31:
+            raise ValueError(f"workspace must be contiguous, 32-byte aligned and hold {need} bytes")
         _launch("welm_rope_attend", index, q.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(),
                 key_cache.data_ptr(), value_cache.data_ptr(), block_table.data_ptr(), seq_lens.data_ptr(), starts_ptr,
                 prefix_ptr, prefix_len, tokens, batch, q_heads, k_heads, q_token, q_head, out_token, out_head, width,

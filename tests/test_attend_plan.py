@@ -43,6 +43,20 @@ class Plan:
     def tiles(self, b, rt):
         return div_up(self.seen(b, rt), KEYS)
 
+    def tiles_before(self, b, rt):
+        """The closed form of sum(tiles(b, x) for x < rt), rt below own_tiles(b)."""
+        if rt == 0:
+            return 0
+        c = (127 + self.group * (self.lens[b] - self.counts[b] + 128)) >> 7
+
+        def total(x):
+            if x <= 0:
+                return 0
+            q, r = divmod(x, self.group)
+            return self.group * q * (q - 1) // 2 + q * r
+
+        return total(rt + c) - total(c)
+
     def begin(self, c):
         each, more = divmod(self.units, self.grid)
         return each * c + min(c, more)
@@ -95,7 +109,7 @@ class Plan:
             ranges.append((0, lo, lo + key_tiles, packed % ROWS))
         packed = (token - self.starts[b]) * self.group + g
         rt = packed // ROWS
-        lo = self.pre + self.before[b] + self.k_heads * sum(self.tiles(b, x) for x in range(rt)) + h * self.tiles(b, rt)
+        lo = self.pre + self.before[b] + self.k_heads * self.tiles_before(b, rt) + h * self.tiles(b, rt)
         ranges.append((1, lo, lo + self.tiles(b, rt), packed % ROWS))
         for x, lo, hi, row in ranges:
             if lo == hi:
@@ -198,3 +212,25 @@ def test_ring_order_names_every_entry_once():
             if j > 0:
                 taken.append(ring_v(j - 1, n))
         assert taken == list(range(2 * n))
+
+
+def test_closed_form_of_a_requests_tiles():
+    rng = random.Random(11)
+    for _ in range(400):
+        count, length = rng.randint(1, 2000), rng.choice([0, 1, rng.randint(0, 3000)])
+        group = rng.choice([1, 2, 3, 5, 6, 7, 8, 12, 64, 127, 128, 129, 200])
+        plan = Plan([count], [length], 0, group, 1, 148)
+        n = plan.own_tiles(0)
+        for rt in sorted({0, 1, n // 2, n - 1, rng.randrange(n)} & set(range(n))):
+            assert plan.tiles_before(0, rt) == sum(plan.tiles(0, x) for x in range(rt)), (count, length, group, rt)
+        assert plan.tiles_before(0, n - 1) + div_up(length, KEYS) == plan.units
+
+
+def test_division_by_multiplication():
+    for d in list(range(1, 300)) + [1000, 4095, 4096, 4097, 2 ** 20 + 1, 2 ** 30 - 1, 2 ** 30]:
+        log = (d - 1).bit_length()
+        mul = ((1 << (31 + log)) + d - 1) // d
+        assert mul < 2 ** 32
+        for x in [0, 1, d - 1, d, d + 1, 2 ** 31 - 1, (2 ** 31 - 1) // d * d - 1, (2 ** 31 - 1) // d * d]:
+            if 0 <= x < 2 ** 31:
+                assert (x * mul) >> (31 + log) == x // d
