@@ -43,6 +43,12 @@ constexpr int kChunkBytes = kKeys * 128;   // 64 lanes of 128 keys
 constexpr int kStageBytes = 2 * kChunkBytes;
 constexpr int kQChunkBytes = kRows * 128;  // 64 lanes of 128 rows
 constexpr int kQBytes = kRows * kHeadDim * 2;
+// What an item costs beside its tiles (its Q rows, its results), in tiles.
+// Measured with 0, 1, 2, 3 and 6 on one B200 (graph replay, us): 2560 query
+// tokens over 8192 shared and 900 own keys, whose own items are short and
+// numerous, 171.7, 145.8, 130.5, 131.3, 136.0; 24 requests' verification 24.3,
+// 24.2, 26.5, 26.9, 29.4; 256 requests over 32768 keys 82.4, 83.3, 84.7, 84.9, 96.2.
+constexpr int kItemCost = 2;
 constexpr int kPieces = 4;             // ring of piece descriptors
 constexpr int kThreads = 384;
 constexpr int kSoftmaxWarp0 = 4, kSoftmaxWarps = 8;
@@ -86,7 +92,7 @@ struct AttendArgs {
   int32_t grid;
   int32_t fill;                 // 1: rows of no request become zeros
   float scale;                  // times log2(e)
-  int32_t* units_before;        // [batch + 1] tiles of the items before each request
+  int32_t* units_before;        // [batch + 1] units of the own items before each request
   // Partial results.  O is laid out [32][rows][8 lanes]: the threads of a warp,
   // a row each, then write (and a row's reader reads) whole 32-byte sectors.
   float* slot_ml;               // [2 grid][slot_rows][2]
@@ -127,9 +133,17 @@ struct Request {
     };
     return sum(rt + c) - sum(c);
   }
-  __device__ __forceinline__ int all_tiles(const AttendArgs& a) const {
+  // Units of the line that one head's row tiles before rt take: their tiles,
+  // and kItemCost for each that has any (tile x has none while x + c < G).
+  __device__ __forceinline__ int units_before(const AttendArgs& a, int rt) const {
+    if (rt == 0) return 0;
+    const int c = int((127 + int64_t(a.group) * (len - count + 128)) >> 7);
+    const int none = min(max(a.group - c, 0), rt);
+    return tiles_before(a, rt) + (rt - none) * kItemCost;
+  }
+  __device__ __forceinline__ int all_units(const AttendArgs& a) const {
     const int n = row_tiles(a);
-    return n == 0 ? 0 : tiles_before(a, n - 1) + div_up(len, kKeys);
+    return n == 0 ? 0 : units_before(a, n - 1) + (len > 0 ? div_up(len, kKeys) + kItemCost : 0);
   }
 };
 
@@ -156,8 +170,11 @@ __device__ __forceinline__ int used_tokens(const AttendArgs& a) {
   return a.query_starts != nullptr ? int(clamp64(__ldg(a.query_starts + a.batch), 0, a.tokens)) : a.tokens;
 }
 
-// The line of tiles, cut into `grid` runs: CTA c has [begin(c), begin(c + 1)).
-// No run is empty: a line of fewer tiles than CTAs keeps only as many busy.
+// The line of all items' units, cut into `grid` runs: CTA c has [begin(c),
+// begin(c + 1)).  An item's first kItemCost units stand for its own cost (its
+// rows, its results) and hold no tile; a run that ends among them does nothing
+// for the item.  No run is empty: a line of fewer units than CTAs keeps only as
+// many busy.
 struct Line {
   int units, grid, each, more;  // the first `more` runs have each + 1 tiles
   __device__ __forceinline__ Line(int n, int ctas) : units(n), grid(n < ctas ? n : ctas) {
@@ -172,7 +189,7 @@ struct Line {
 };
 
 __device__ __forceinline__ int prefix_units(const AttendArgs& a, int used) {
-  return div_up(used * a.group, kRows) * a.k_heads * div_up(a.prefix_len, kKeys);
+  return a.prefix_len == 0 ? 0 : div_up(used * a.group, kRows) * a.k_heads * (div_up(a.prefix_len, kKeys) + kItemCost);
 }
 
 enum Destination { kToOutput, kToSlot, kToPart };
@@ -362,10 +379,13 @@ __device__ void list_pieces(const AttendArgs& a, Control& ctl, const Line& line,
   const int key_tiles = div_up(a.prefix_len, kKeys);
   const int row_tiles = div_up(used * a.group, kRows);
   while (u < end && u < pre) {
-    const int item = u / key_tiles;
+    const int item = u / (key_tiles + kItemCost);
+    const int at = u - item * (key_tiles + kItemCost), step = min(end - u, key_tiles + kItemCost - at);
+    u += step;
     Piece p;
-    p.first_tile = u - item * key_tiles;
-    p.tiles = min(end - u, key_tiles - p.first_tile);
+    p.first_tile = max(at - kItemCost, 0);
+    p.tiles = at + step - kItemCost - p.first_tile;
+    if (p.tiles <= 0) continue;
     p.keys = a.prefix_len;
     p.head = item / row_tiles;
     p.row0 = (item - p.head * row_tiles) * kRows;
@@ -377,7 +397,6 @@ __device__ void list_pieces(const AttendArgs& a, Control& ctl, const Line& line,
     p.to = p.tiles == key_tiles ? kToPart : kToSlot;
     p.slot = 2 * cta + (p.first_tile > 0 ? 0 : 1);
     if (!emit(p)) return;
-    u += p.tiles;
   }
   int base = ctl.start_units + pre;  // of request `start_request`
   for (int b0 = ctl.start_request; u < end && b0 < a.batch; b0 += 32) {
@@ -392,17 +411,20 @@ __device__ void list_pieces(const AttendArgs& a, Control& ctl, const Line& line,
         int hi = rts;
         while (hi - rt > 1) {
           const int mid = (rt + hi) >> 1;
-          if (base + a.k_heads * r.tiles_before(a, mid) <= u) rt = mid; else hi = mid;
+          if (base + a.k_heads * r.units_before(a, mid) <= u) rt = mid; else hi = mid;
         }
-        base += a.k_heads * r.tiles_before(a, rt);
+        base += a.k_heads * r.units_before(a, rt);
       }
       for (; rt < rts && u < end; ++rt) {
-        const int t = r.tiles(a, rt);
-        for (int h = 0; h < a.k_heads && u < end; ++h, base += t) {
-          if (u >= base + t) continue;
+        const int t = r.tiles(a, rt), cost = t > 0 ? t + kItemCost : 0;
+        for (int h = 0; h < a.k_heads && u < end; ++h, base += cost) {
+          if (u >= base + cost) continue;
+          const int at = u - base, step = min(end - u, cost - at);
+          u += step;
           Piece p;
-          p.first_tile = u - base;
-          p.tiles = min(end - u, t - p.first_tile);
+          p.first_tile = max(at - kItemCost, 0);
+          p.tiles = at + step - kItemCost - p.first_tile;
+          if (p.tiles <= 0) continue;
           p.keys = r.seen(a, rt);
           p.head = h;
           p.row0 = rt * kRows;
@@ -414,7 +436,6 @@ __device__ void list_pieces(const AttendArgs& a, Control& ctl, const Line& line,
           p.to = p.tiles < t ? kToSlot : a.prefix_len > 0 ? kToPart : kToOutput;
           p.slot = 2 * cta + (p.first_tile > 0 ? 0 : 1);
           if (!emit(p)) return;
-          u += p.tiles;
         }
       }
     }
@@ -798,9 +819,9 @@ __device__ void softmax_rows(const AttendArgs& a, Control& ctl, Swap& swap, uint
   }
 }
 
-// Tiles of a request's own items.
+// Units of a request's own items.
 __device__ __forceinline__ int request_units(const AttendArgs& a, int b, bool tell) {
-  return load_request(a, b, tell).all_tiles(a) * a.k_heads;
+  return load_request(a, b, tell).all_units(a) * a.k_heads;
 }
 
 __global__ void __launch_bounds__(kThreads, 1)
@@ -952,16 +973,16 @@ __device__ __forceinline__ RowParts find_parts(const AttendArgs& a, int flat) {
   auto place = [&](int x, int first, int tiles, int in_tile) {
     r.in_tile[x] = in_tile;
     if (tiles == 0) return;
-    r.cta[x] = line.cta_of(first);
-    r.count[x] = line.cta_of(first + tiles - 1) - r.cta[x] + 1;
+    r.cta[x] = line.cta_of(first + kItemCost);
+    r.count[x] = line.cta_of(first + kItemCost + tiles - 1) - r.cta[x] + 1;
   };
   if (pre > 0) {
     const int packed = token * a.group + g, key_tiles = div_up(a.prefix_len, kKeys);
-    place(0, (h * div_up(used * a.group, kRows) + packed / kRows) * key_tiles, key_tiles, packed % kRows);
+    place(0, (h * div_up(used * a.group, kRows) + packed / kRows) * (key_tiles + kItemCost), key_tiles, packed % kRows);
   }
   const int packed = (token - q.first) * a.group + g, rt = packed / kRows;
   const int t = q.tiles(a, rt);
-  place(1, pre + a.units_before[b] + q.tiles_before(a, rt) * a.k_heads + h * t, t, packed % kRows);
+  place(1, pre + a.units_before[b] + q.units_before(a, rt) * a.k_heads + h * (t + kItemCost), t, packed % kRows);
   r.live = pre > 0 || r.count[1] != 1;  // otherwise the first kernel wrote the row
   return r;
 }
@@ -1158,12 +1179,12 @@ int welm_rope_attend(const void* q, void* out, float* lse, const void* key_cache
       table_width > kMaxItems / block_size)
     return WELM_ROPE_ERR_BAD_SIZE;
   if (!query_starts && n_tokens != batch_size) return WELM_ROPE_ERR_BAD_SIZE;
-  // tiles are counted in 32 bits, and a request's rows against its keys too
+  // units are counted in 32 bits, and a request's rows against its keys too
   if (num_q_heads / num_k_heads > (int64_t(1) << 36) / (table_width * block_size + n_tokens + 256))
     return WELM_ROPE_ERR_BAD_SIZE;
   const __int128 row_tiles = (n_tokens * (num_q_heads / num_k_heads) + kRows - 1) / kRows;
-  if ((row_tiles * ((prefix_len + kKeys - 1) / kKeys) +
-       (row_tiles + batch_size) * ((table_width * block_size + kKeys - 1) / kKeys)) * num_k_heads >= INT32_MAX)
+  if ((row_tiles * ((prefix_len + kKeys - 1) / kKeys + kItemCost) +
+       (row_tiles + batch_size) * ((table_width * block_size + kKeys - 1) / kKeys + kItemCost)) * num_k_heads >= INT32_MAX)
     return WELM_ROPE_ERR_BAD_SIZE;
   if (!(scale > 0.0f) || scale > 3.0e38f || (fill_unused != 0 && fill_unused != 1)) return WELM_ROPE_ERR_BAD_MODE;
   if (n_tokens == 0 || batch_size == 0) return WELM_ROPE_OK;

@@ -10,6 +10,7 @@ import random
 import pytest
 
 ROWS = KEYS = 128
+COST = 2  # kItemCost
 
 
 def div_up(a, b):
@@ -25,10 +26,10 @@ class Plan:
             self.starts.append(self.starts[-1] + n)
         self.tokens = self.starts[-1]
         self.row_tiles = div_up(self.tokens * self.group, ROWS)
-        self.pre = self.row_tiles * k_heads * div_up(prefix, KEYS)
+        self.pre = self.row_tiles * k_heads * (div_up(prefix, KEYS) + COST) if prefix else 0
         self.before = [0]
         for b in range(len(counts)):
-            self.before.append(self.before[-1] + k_heads * sum(self.tiles(b, rt) for rt in range(self.own_tiles(b))))
+            self.before.append(self.before[-1] + k_heads * sum(self.cost(b, rt) for rt in range(self.own_tiles(b))))
         self.units = self.pre + self.before[-1]
         self.grid = min(grid, self.units)
         self.slot_rows = min(ROWS, self.tokens * self.group)
@@ -42,6 +43,16 @@ class Plan:
 
     def tiles(self, b, rt):
         return div_up(self.seen(b, rt), KEYS)
+
+    def cost(self, b, rt):
+        t = self.tiles(b, rt)
+        return t + COST if t else 0
+
+    def units_before(self, b, rt):
+        if rt == 0:
+            return 0
+        c = (127 + self.group * (self.lens[b] - self.counts[b] + 128)) >> 7
+        return self.tiles_before(b, rt) + (rt - min(max(self.group - c, 0), rt)) * COST
 
     def tiles_before(self, b, rt):
         """The closed form of sum(tiles(b, x) for x < rt), rt below own_tiles(b)."""
@@ -71,29 +82,36 @@ class Plan:
         u, end = self.begin(cta), self.begin(cta + 1)
         key_tiles = div_up(self.prefix, KEYS)
         while u < end and u < self.pre:
-            item, first = divmod(u, key_tiles)
-            n = min(end - u, key_tiles - first)
+            item, at = divmod(u, key_tiles + COST)
+            step = min(end - u, key_tiles + COST - at)
+            u += step
+            first = max(at - COST, 0)
+            n = at + step - COST - first
+            if n <= 0:
+                continue
             head, tile = divmod(item, self.row_tiles)
             to = ("part", 0) if n == key_tiles else ("slot", 2 * cta + (0 if first > 0 else 1))
             yield ("prefix", head, tile), first, n, to
-            u += n
         want = max(0, min(self.begin(cta) - self.pre, self.before[-1]))
         start = next((b for b in range(len(self.counts)) if self.before[b] <= want < self.before[b + 1]),
                      len(self.counts))
         base = self.pre + (self.before[start] if start < len(self.counts) else 0)
         for b in range(start, len(self.counts)):
             for rt in range(self.own_tiles(b)):
-                t = self.tiles(b, rt)
+                t, cost = self.tiles(b, rt), self.cost(b, rt)
                 for h in range(self.k_heads):
-                    if u < end and u < base + t:
-                        first = u - base
-                        assert first >= 0
-                        n = min(end - u, t - first)
+                    if u < end and u < base + cost:
+                        at = u - base
+                        assert at >= 0
+                        step = min(end - u, cost - at)
+                        u += step
+                        first = max(at - COST, 0)
+                        n = at + step - COST - first
                         to = ("slot", 2 * cta + (0 if first > 0 else 1)) if n < t else (
                             ("part", 1) if self.prefix else ("out", 0))
-                        yield ("own", b, rt, h), first, n, to
-                        u += n
-                    base += t
+                        if n > 0:
+                            yield ("own", b, rt, h), first, n, to
+                    base += cost
         assert u == end
 
     def join(self, token, hq):
@@ -105,11 +123,12 @@ class Plan:
         if self.pre:
             packed = token * self.group + g
             key_tiles = div_up(self.prefix, KEYS)
-            lo = (h * self.row_tiles + packed // ROWS) * key_tiles
+            lo = (h * self.row_tiles + packed // ROWS) * (key_tiles + COST) + COST
             ranges.append((0, lo, lo + key_tiles, packed % ROWS))
         packed = (token - self.starts[b]) * self.group + g
         rt = packed // ROWS
-        lo = self.pre + self.before[b] + self.k_heads * self.tiles_before(b, rt) + h * self.tiles(b, rt)
+        lo = self.pre + self.before[b] + self.k_heads * self.units_before(b, rt) + (
+            h * (self.tiles(b, rt) + COST) + COST)
         ranges.append((1, lo, lo + self.tiles(b, rt), packed % ROWS))
         for x, lo, hi, row in ranges:
             if lo == hi:
@@ -223,7 +242,9 @@ def test_closed_form_of_a_requests_tiles():
         n = plan.own_tiles(0)
         for rt in sorted({0, 1, n // 2, n - 1, rng.randrange(n)} & set(range(n))):
             assert plan.tiles_before(0, rt) == sum(plan.tiles(0, x) for x in range(rt)), (count, length, group, rt)
-        assert plan.tiles_before(0, n - 1) + div_up(length, KEYS) == plan.units
+            assert plan.units_before(0, rt) == sum(plan.cost(0, x) for x in range(rt)), (count, length, group, rt)
+        last = div_up(length, KEYS) + COST if length else 0
+        assert plan.units_before(0, n - 1) + last == plan.units
 
 
 def test_division_by_multiplication():
