@@ -1,10 +1,13 @@
-"""Build recipe for the in-tree sm_100a shared library.
+"""Build recipe for the in-tree sm_100a shared library and its torch binding.
 
 ``python -m testfiles_b200.build`` (or ``build_native()``) compiles the
 ``csrc/*.cu`` translation units with nvcc for ``sm_100a`` only into
 ``testfiles_b200/libwelm_rope_b200.so``.  The CUDA runtime is linked
 statically, so the library loads on a machine without a GPU (the host-only
 entry points then work; the device ones report a CUDA error).
+``build_binding()`` compiles ``csrc/torch_binding.cpp`` against the installed
+torch into the Python module ``testfiles_b200/_welm_torch.so``, which calls the
+library; ``build_native()`` builds it too.
 """
 
 from __future__ import annotations
@@ -13,6 +16,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PACKAGE_DIR = Path(__file__).resolve().parent
@@ -25,6 +29,8 @@ SOURCES = tuple(CSRC / name for name in (
 HEADERS = (REPO_ROOT / "include" / "welm_rope.h", *(CSRC / name for name in (
     "rope_device.cuh", "rope_host.cuh", "rope_axes.cuh", "rope_tma.cuh")))
 LIBRARY = PACKAGE_DIR / "libwelm_rope_b200.so"
+BINDING_SOURCE = CSRC / "torch_binding.cpp"
+BINDING = PACKAGE_DIR / "_welm_torch.so"
 
 NVCC_FLAGS = (
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -51,9 +57,14 @@ def _stale() -> bool:
 
 
 def build_native(force: bool = False, verbose: bool = False, extra_flags: tuple[str, ...] = ()) -> Path:
-    """Compile the library if it is missing or older than its sources."""
-    if not force and not _stale():
-        return LIBRARY
+    """Compile the library and the binding if they are missing or older than their sources."""
+    if force or _stale():
+        _build_library(verbose, extra_flags)
+    build_binding(force, verbose)
+    return LIBRARY
+
+
+def _build_library(verbose: bool, extra_flags: tuple[str, ...]) -> None:
     tmp = LIBRARY.with_suffix(".so.tmp")
     cmd = [
         _nvcc(), *NVCC_FLAGS, *extra_flags,
@@ -63,13 +74,46 @@ def build_native(force: bool = False, verbose: bool = False, extra_flags: tuple[
     ]
     if verbose:
         print(" ".join(cmd), flush=True)
+    _run("nvcc", cmd, verbose)
+    os.replace(tmp, LIBRARY)
+
+
+def build_binding(force: bool = False, verbose: bool = False) -> Path:
+    """Compile the torch binding if it is missing or older than its source or the installed torch."""
+    import torch
+
+    torch_dir = Path(torch.__file__).resolve().parent
+    newer = (BINDING_SOURCE, REPO_ROOT / "include" / "welm_rope.h", torch_dir / "version.py")
+    if not force and BINDING.exists() and all(p.stat().st_mtime <= BINDING.stat().st_mtime for p in newer):
+        return BINDING
+    cuda = Path(_nvcc()).resolve().parent.parent
+    tmp = BINDING.with_suffix(".so.tmp")
+    cmd = [
+        shutil.which("g++") or "c++", "-std=c++17", "-O2", "-Wall", "-fPIC", "-shared", "-fvisibility=hidden",
+        f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+        "-I", str(REPO_ROOT / "include"),
+        "-isystem", str(torch_dir / "include"),
+        "-isystem", str(torch_dir / "include" / "torch" / "csrc" / "api" / "include"),
+        "-isystem", str(cuda / "include"),
+        "-isystem", sysconfig.get_paths()["include"],
+        str(BINDING_SOURCE),
+        "-L", str(torch_dir / "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10_cuda", "-lc10",
+        "-L", str(PACKAGE_DIR), f"-l:{LIBRARY.name}", "-Wl,-rpath,$ORIGIN",
+        "-o", str(tmp),
+    ]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    _run("g++", cmd, verbose)
+    os.replace(tmp, BINDING)
+    return BINDING
+
+
+def _run(tool: str, cmd: list[str], verbose: bool) -> None:
     result = subprocess.run(cmd, capture_output=True, text=True)
     if result.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({result.returncode}):\n{result.stdout}\n{result.stderr}")
+        raise RuntimeError(f"{tool} failed ({result.returncode}):\n{result.stdout}\n{result.stderr}")
     if verbose and (result.stdout or result.stderr):
         print(result.stdout + result.stderr, flush=True)
-    os.replace(tmp, LIBRARY)
-    return LIBRARY
 
 
 if __name__ == "__main__":

@@ -9,7 +9,7 @@ import pytest
 import torch
 
 import testfiles_b200 as welm
-from testfiles_b200 import _native, paged
+from testfiles_b200 import _native, build
 
 FAKE = 0x1000  # a non-NULL address; every call below is rejected before it is used
 
@@ -102,7 +102,7 @@ def test_workspace_entry():
     assert size.value == -1
 
 
-def test_python_refuses_cpu_tensors_and_bad_sections():
+def test_python_refuses_cpu_tensors():
     q, k = torch.zeros((4, 6, 256), dtype=torch.bfloat16), torch.zeros((4, 1, 256), dtype=torch.bfloat16)
     pos, cache = torch.zeros((3, 4), dtype=torch.int64), torch.zeros((8, 64))
     for call in (welm.rope_multi_axis, welm.rope_multi_axis_inplace):
@@ -112,9 +112,14 @@ def test_python_refuses_cpu_tensors_and_bad_sections():
         welm.rope_kv_append(q, k, k, pos[0], cache, pos[0], k[None], k[None])
     with pytest.raises(ValueError, match="CUDA"):
         welm.attend_shared_prefix(q, k[None], k[None], pos.int(), pos[0])
-    for bad in ((16, 8), (), (8,) * 5, (40, -8), (33,)):
-        with pytest.raises(ValueError, match="sections"):
-            paged._sections(bad)
+
+
+def test_binding_is_built_and_of_the_librarys_version():
+    assert build.BINDING.exists(), "run python -m testfiles_b200.build"
+    from testfiles_b200 import _welm_torch
+
+    with pytest.raises(TypeError, match="13 arguments"):
+        _welm_torch.attend()
 
 
 DEV = "cuda:0"
@@ -153,7 +158,10 @@ def test_append_refuses(change, error):
 @pytest.mark.gpu
 @pytest.mark.parametrize("change,error", [
     (dict(positions=lambda t: t[:2]), ValueError), (dict(positions=lambda t: t.t().contiguous().t()), ValueError),
-    (dict(sections=(16, 8)), ValueError), (dict(q=lambda t: t[:3]), ValueError), (dict(k=lambda t: t.half()), TypeError),
+    (dict(sections=(16, 8)), ValueError), (dict(sections=()), ValueError), (dict(sections=(8,) * 5), ValueError),
+    (dict(sections=(40, -8, 0)), ValueError), (dict(sections="abc"), TypeError), (dict(sections=3), TypeError),
+    (dict(sections=(16.0, 8, 8)), TypeError), (dict(q=None), ValueError), (dict(k=None), ValueError),
+    (dict(positions=[0]), TypeError), (dict(q=lambda t: t[:3]), ValueError), (dict(k=lambda t: t.half()), TypeError),
     (dict(q=lambda t: t.requires_grad_()), ValueError), (dict(cos_sin_cache=lambda t: t.double()), TypeError),
     (dict(q=lambda t: torch.zeros(4 * 6 * 256 + 1, dtype=t.dtype, device=DEV)[1:].view(4, 6, 256)), ValueError),
     (dict(q=lambda t: t[:1].expand(4, 6, 256)), RuntimeError),
