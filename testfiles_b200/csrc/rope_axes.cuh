@@ -31,20 +31,24 @@ struct AxisArgs {
   AxisMap map;
 };
 
-// Cache rows of one token; false when a used axis' position lies outside the
-// cache (then nothing may be read).  Every thread of a token comes to the same
-// answer, whichever pairs it rotates.
+// Cache rows of one token.  load() starts the position loads, ready() turns
+// them into rows: false when a used axis' position lies outside the cache (then
+// nothing may be read).  Every thread of a token comes to the same answer,
+// whichever pairs it rotates.
 struct AxisRows {
+  int64_t pos[kMaxAxes];
   const float* row[kMaxAxes];
-  __device__ __forceinline__ bool load(const AxisArgs& a, int64_t tok) {
+  __device__ __forceinline__ void load(const AxisArgs& a, int64_t tok) {
+#pragma unroll
+    for (int x = 0; x < kMaxAxes; ++x)
+      pos[x] = a.map.used >> x & 1u ? __ldg(a.positions + x * a.pos_stride + tok) : 0;
+  }
+  __device__ __forceinline__ bool ready(const AxisArgs& a) {
     bool ok = true;
 #pragma unroll
     for (int x = 0; x < kMaxAxes; ++x) {
-      row[x] = a.cache;
-      if (!(a.map.used >> x & 1u)) continue;
-      const int64_t pos = __ldg(a.positions + x * a.pos_stride + tok);
-      if (pos < 0 || pos >= a.max_position) ok = false;
-      else row[x] = a.cache + pos * kRopeDim;
+      if (a.map.used >> x & 1u) ok = ok && pos[x] >= 0 && pos[x] < a.max_position;
+      row[x] = a.cache + pos[x] * kRopeDim;
     }
     return ok;
   }
@@ -105,6 +109,11 @@ struct WholeHead {
 // ---------------------------------------------------------------------------
 // Host side.
 // ---------------------------------------------------------------------------
+// In-place rotations of at most this many (token, head) rows take one head a
+// thread, so that a small launch spreads over more threads; larger ones take up
+// to four, so that more loads share a position and are in flight at once.
+constexpr int64_t kOneHeadRows = 8192;
+
 // Sections: the pairs of each axis, 32 in all.  In runs (axis 0's pairs
 // first), or dealt out in turn over the axes that still have pairs left.
 bool make_axis_map(const int32_t* sections, int64_t axes, int64_t interleaved, AxisMap& m) {

@@ -3,9 +3,9 @@
 //
 // Q is rotated in place; the rotated K and the V of every token are written to
 // the token's cache slot, so K is read once and never written back.
-// Memory-bound.  Work items: one per (token, Q head, part), then one per
-// (token, K head, part), whose thread moves a quarter of a K head and of its V
-// head with all sixteen 16-byte loads in flight at once.
+// Memory-bound.  Work items: one per (token, K head, part), whose thread moves a
+// quarter of a K head and of its V head with all sixteen 16-byte loads in
+// flight at once, then one per (token, chunk of Q heads, part).
 
 #include "rope_axes.cuh"
 
@@ -23,52 +23,77 @@ struct AppendArgs {
   int64_t num_slots;
   AxisArgs axes;
   int32_t* status;
-  int32_t q_items, kv_items, q_heads, k_heads, block_size;
+  int32_t q_items, kv_items, q_heads, q_chunks, k_heads, block_size;
 };
 
 constexpr int kValueChunks = kHeadDim / kParts / 8;  // 16-byte chunks of V a thread moves
 
-// Slot and cache rows of one token; false when the token is padding or is
-// flagged, and then nothing of it is written.  `tell`: this thread reports.
-__device__ __forceinline__ bool append_token(const AppendArgs& a, int tok, bool tell, int64_t& slot, AxisRows& rows) {
-  slot = __ldg(a.slots + tok);
+// Whether the token is written; otherwise it is padding or flagged.  `tell`:
+// this thread reports.
+__device__ __forceinline__ bool append_token(const AppendArgs& a, int64_t slot, AxisRows& rows, bool tell) {
   if (slot < 0) return false;
-  const bool ok = rows.load(a.axes, tok);
+  const bool ok = rows.ready(a.axes);
   if (tell && !ok) raise_status(a.status, WELM_ROPE_DEV_BAD_POSITION);
   if (slot < a.num_slots) return ok;
   if (tell) raise_status(a.status, WELM_ROPE_DEV_BAD_SLOT);
   return false;
 }
 
+// kHeads: Q heads a thread rotates with the cos/sin that it gathered once.
+template <int kHeads>
 __global__ void __launch_bounds__(kBlock) rope_kv_append_kernel(const AppendArgs a) {
   const int item = blockIdx.x * blockDim.x + threadIdx.x;
   const int part = item & (kParts - 1);
+  const bool is_q = item >= a.kv_items;
+  const int row = (is_q ? item - a.kv_items : item) >> kPartShift;
+  const int per_token = is_q ? max(a.q_chunks, 1) : a.k_heads;
+  const int tok = row / per_token;
+  const int h = row - tok * per_token;
+  const bool live = item < a.kv_items + a.q_items;
+  const uint16_t* k = a.k + tok * a.k_token + h * a.k_head;
+  const uint16_t* v = a.v + tok * a.v_token + h * a.v_head;
+  uint16_t* q = a.q + tok * a.q_token + h * a.q_head + kRopeLane0 + part * kLanes;
+  const int64_t q_step = a.q_chunks * a.q_head;
+  const int heads = (a.q_heads - h + a.q_chunks - 1) / per_token;  // h, h + chunks, ...
+  if (live) {
+    if (!is_q) {
+      prefetch_line(k + part * 64);
+      prefetch_line(v + part * 64);
+    } else if (kHeads > 1 && part < heads) {
+      prefetch_line(q + part * q_step);
+    }
+  }
   pdl_enter();
+  if (!live) return;
+  const int64_t slot = __ldg(a.slots + tok);
   AxisRows rows;
+  rows.load(a.axes, tok);
   CosSin cs;
-  int64_t slot;
-  if (item < a.q_items) {
-    const int row = item >> kPartShift;
-    const int tok = row / a.q_heads;
-    uint16_t* p = a.q + tok * a.q_token + (row - tok * a.q_heads) * a.q_head + kRopeLane0 + part * kLanes;
-    uint4 x1 = *reinterpret_cast<const uint4*>(p);
-    uint4 x2 = *reinterpret_cast<const uint4*>(p + kHalf);
-    if (!append_token(a, tok, false, slot, rows)) return;
+  if (is_q) {
+    uint4 x1[kHeads], x2[kHeads];
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+      if (i >= heads) continue;
+      x1[i] = *reinterpret_cast<const uint4*>(q + i * q_step);
+      x2[i] = *reinterpret_cast<const uint4*>(q + i * q_step + kHalf);
+    }
+    if (!append_token(a, slot, rows, false)) return;
     rows.gather(a.axes.map, part, cs);
-    rotate8(x1, x2, cs);
-    *reinterpret_cast<uint4*>(p) = x1;
-    *reinterpret_cast<uint4*>(p + kHalf) = x2;
-  } else if (item - a.q_items < a.kv_items) {
-    const int row = (item - a.q_items) >> kPartShift;
-    const int tok = row / a.k_heads;
-    const int h = row - tok * a.k_heads;
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i) {
+      if (i >= heads) continue;
+      rotate8(x1[i], x2[i], cs);
+      *reinterpret_cast<uint4*>(q + i * q_step) = x1[i];
+      *reinterpret_cast<uint4*>(q + i * q_step + kHalf) = x2[i];
+    }
+  } else {
     WholeHead piece;
-    piece.load(a.k + tok * a.k_token + h * a.k_head, part);
-    const uint16_t* v = a.v + tok * a.v_token + h * a.v_head + part * 8;
+    piece.load(k, part);
     uint4 vv[kValueChunks];
 #pragma unroll
-    for (int c = 0; c < kValueChunks; ++c) vv[c] = *reinterpret_cast<const uint4*>(v + 8 * kParts * c);
-    if (!append_token(a, tok, part == 0 && h == 0, slot, rows)) return;
+    for (int c = 0; c < kValueChunks; ++c)
+      vv[c] = *reinterpret_cast<const uint4*>(v + part * 8 + 8 * kParts * c);
+    if (!append_token(a, slot, rows, part == 0 && h == 0)) return;
     rows.gather(a.axes.map, part, cs);
     rotate8(piece.x1, piece.x2, cs);
     const int64_t block = slot / a.block_size;
@@ -151,11 +176,14 @@ int welm_rope_kv_append(void* q, const void* k, const void* v, const int64_t* po
   a.q_heads = int32_t(num_q_heads);
   a.k_heads = int32_t(num_k_heads);
   a.block_size = int32_t(block_size);
-  a.q_items = int32_t(n_tokens * num_q_heads * kParts);
+  const bool one = n_tokens * num_q_heads <= kOneHeadRows;
+  a.q_chunks = int32_t(one ? num_q_heads : (num_q_heads + 3) / 4);
+  a.q_items = int32_t(n_tokens * a.q_chunks * kParts);
   a.kv_items = int32_t(n_tokens * num_k_heads * kParts);
-  const int64_t total = int64_t(a.q_items) + a.kv_items;
-  return launch(rope_kv_append_kernel, unsigned((total + kBlock - 1) / kBlock), kBlock, 0,
-                static_cast<cudaStream_t>(stream), a);
+  const unsigned grid = unsigned((int64_t(a.q_items) + a.kv_items + kBlock - 1) / kBlock);
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return one ? launch(rope_kv_append_kernel<1>, grid, kBlock, 0, s, a)
+             : launch(rope_kv_append_kernel<4>, grid, kBlock, 0, s, a);
 }
 
 }  // extern "C"

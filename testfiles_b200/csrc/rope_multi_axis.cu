@@ -4,10 +4,9 @@
 //
 // The rotation of a pair is orthogonal, so the gradient of the inputs is the
 // inverse rotation (sin negated) of the gradient of the outputs: the backward
-// pass is this kernel again.  Memory-bound: six FP32 operations a pair.  Work
-// item: (token, head, part), four threads a head as in the other kernels; the
-// Q heads of a token come first, then its K heads, so the threads of a warp
-// share the token's cos/sin lines in L1.
+// pass is the same kernel again.  Memory-bound: six FP32 operations a pair.
+// Four threads ("parts") share a head's rotated lanes as in the other kernels;
+// the Q heads of a token come first, then its K heads.
 
 #include "rope_axes.cuh"
 
@@ -23,11 +22,62 @@ struct MultiAxisArgs {
   float sign;  // +1 forward, -1 inverse
 };
 
-// kCopy: whole heads are read and written (lanes 0..191 copied); otherwise only
-// the rotated lanes move.  A token whose position is out of range is copied
-// unrotated, or left as it is, and flagged.
-template <bool kCopy>
+// In place: only the rotated lanes move.  A thread rotates up to kHeads heads of
+// its token with the cos/sin it gathered once, their loads all in flight.
+template <int kHeads>
 __global__ void __launch_bounds__(kBlock) rope_multi_axis_kernel(const MultiAxisArgs a) {
+  const int item = blockIdx.x * blockDim.x + threadIdx.x;
+  const int part = item & (kParts - 1);
+  const int row = item >> kPartShift;
+  const int chunks = (a.heads + kHeads - 1) / kHeads;
+  const int tok = row / chunks;
+  const int first = row - tok * chunks;  // heads first, first + chunks, ...
+  uint16_t* head[kHeads];
+#pragma unroll
+  for (int i = 0; i < kHeads; ++i) {
+    const int h = first + i * chunks;
+    const int x = h >= a.q_heads;
+    head[i] = h < a.heads ? a.dst[x] + tok * a.dst_token[x] + (x ? h - a.q_heads : h) * a.dst_head[x] + kRopeLane0 +
+                                part * kLanes
+                          : nullptr;
+  }
+  if (kHeads > 1 && item < a.items) {
+#pragma unroll
+    for (int i = 0; i < kHeads; ++i)
+      if ((i & 3) == part && head[i] != nullptr) prefetch_line(head[i]);
+  }
+  pdl_enter();
+  if (item >= a.items) return;
+  AxisRows rows;
+  rows.load(a.axes, tok);
+  uint4 x1[kHeads], x2[kHeads];
+#pragma unroll
+  for (int i = 0; i < kHeads; ++i) {
+    if (head[i] == nullptr) continue;
+    x1[i] = *reinterpret_cast<const uint4*>(head[i]);
+    x2[i] = *reinterpret_cast<const uint4*>(head[i] + kHalf);
+  }
+  if (!rows.ready(a.axes)) {  // the token stays as it is
+    if (part == 0 && first == 0) raise_status(a.status, WELM_ROPE_DEV_BAD_POSITION);
+    return;
+  }
+  CosSin cs;
+  rows.gather(a.axes.map, part, cs);
+#pragma unroll
+  for (int i = 0; i < kLanes; ++i) cs.s[i] *= a.sign;
+#pragma unroll
+  for (int i = 0; i < kHeads; ++i) {
+    if (head[i] == nullptr) continue;
+    rotate8(x1[i], x2[i], cs);
+    *reinterpret_cast<uint4*>(head[i]) = x1[i];
+    *reinterpret_cast<uint4*>(head[i] + kHalf) = x2[i];
+  }
+}
+
+// Into new tensors: whole heads are read and written, one a thread group of
+// four (eight 16-byte loads in flight a thread).  A token whose position is out
+// of range is copied as it is.
+__global__ void __launch_bounds__(kBlock) rope_multi_axis_copy_kernel(const MultiAxisArgs a) {
   const int item = blockIdx.x * blockDim.x + threadIdx.x;
   const int part = item & (kParts - 1);
   const int row = item >> kPartShift;
@@ -36,18 +86,14 @@ __global__ void __launch_bounds__(kBlock) rope_multi_axis_kernel(const MultiAxis
   const int x = head >= a.q_heads;
   const int h = x ? head - a.q_heads : head;
   const uint16_t* src = a.src[x] + tok * a.src_token[x] + h * a.src_head[x];
+  if (item < a.items) prefetch_line(src + part * 64);
   pdl_enter();
   if (item >= a.items) return;
-  WholeHead piece;
-  if (kCopy) {
-    piece.load(src, part);
-  } else {
-    piece.x1 = *reinterpret_cast<const uint4*>(src + kRopeLane0 + part * kLanes);
-    piece.x2 = *reinterpret_cast<const uint4*>(src + kRopeLane0 + kHalf + part * kLanes);
-  }
   AxisRows rows;
-  const bool ok = rows.load(a.axes, tok);
-  if (ok) {
+  rows.load(a.axes, tok);
+  WholeHead piece;
+  piece.load(src, part);
+  if (rows.ready(a.axes)) {
     CosSin cs;
     rows.gather(a.axes.map, part, cs);
 #pragma unroll
@@ -56,13 +102,7 @@ __global__ void __launch_bounds__(kBlock) rope_multi_axis_kernel(const MultiAxis
   } else if (part == 0 && head == 0) {
     raise_status(a.status, WELM_ROPE_DEV_BAD_POSITION);
   }
-  uint16_t* dst = a.dst[x] + tok * a.dst_token[x] + h * a.dst_head[x];
-  if (kCopy) {
-    piece.store(dst, part);
-  } else if (ok) {
-    *reinterpret_cast<uint4*>(dst + kRopeLane0 + part * kLanes) = piece.x1;
-    *reinterpret_cast<uint4*>(dst + kRopeLane0 + kHalf + part * kLanes) = piece.x2;
-  }
+  piece.store(a.dst[x] + tok * a.dst_token[x] + h * a.dst_head[x], part);
 }
 
 }  // namespace
@@ -117,12 +157,22 @@ int welm_rope_multi_axis(const void* q, void* q_out, const void* k, void* k_out,
   a.status = device_status;
   a.heads = int32_t(heads);
   a.q_heads = int32_t(num_q_heads);
-  a.items = int32_t(n_tokens * heads * kParts);
   a.sign = inverse ? -1.0f : 1.0f;
-  const unsigned grid = unsigned((int64_t(a.items) + kBlock - 1) / kBlock);
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return in_place ? launch(rope_multi_axis_kernel<false>, grid, kBlock, 0, s, a)
-                  : launch(rope_multi_axis_kernel<true>, grid, kBlock, 0, s, a);
+  auto grid = [&](int64_t rows) {
+    a.items = int32_t(rows * kParts);
+    return unsigned((rows * kParts + kBlock - 1) / kBlock);
+  };
+  if (!in_place) {
+    const unsigned ctas = grid(n_tokens * heads);
+    return launch(rope_multi_axis_copy_kernel, ctas, kBlock, 0, s, a);
+  }
+  if (n_tokens * heads <= kOneHeadRows) {
+    const unsigned ctas = grid(n_tokens * heads);
+    return launch(rope_multi_axis_kernel<1>, ctas, kBlock, 0, s, a);
+  }
+  const unsigned ctas = grid(n_tokens * ((heads + 3) / 4));
+  return launch(rope_multi_axis_kernel<4>, ctas, kBlock, 0, s, a);
 }
 
 }  // extern "C"
