@@ -19,10 +19,10 @@
 // do not depend on timing.  Lengths stay on the device: every CTA adds the
 // requests' tiles up for itself, and a captured launch follows new lengths.
 //
-// One CTA on an SM, twelve warps:
+// One CTA on an SM, thirteen warps:
 //   0      TMA producer: K and V, half a tile (128 keys x 128 lanes, 32 KB) at
 //          a time, into a ring of five
-//   1      issues tcgen05.mma: S = Q K^T (128 x 128) and O += P V (128 x 256)
+//   1, 12  issue tcgen05.mma: S = Q K^T (128 x 128), and O += P V (128 x 256)
 //   2      brings the piece's Q rows into shared memory (64 KB)
 //   3      lists the CTA's pieces
 //   4..11  softmax: two threads a row, 64 keys each; rescaling of O; results
@@ -50,9 +50,9 @@ constexpr int kQBytes = kRows * kHeadDim * 2;
 // 24.2, 26.5, 26.9, 29.4; 256 requests over 32768 keys 82.4, 83.3, 84.7, 84.9, 96.2.
 constexpr int kItemCost = 2;
 constexpr int kPieces = 4;             // ring of piece descriptors
-constexpr int kThreads = 384;
+constexpr int kThreads = 416;
 constexpr int kSoftmaxWarp0 = 4, kSoftmaxWarps = 8;
-constexpr int kPieceReaders = 3 + kSoftmaxWarps;  // producer, issuer, Q warp, softmax warps
+constexpr int kPieceReaders = 4 + kSoftmaxWarps;  // producer, two issuers, Q warp, softmax warps
 constexpr uint32_t kColS = 0, kColO = 256;  // TMEM columns: S (and P) of even and odd tiles, then O
 constexpr long long kWaitClocks = 1ll << 32;  // about two seconds
 constexpr float kRescaleStep = 8.0f;   // O is rescaled when the maximum grows by more than 2^8
@@ -213,7 +213,7 @@ struct Piece {
 struct Control {
   uint64_t full[kStages], empty[kStages];
   uint64_t s_full[2], p_full[2], pv_done[2];
-  uint64_t q_full, q_empty, o_free, drained;
+  uint64_t q_full, q_empty, o_free, drained[2];
   uint64_t swap[4];  // the two warps of 32 rows
   uint64_t piece_full[kPieces], piece_empty[kPieces];
   Piece piece[kPieces];
@@ -520,89 +520,111 @@ __device__ void produce(const AttendArgs& a, Control& ctl, const CUtensorMap* km
   }
 }
 
-__device__ void issue_products(Control& ctl, uint32_t q, uint32_t ring, uint32_t tmem) {
-  constexpr uint32_t kIdescS = instr_desc(kKeys, false), kIdescO = instr_desc(kHalfLanes, true);
-  constexpr uint32_t kFull = 0xffffffffu;
+// Waits until both halves of a tile of K or V have landed in the ring.
+__device__ __forceinline__ bool landed(Control& ctl, uint32_t entry) {
+  return mbar_wait(ctl, &ctl.full[entry % kStages], (entry / kStages) & 1) &&
+         mbar_wait(ctl, &ctl.full[(entry + 1) % kStages], ((entry + 1) / kStages) & 1);
+}
+
+// No product may outlive the TMEM or the shared memory it works on.
+__device__ __forceinline__ void drain(uint64_t* bar) {
+  if (elect_one()) mma_commit(bar);
+  __syncwarp();
+  const long long t0 = clock64();
+  while (!mbar_poll(bar, 0) && clock64() - t0 < kWaitClocks) {
+  }
+}
+
+// Two warps issue the products, so that what one waits for does not hold up the
+// other's.  One warp for both left the tensor cores idle for about 1200 of 3900
+// clocks a tile (both waits take some 300 clocks even when they are over).
+//
+// S(t) = Q K(t)^T, once P(t - 2), which takes the same columns, has been used.
+__device__ void issue_scores(Control& ctl, uint32_t q, uint32_t ring, uint32_t tmem) {
+  constexpr uint32_t kIdesc = instr_desc(kKeys, false);
   const uint64_t q_desc = operand_desc(q, 16, 1024);
   PieceReader pieces;
   Piece p;
-  uint32_t base = 0;   // ring entries before this piece, in whole tiles of K or V
-  uint32_t tile = 0;   // tiles before this piece
-  for (uint32_t np = 0; pieces.next(ctl, p); ++np) {
-    if (!__all_sync(kFull, mbar_wait(ctl, &ctl.q_full, np & 1))) break;
-    // the Q rows came by ordinary asynchronous copies
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  uint32_t base = 0;  // ring entries before this piece, in whole tiles of K or V
+  uint32_t t = 0;     // tiles so far
+  bool ok = true;
+  for (uint32_t np = 0; ok && pieces.next(ctl, p); ++np) {
     const int tiles = int(uniform(p.tiles));
-    bool ok = true;
-    // Both halves of a tile of K or V; what the ring already holds is waited for
-    // before what the products before it decide.
-    auto landed = [&](uint32_t e) {
-      return mbar_wait(ctl, &ctl.full[e % kStages], (e / kStages) & 1) &&
-             mbar_wait(ctl, &ctl.full[(e + 1) % kStages], ((e + 1) / kStages) & 1);
-    };
-    for (int j = 0; j <= tiles; ++j) {
-      if (j < tiles) {  // S(j) = Q K(j)^T, once P(j - 2) in its place has been used
-        const uint32_t t = tile + j, buf = t & 1, e = 2 * (base + ring_k(j));
-        ok = landed(e) && (t < 2 || mbar_wait(ctl, &ctl.pv_done[buf], ((t >> 1) & 1) ^ 1));
-        if (!__all_sync(kFull, ok)) break;
-        tmem_fence_after();
-        const uint32_t s0 = uniform(e % kStages), s1 = uniform((e + 1) % kStages);
-        const uint64_t k_desc[2] = {operand_desc(ring + s0 * kStageBytes, 16, 1024),
-                                    operand_desc(ring + s1 * kStageBytes, 16, 1024)};
-        const uint32_t d = tmem + kColS + buf * kKeys;
-        if (elect_one()) {
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-              for (int kk = 0; kk < 4; ++kk)
-                mma_ss(d, q_desc + (((2 * half + c) * kQChunkBytes + kk * 32) >> 4),
-                       k_desc[half] + ((c * kChunkBytes + kk * 32) >> 4), kIdescS, half + c + kk > 0);
-            mma_commit(&ctl.empty[half == 0 ? s0 : s1]);
-          }
-          mma_commit(&ctl.s_full[buf]);
-          if (j == tiles - 1) mma_commit(&ctl.q_empty);
-        }
-        __syncwarp();
+    for (int j = 0; j < tiles; ++j, ++t) {
+      const uint32_t e = 2 * (base + ring_k(j)), buf = t & 1;
+      const uint32_t s0 = uniform(e % kStages), s1 = uniform((e + 1) % kStages);
+      const uint64_t k_desc[2] = {operand_desc(ring + s0 * kStageBytes, 16, 1024),
+                                  operand_desc(ring + s1 * kStageBytes, 16, 1024)};
+      const uint32_t d = tmem + kColS + buf * kKeys;
+      ok = landed(ctl, e);
+      if (j == 0) {
+        ok = ok && mbar_wait(ctl, &ctl.q_full, np & 1);
+        // the Q rows came by ordinary asynchronous copies
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
-      if (j > 0) {  // O += P(j-1) V(j-1)
-        const int jv = j - 1;
-        const uint32_t t = tile + jv, buf = t & 1, e = 2 * (base + ring_v(jv, tiles));
-        ok = landed(e) && (jv > 0 || mbar_wait(ctl, &ctl.o_free, (np & 1) ^ 1)) &&
-             mbar_wait(ctl, &ctl.p_full[buf], (t >> 1) & 1);
-        if (!__all_sync(kFull, ok)) break;
-        tmem_fence_after();
-        const uint32_t s0 = uniform(e % kStages), s1 = uniform((e + 1) % kStages);
-        const uint64_t v_desc[2] = {operand_desc(ring + s0 * kStageBytes, kChunkBytes, 1024),
-                                    operand_desc(ring + s1 * kStageBytes, kChunkBytes, 1024)};
-        // P: keys 0..63 in the first 32 columns of S, keys 64..127 in those from column 64
-        const uint32_t p_at = tmem + kColS + buf * kKeys;
-        if (elect_one()) {
+      ok = __all_sync(0xffffffffu, ok && (t < 2 || mbar_wait(ctl, &ctl.pv_done[buf], ((t >> 1) & 1) ^ 1)));
+      if (!ok) break;
+      tmem_fence_after();
+      if (elect_one()) {
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
+        for (int half = 0; half < 2; ++half) {
 #pragma unroll
-            for (int ks = 0; ks < kKeys / 16; ++ks)
-              mma_ts(tmem + kColO + half * kHalfLanes, p_at + (ks >> 2) * 64 + (ks & 3) * 8,
-                     v_desc[half] + ((ks * 16 * 128) >> 4), kIdescO, jv > 0 || ks > 0);
-            mma_commit(&ctl.empty[half == 0 ? s0 : s1]);
-          }
-          mma_commit(&ctl.pv_done[buf]);
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              mma_ss(d, q_desc + (((2 * half + c) * kQChunkBytes + kk * 32) >> 4),
+                     k_desc[half] + ((c * kChunkBytes + kk * 32) >> 4), kIdesc, half + c + kk > 0);
+          if (half == 0) mma_commit(&ctl.empty[s0]);
         }
-        __syncwarp();
+        mma_commit(&ctl.s_full[buf]);
+        mma_commit(&ctl.empty[s1]);
+        if (j == tiles - 1) mma_commit(&ctl.q_empty);
       }
+      __syncwarp();
     }
-    ok = __all_sync(kFull, ok);
-    if (!ok) break;
     base += 2 * tiles;
-    tile += tiles;
   }
-  // no product may outlive the TMEM or the shared memory it works on
-  if (elect_one()) mma_commit(&ctl.drained);
-  __syncwarp();
-  const long long t0 = clock64();
-  while (!mbar_poll(&ctl.drained, 0) && clock64() - t0 < kWaitClocks) {
+  drain(&ctl.drained[0]);
+}
+
+// O += P(t) V(t).
+__device__ void issue_values(Control& ctl, uint32_t ring, uint32_t tmem) {
+  constexpr uint32_t kIdesc = instr_desc(kHalfLanes, true);
+  PieceReader pieces;
+  Piece p;
+  uint32_t base = 0, t = 0;
+  bool ok = true;
+  for (uint32_t np = 0; ok && pieces.next(ctl, p); ++np) {
+    const int tiles = int(uniform(p.tiles));
+    for (int j = 0; j < tiles; ++j, ++t) {
+      const uint32_t e = 2 * (base + ring_v(j, tiles)), buf = t & 1;
+      const uint32_t s0 = uniform(e % kStages), s1 = uniform((e + 1) % kStages);
+      const uint64_t v_desc[2] = {operand_desc(ring + s0 * kStageBytes, kChunkBytes, 1024),
+                                  operand_desc(ring + s1 * kStageBytes, kChunkBytes, 1024)};
+      // P: keys 0..63 in the first 32 columns of S, keys 64..127 in those from column 64
+      const uint32_t p_at = tmem + kColS + buf * kKeys;
+      ok = landed(ctl, e) && (j > 0 || mbar_wait(ctl, &ctl.o_free, (np & 1) ^ 1)) &&
+           mbar_wait(ctl, &ctl.p_full[buf], (t >> 1) & 1);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tmem_fence_after();
+      if (elect_one()) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+          for (int ks = 0; ks < kKeys / 16; ++ks)
+            mma_ts(tmem + kColO + half * kHalfLanes, p_at + (ks >> 2) * 64 + (ks & 3) * 8,
+                   v_desc[half] + ((ks * 16 * 128) >> 4), kIdesc, j > 0 || ks > 0);
+          if (half == 0) mma_commit(&ctl.empty[s0]);
+        }
+        mma_commit(&ctl.pv_done[buf]);
+        mma_commit(&ctl.empty[s1]);
+      }
+      __syncwarp();
+    }
+    base += 2 * tiles;
   }
+  drain(&ctl.drained[1]);
 }
 
 // Q rows of each piece: one row of 512 bytes a warp instruction, into the
@@ -845,7 +867,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(&ctl.q_full, 32);
     mbar_init(&ctl.q_empty, 1);
     mbar_init(&ctl.o_free, kSoftmaxWarps);
-    mbar_init(&ctl.drained, 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&ctl.drained[i], 1);
     for (int i = 0; i < 4; ++i) mbar_init(&ctl.swap[i], 2);
     for (int i = 0; i < kPieces; ++i) {
       mbar_init(&ctl.piece_full[i], 1);
@@ -913,13 +935,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 0) {
       produce(a, ctl, &kmap, &vmap, ring_at);
     } else if (warp == 1) {
-      issue_products(ctl, q_at, ring_at, uniform(tmem));
+      issue_scores(ctl, q_at, ring_at, uniform(tmem));
     } else if (warp == 2) {
       load_queries(a, ctl, q_at);
     } else if (warp == 3) {
       list_pieces(a, ctl, line, blockIdx.x, used, pre);
-    } else {
+    } else if (warp < kSoftmaxWarp0 + kSoftmaxWarps) {
       softmax_rows(a, ctl, swap, ring, tmem);
+    } else {
+      issue_values(ctl, ring_at, uniform(tmem));
     }
   }
   tmem_fence_before();
