@@ -24,7 +24,7 @@
 //          a time, into a ring of five
 //   1, 12  issue tcgen05.mma: S = Q K^T (128 x 128), and O += P V (128 x 256)
 //   2      brings the piece's Q rows into shared memory (64 KB)
-//   3      lists the CTA's pieces
+//   3      adds up the line and lists the CTA's pieces
 //   4..11  softmax: two threads a row, 64 keys each; rescaling of O; results
 // S and O live in TMEM, S twice, so that the softmax of one tile runs beside
 // the products of its neighbours; P (BF16) takes the place of S.  P is rounded
@@ -64,7 +64,7 @@ struct Divisor {
   uint32_t mul = 0;
   int32_t shift = 0, d = 1;
   Divisor() = default;
-  explicit Divisor(int64_t by) : d(int32_t(by)) {
+  __host__ __device__ explicit Divisor(int64_t by) : d(int32_t(by)) {
     int log = 0;
     while ((int64_t(1) << log) < by) ++log;
     shift = 31 + log;
@@ -92,7 +92,8 @@ struct AttendArgs {
   int32_t grid;
   int32_t fill;                 // 1: rows of no request become zeros
   float scale;                  // times log2(e)
-  int32_t* units_before;        // [batch + 1] units of the own items before each request
+  struct LineNote* note;        // what the join needs of the line
+  int32_t* units_before;        // [batch] units of the own items before each request
   // Partial results.  O is laid out [32][rows][8 lanes]: the threads of a warp,
   // a row each, then write (and a row's reader reads) whole 32-byte sectors.
   float* slot_ml;               // [2 grid][slot_rows][2]
@@ -147,23 +148,20 @@ struct Request {
   }
 };
 
-__device__ __forceinline__ Request load_request(const AttendArgs& a, int b, bool tell) {
-  Request r;
-  int64_t lo = b, hi = b + 1;
-  bool good = true;
-  if (a.query_starts != nullptr) {
-    const int64_t s0 = __ldg(a.query_starts + b), s1 = __ldg(a.query_starts + b + 1);
-    lo = clamp64(s0, 0, a.tokens);
-    hi = clamp64(s1, lo, a.tokens);
-    good = lo == s0 && hi == s1;
+// A request as the device arrays have it, and checked.
+struct RawRequest {
+  int64_t start, end, len;
+  __device__ __forceinline__ void load(const AttendArgs& a, int b) {
+    start = a.query_starts != nullptr ? __ldg(a.query_starts + b) : b;
+    end = a.query_starts != nullptr ? __ldg(a.query_starts + b + 1) : b + 1;
+    len = __ldg(a.seq_lens + b);
   }
-  const int64_t n = __ldg(a.seq_lens + b);
-  r.first = int(lo);
-  r.count = int(hi - lo);
-  r.len = int(clamp64(n, 0, a.max_len));
-  if (tell && !(good && r.len == n)) raise_status(a.status, WELM_ROPE_DEV_BAD_LENGTH);
-  return r;
-}
+  __device__ __forceinline__ Request checked(const AttendArgs& a, bool tell) const {
+    const int64_t lo = clamp64(start, 0, a.tokens), hi = clamp64(end, lo, a.tokens), n = clamp64(len, 0, a.max_len);
+    if (tell && !(lo == start && hi == end && n == len)) raise_status(a.status, WELM_ROPE_DEV_BAD_LENGTH);
+    return Request{int(lo), int(hi - lo), int(n)};
+  }
+};
 
 // Query tokens in use: those behind the last request are left alone.
 __device__ __forceinline__ int used_tokens(const AttendArgs& a) {
@@ -182,9 +180,15 @@ struct Line {
     more = n - each * grid;
   }
   __device__ __forceinline__ int begin(int c) const { return each * c + (c < more ? c : more); }
+};
+
+// The line as the join kernel reads it; divisions are by each and each + 1.
+struct LineNote {
+  int32_t pre, each, more;
+  Divisor by_each, by_longer;
   __device__ __forceinline__ int cta_of(int u) const {
     const int longer = more * (each + 1);
-    return u < longer ? u / (each + 1) : more + (u - longer) / each;
+    return u < longer ? by_longer.of(u) : more + by_each.of(u - longer);
   }
 };
 
@@ -217,9 +221,6 @@ struct Control {
   uint64_t swap[4];  // the two warps of 32 rows
   uint64_t piece_full[kPieces], piece_empty[kPieces];
   Piece piece[kPieces];
-  int32_t scan[kThreads / 32];
-  int32_t start_units;
-  int32_t start_request;
   uint32_t tmem;
   int32_t failed;
 };
@@ -358,9 +359,44 @@ struct PieceReader {
   }
 };
 
-// Lists the pieces of this CTA's run of tiles.
-__device__ void list_pieces(const AttendArgs& a, Control& ctl, const Line& line, int cta, int used, int pre) {
-  const int lane = threadIdx.x & 31;
+// Adds up the requests' units, finds where this CTA's run begins and lists the
+// run's pieces; CTA 0 also notes the line for the join.  One warp does it all, a
+// request a lane, while the others get ready.
+__device__ void list_pieces(const AttendArgs& a, Control& ctl) {
+  const int lane = threadIdx.x & 31, cta = blockIdx.x;
+  const int used = used_tokens(a);
+  const int key_tiles = div_up(a.prefix_len, kKeys), row_tiles = div_up(used * a.group, kRows);
+  const int pre = prefix_units(a, used);
+  // The 32 requests from `held` on, one a lane: its units, and with those before it in the 32.
+  Request mine{0, 0, 0};
+  int held = 0, my_units = 0, my_sum = 0;
+  auto hold = [&](int b0) {
+    held = b0;
+    mine = Request{0, 0, 0};
+    if (b0 + lane < a.batch) {
+      RawRequest raw;
+      raw.load(a, b0 + lane);
+      mine = raw.checked(a, false);
+    }
+    my_units = my_sum = mine.all_units(a) * a.k_heads;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, my_sum, d);
+      if (lane >= d) my_sum += x;
+    }
+  };
+  int total = 0;
+  for (int b0 = lane; b0 < a.batch; b0 += 256) {  // eight loads in flight
+    RawRequest raw[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (b0 + 32 * i < a.batch) raw[i].load(a, b0 + 32 * i);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (b0 + 32 * i < a.batch) total += raw[i].checked(a, cta == 0).all_units(a) * a.k_heads;
+  }
+  total = __reduce_add_sync(0xffffffffu, total);
+  const Line line(pre + total, a.grid);
   int n = 0;
   // every lane holds the piece; lane 0 writes it
   auto emit = [&](const Piece& p) {
@@ -374,11 +410,11 @@ __device__ void list_pieces(const AttendArgs& a, Control& ctl, const Line& line,
     ++n;
     return true;
   };
-  int u = line.begin(cta);
-  const int end = line.begin(cta + 1);
-  const int key_tiles = div_up(a.prefix_len, kKeys);
-  const int row_tiles = div_up(used * a.group, kRows);
-  while (u < end && u < pre) {
+  const bool works = cta < line.grid;
+  bool ok = true;
+  int u = works ? line.begin(cta) : 0;
+  const int end = works ? line.begin(cta + 1) : 0;
+  while (ok && u < end && u < pre) {
     const int item = u / (key_tiles + kItemCost);
     const int at = u - item * (key_tiles + kItemCost), step = min(end - u, key_tiles + kItemCost - at);
     u += step;
@@ -396,52 +432,74 @@ __device__ void list_pieces(const AttendArgs& a, Control& ctl, const Line& line,
     p.table_row = 0;
     p.to = p.tiles == key_tiles ? kToPart : kToSlot;
     p.slot = 2 * cta + (p.first_tile > 0 ? 0 : 1);
-    if (!emit(p)) return;
+    ok = emit(p);
   }
-  int base = ctl.start_units + pre;  // of request `start_request`
-  for (int b0 = ctl.start_request; u < end && b0 < a.batch; b0 += 32) {
-    Request mine{0, 0, 0};
-    if (b0 + lane < a.batch) mine = load_request(a, b0 + lane, false);
-    for (int i = 0; i < 32 && u < end && b0 + i < a.batch; ++i) {
-      const Request r{__shfl_sync(0xffffffffu, mine.first, i), __shfl_sync(0xffffffffu, mine.count, i),
-                      __shfl_sync(0xffffffffu, mine.len, i)};
-      const int rts = r.row_tiles(a);
-      int rt = 0;
-      if (rts > 1 && u > base) {  // the last row tile that begins at or before u
-        int hi = rts;
-        while (hi - rt > 1) {
-          const int mid = (rt + hi) >> 1;
-          if (base + a.k_heads * r.units_before(a, mid) <= u) rt = mid; else hi = mid;
-        }
-        base += a.k_heads * r.units_before(a, rt);
+  int held_base = pre;  // units before the 32 requests in hand
+  if (u < end) hold(0);
+  while (ok && u < end) {
+    const uint32_t past = __ballot_sync(0xffffffffu, u < held_base + my_sum);
+    if (past == 0) {  // none of these 32
+      held_base += __shfl_sync(0xffffffffu, my_sum, 31);
+      if (held + 32 >= a.batch) break;
+      hold(held + 32);
+      continue;
+    }
+    const int i = __ffs(past) - 1, b = held + i;
+    int base = held_base + __shfl_sync(0xffffffffu, my_sum - my_units, i);  // of request b
+    const Request r{__shfl_sync(0xffffffffu, mine.first, i), __shfl_sync(0xffffffffu, mine.count, i),
+                    __shfl_sync(0xffffffffu, mine.len, i)};
+    const int rts = r.row_tiles(a);
+    int rt = 0;
+    if (rts > 1 && u > base) {  // the last row tile that begins at or before u
+      int hi = rts;
+      while (hi - rt > 1) {
+        const int mid = (rt + hi) >> 1;
+        if (base + a.k_heads * r.units_before(a, mid) <= u) rt = mid; else hi = mid;
       }
-      for (; rt < rts && u < end; ++rt) {
-        const int t = r.tiles(a, rt), cost = t > 0 ? t + kItemCost : 0;
-        for (int h = 0; h < a.k_heads && u < end; ++h, base += cost) {
-          if (u >= base + cost) continue;
-          const int at = u - base, step = min(end - u, cost - at);
-          u += step;
-          Piece p;
-          p.first_tile = max(at - kItemCost, 0);
-          p.tiles = at + step - kItemCost - p.first_tile;
-          if (p.tiles <= 0) continue;
-          p.keys = r.seen(a, rt);
-          p.head = h;
-          p.row0 = rt * kRows;
-          p.rows = min(r.count * a.group - p.row0, kRows);
-          p.first = r.first;
-          p.seen0 = r.len - r.count + 1;
-          p.own = 1;
-          p.table_row = b0 + i;
-          p.to = p.tiles < t ? kToSlot : a.prefix_len > 0 ? kToPart : kToOutput;
-          p.slot = 2 * cta + (p.first_tile > 0 ? 0 : 1);
-          if (!emit(p)) return;
-        }
+      base += a.k_heads * r.units_before(a, rt);
+    }
+    for (; ok && rt < rts && u < end; ++rt) {
+      const int t = r.tiles(a, rt), cost = t > 0 ? t + kItemCost : 0;
+      for (int h = 0; ok && h < a.k_heads && u < end; ++h, base += cost) {
+        if (u >= base + cost) continue;
+        const int at = u - base, step = min(end - u, cost - at);
+        u += step;
+        Piece p;
+        p.first_tile = max(at - kItemCost, 0);
+        p.tiles = at + step - kItemCost - p.first_tile;
+        if (p.tiles <= 0) continue;
+        p.keys = r.seen(a, rt);
+        p.head = h;
+        p.row0 = rt * kRows;
+        p.rows = min(r.count * a.group - p.row0, kRows);
+        p.first = r.first;
+        p.seen0 = r.len - r.count + 1;
+        p.own = 1;
+        p.table_row = b;
+        p.to = p.tiles < t ? kToSlot : a.prefix_len > 0 ? kToPart : kToOutput;
+        p.slot = 2 * cta + (p.first_tile > 0 ? 0 : 1);
+        ok = emit(p);
       }
     }
   }
-  Piece last{};
-  emit(last);
+  if (ok) emit(Piece{});
+  if (cta != 0) return;
+  // for the join: every request's place on the line
+  int before = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += 32) {
+    hold(b0);
+    if (b0 + lane < a.batch) a.units_before[b0 + lane] = before + my_sum - my_units;
+    before += __shfl_sync(0xffffffffu, my_sum, 31);
+  }
+  if (lane == 0) {
+    LineNote note;
+    note.pre = pre;
+    note.each = line.each;
+    note.more = line.more;
+    note.by_each = Divisor(max(line.each, 1));
+    note.by_longer = Divisor(line.each + 1);
+    *a.note = note;
+  }
 }
 
 // Order of a piece's tiles in the ring: K0, K1, V0, K2, V1, ..., V(n-1), each
@@ -584,7 +642,7 @@ __device__ void issue_scores(Control& ctl, uint32_t q, uint32_t ring, uint32_t t
     }
     base += 2 * tiles;
   }
-  drain(&ctl.drained[0]);
+  if (t > 0) drain(&ctl.drained[0]);
 }
 
 // O += P(t) V(t).
@@ -624,7 +682,7 @@ __device__ void issue_values(Control& ctl, uint32_t ring, uint32_t tmem) {
     }
     base += 2 * tiles;
   }
-  drain(&ctl.drained[1]);
+  if (t > 0) drain(&ctl.drained[1]);
 }
 
 // Q rows of each piece: one row of 512 bytes a warp instruction, into the
@@ -841,11 +899,6 @@ __device__ void softmax_rows(const AttendArgs& a, Control& ctl, Swap& swap, uint
   }
 }
 
-// Units of a request's own items.
-__device__ __forceinline__ int request_units(const AttendArgs& a, int b, bool tell) {
-  return load_request(a, b, tell).all_units(a) * a.k_heads;
-}
-
 __global__ void __launch_bounds__(kThreads, 1)
     rope_attend_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                        const __grid_constant__ AttendArgs a) {
@@ -853,7 +906,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* ring = smem + kQBytes;
   Swap& swap = *reinterpret_cast<Swap*>(ring + kStages * kStageBytes);
   Control& ctl = *reinterpret_cast<Control*>(&swap + 1);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = tid >> 5;
   if (tid == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&ctl.full[s], 1);
@@ -885,66 +938,20 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tmem_fence_after();
   pdl_enter();
-  // Where this CTA's run begins: each thread adds up a stretch of requests.
-  const int used = used_tokens(a);
-  const int pre = prefix_units(a, used);
-  const int stretch = div_up(a.batch, kThreads);
-  const int b0 = min(tid * stretch, a.batch), b1 = min(b0 + stretch, a.batch);
-  const bool writer = blockIdx.x == 0;
-  int sum = 0;
-  for (int b = b0; b < b1; ++b) sum += request_units(a, b, writer);
-  int incl = sum;
-  for (int d = 1; d < 32; d <<= 1) {
-    const int x = __shfl_up_sync(0xffffffffu, incl, d);
-    if (lane >= d) incl += x;
-  }
-  if (lane == 31) ctl.scan[warp] = incl;
-  if (tid == 0) {
-    ctl.start_request = a.batch;
-    ctl.start_units = 0;
-  }
-  __syncthreads();
-  int before = incl - sum, total = 0;
-  for (int w = 0; w < kThreads / 32; ++w) {
-    if (w < warp) before += ctl.scan[w];
-    total += ctl.scan[w];
-  }
-  const Line line(pre + total, a.grid);
-  const bool works = int(blockIdx.x) < line.grid;
-  if (works) {
-    const int want = max(line.begin(blockIdx.x) - pre, 0);
-    const bool find = want >= before && want < before + sum;
-    if (find || writer) {
-      int u = before;
-      for (int b = b0; b < b1; ++b) {
-        const int n = request_units(a, b, false);
-        if (find && want >= u && want < u + n) {
-          ctl.start_request = b;
-          ctl.start_units = u;
-        }
-        if (writer) a.units_before[b] = u;
-        u += n;
-      }
-    }
-  }
-  if (writer && tid == 0) a.units_before[a.batch] = total;
-  __syncthreads();
   const uint32_t tmem = ctl.tmem;
-  if (works) {
-    const uint32_t q_at = smem_u32(smem), ring_at = smem_u32(ring);
-    if (warp == 0) {
-      produce(a, ctl, &kmap, &vmap, ring_at);
-    } else if (warp == 1) {
-      issue_scores(ctl, q_at, ring_at, uniform(tmem));
-    } else if (warp == 2) {
-      load_queries(a, ctl, q_at);
-    } else if (warp == 3) {
-      list_pieces(a, ctl, line, blockIdx.x, used, pre);
-    } else if (warp < kSoftmaxWarp0 + kSoftmaxWarps) {
-      softmax_rows(a, ctl, swap, ring, tmem);
-    } else {
-      issue_values(ctl, ring_at, uniform(tmem));
-    }
+  const uint32_t q_at = smem_u32(smem), ring_at = smem_u32(ring);
+  if (warp == 0) {
+    produce(a, ctl, &kmap, &vmap, ring_at);
+  } else if (warp == 1) {
+    issue_scores(ctl, q_at, ring_at, uniform(tmem));
+  } else if (warp == 2) {
+    load_queries(a, ctl, q_at);
+  } else if (warp == 3) {
+    list_pieces(a, ctl);
+  } else if (warp < kSoftmaxWarp0 + kSoftmaxWarps) {
+    softmax_rows(a, ctl, swap, ring, tmem);
+  } else {
+    issue_values(ctl, ring_at, uniform(tmem));
   }
   tmem_fence_before();
   __syncthreads();
@@ -969,7 +976,22 @@ struct RowParts {
   int token, head;
 };
 
-__device__ __forceinline__ RowParts find_parts(const AttendArgs& a, int flat) {
+// The last request that starts at or before `token`, found by the whole CTA.
+__device__ __forceinline__ int find_request(const AttendArgs& a, int token, int& shared) {
+  if (a.query_starts == nullptr) return token;
+  if (threadIdx.x == 0) shared = 0;
+  __syncthreads();
+  int last = -1;
+  for (int b = threadIdx.x; b < a.batch; b += blockDim.x)
+    if (__ldg(a.query_starts + b) <= token) last = b;
+  last = __reduce_max_sync(0xffffffffu, last);
+  if ((threadIdx.x & 31) == 0 && last > 0) atomicMax(&shared, last);
+  __syncthreads();
+  return shared;
+}
+
+// `b`: a request that begins at or before the row's token, not far before.
+__device__ __forceinline__ RowParts find_parts(const AttendArgs& a, int flat, int b) {
   const int used = used_tokens(a);
   RowParts r{};
   if (flat >= a.tokens * a.q_heads) return r;
@@ -977,28 +999,28 @@ __device__ __forceinline__ RowParts find_parts(const AttendArgs& a, int flat) {
   const int h = a.by_group.of(hq), g = hq - h * a.group;
   r.token = token;
   r.head = hq;
-  int b = token;  // the row's request: the last that starts at or before the token
-  if (a.query_starts != nullptr) {
-    int lo = 0, hi = a.batch;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (__ldg(a.query_starts + mid) <= token) lo = mid; else hi = mid;
-    }
-    b = lo;
+  if (a.query_starts == nullptr) {
+    b = token;
+  } else {
+    while (b + 1 < a.batch && __ldg(a.query_starts + b + 1) <= token) ++b;
   }
   Request q{0, 0, 0};
-  if (token < used) q = load_request(a, b, false);
+  if (token < used) {
+    RawRequest raw;
+    raw.load(a, b);
+    q = raw.checked(a, false);
+  }
   if (token < q.first || token >= q.first + q.count) {  // a row of no request
     r.live = a.fill;
     return r;
   }
-  const int pre = prefix_units(a, used);
-  const Line line(pre + a.units_before[a.batch], a.grid);
+  const LineNote note = *a.note;
+  const int pre = note.pre;
   auto place = [&](int x, int first, int tiles, int in_tile) {
     r.in_tile[x] = in_tile;
     if (tiles == 0) return;
-    r.cta[x] = line.cta_of(first + kItemCost);
-    r.count[x] = line.cta_of(first + kItemCost + tiles - 1) - r.cta[x] + 1;
+    r.cta[x] = note.cta_of(first + kItemCost);
+    r.count[x] = note.cta_of(first + kItemCost + tiles - 1) - r.cta[x] + 1;
   };
   if (pre > 0) {
     const int packed = token * a.group + g, key_tiles = div_up(a.prefix_len, kKeys);
@@ -1039,11 +1061,13 @@ __global__ void __launch_bounds__(kGroups == 1 ? 256 : 128 * kGroups)
     rope_attend_join_kernel(const __grid_constant__ AttendArgs a) {
   constexpr int kRowsPerCta = kGroups == 1 ? 32 : 4, kUnroll = 4;
   __shared__ RowParts parts[kRowsPerCta];
+  __shared__ int s_request;
   __shared__ float s_o[kGroups == 1 ? 1 : kGroups - 1][kGroups == 1 ? 1 : 10][128];
   const int grp = threadIdx.x >> 7, in_grp = threadIdx.x & 127;
   const int lanes8 = in_grp >> 2;  // eight lanes of the head
   pdl_enter();
-  if (threadIdx.x < kRowsPerCta) parts[threadIdx.x] = find_parts(a, blockIdx.x * kRowsPerCta + threadIdx.x);
+  const int request = find_request(a, a.by_q_heads.of(blockIdx.x * kRowsPerCta), s_request);
+  if (threadIdx.x < kRowsPerCta) parts[threadIdx.x] = find_parts(a, blockIdx.x * kRowsPerCta + threadIdx.x, request);
   __syncthreads();
   const int64_t all = int64_t(a.tokens) * a.q_heads;
   for (int row = (kGroups == 1 ? 4 * grp : 0) + (in_grp & 3); row < kRowsPerCta; row += 8) {
@@ -1117,7 +1141,7 @@ __global__ void __launch_bounds__(kGroups == 1 ? 256 : 128 * kGroups)
 // ---------------------------------------------------------------------------
 // Layout of the workspace, in bytes from its base.
 struct Workspace {
-  int64_t units, slot_ml, slot_o, part_ml, part_o, bytes;
+  int64_t note, units, slot_ml, slot_o, part_ml, part_o, bytes;
 };
 
 Workspace attend_workspace(int64_t tokens, int64_t batch, int64_t q_heads, int64_t group, int64_t prefix_len,
@@ -1127,8 +1151,10 @@ Workspace attend_workspace(int64_t tokens, int64_t batch, int64_t q_heads, int64
   const int64_t slots = 2 * grid * rows;
   const int64_t parts = prefix_len > 0 ? 2 * tokens * q_heads : 0;
   Workspace w;
-  w.units = 0;
-  w.slot_ml = up((batch + 1) * 4);
+  w.note = 0;
+  w.units = 256;
+  static_assert(sizeof(LineNote) <= 256, "line note");
+  w.slot_ml = w.units + up(batch * 4);
   w.slot_o = w.slot_ml + up(slots * 8);
   w.part_ml = w.slot_o + up(slots * kHeadDim * 4);
   w.part_o = w.part_ml + up(parts * 8);
@@ -1277,6 +1303,7 @@ int welm_rope_attend(const void* q, void* out, float* lse, const void* key_cache
   a.fill = int32_t(fill_unused);
   a.scale = scale * 1.4426950408889634f;
   char* base = static_cast<char*>(workspace);
+  a.note = reinterpret_cast<LineNote*>(base + w.note);
   a.units_before = reinterpret_cast<int32_t*>(base + w.units);
   a.slot_ml = reinterpret_cast<float*>(base + w.slot_ml);
   a.slot_o = reinterpret_cast<float*>(base + w.slot_o);
