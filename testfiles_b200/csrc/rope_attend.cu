@@ -1019,8 +1019,10 @@ __device__ __forceinline__ RowParts find_parts(const AttendArgs& a, int flat, in
   auto place = [&](int x, int first, int tiles, int in_tile) {
     r.in_tile[x] = in_tile;
     if (tiles == 0) return;
-    r.cta[x] = note.cta_of(first + kItemCost);
-    r.count[x] = note.cta_of(first + kItemCost + tiles - 1) - r.cta[x] + 1;
+    // Within the line whatever is read here: lengths that another stream changes
+    // between the two kernels give wrong rows, but no address outside the workspace.
+    r.cta[x] = min(note.cta_of(first + kItemCost), a.grid - 1);
+    r.count[x] = min(note.cta_of(first + kItemCost + tiles - 1), a.grid - 1) - r.cta[x] + 1;
   };
   if (pre > 0) {
     const int packed = token * a.group + g, key_tiles = div_up(a.prefix_len, kKeys);
