@@ -597,6 +597,14 @@ __device__ __forceinline__ void drain(uint64_t* bar) {
 // other's.  One warp for both left the tensor cores idle for about 1200 of 3900
 // clocks a tile (both waits take some 300 clocks even when they are over).
 //
+// A wait for a stage's next phase returns at once while the phase before that
+// one is still open.  So an issuer looks at a stage only when it knows that the
+// stage's last contents, which may have been the other issuer's, had landed:
+// with five stages an entry of the order above follows, in its stages, the two
+// and three entries before it.  For K(t) these are K(t - 1), an older K, or V of
+// a tile up to t - 2, which pv_done(t - 2) proves used; for V(t) they are K up
+// to t, which p_full(t) proves used, or an older V.
+//
 // S(t) = Q K(t)^T, once P(t - 2), which takes the same columns, has been used.
 __device__ void issue_scores(Control& ctl, uint32_t q, uint32_t ring, uint32_t tmem) {
   constexpr uint32_t kIdesc = instr_desc(kKeys, false);
@@ -614,13 +622,13 @@ __device__ void issue_scores(Control& ctl, uint32_t q, uint32_t ring, uint32_t t
       const uint64_t k_desc[2] = {operand_desc(ring + s0 * kStageBytes, 16, 1024),
                                   operand_desc(ring + s1 * kStageBytes, 16, 1024)};
       const uint32_t d = tmem + kColS + buf * kKeys;
-      ok = landed(ctl, e);
       if (j == 0) {
-        ok = ok && mbar_wait(ctl, &ctl.q_full, np & 1);
+        ok = mbar_wait(ctl, &ctl.q_full, np & 1);
         // the Q rows came by ordinary asynchronous copies
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
-      ok = __all_sync(0xffffffffu, ok && (t < 2 || mbar_wait(ctl, &ctl.pv_done[buf], ((t >> 1) & 1) ^ 1)));
+      ok = ok && (t < 2 || mbar_wait(ctl, &ctl.pv_done[buf], ((t >> 1) & 1) ^ 1)) && landed(ctl, e);
+      ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tmem_fence_after();
       if (elect_one()) {
@@ -661,8 +669,8 @@ __device__ void issue_values(Control& ctl, uint32_t ring, uint32_t tmem) {
                                   operand_desc(ring + s1 * kStageBytes, kChunkBytes, 1024)};
       // P: keys 0..63 in the first 32 columns of S, keys 64..127 in those from column 64
       const uint32_t p_at = tmem + kColS + buf * kKeys;
-      ok = landed(ctl, e) && (j > 0 || mbar_wait(ctl, &ctl.o_free, (np & 1) ^ 1)) &&
-           mbar_wait(ctl, &ctl.p_full[buf], (t >> 1) & 1);
+      ok = (j > 0 || mbar_wait(ctl, &ctl.o_free, (np & 1) ^ 1)) && mbar_wait(ctl, &ctl.p_full[buf], (t >> 1) & 1) &&
+           landed(ctl, e);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
       tmem_fence_after();

@@ -255,3 +255,37 @@ def test_division_by_multiplication():
         for x in [0, 1, d - 1, d, d + 1, 2 ** 31 - 1, (2 ** 31 - 1) // d * d - 1, (2 ** 31 - 1) // d * d]:
             if 0 <= x < 2 ** 31:
                 assert (x * mul) >> (31 + log) == x // d
+
+
+def test_a_stage_is_looked_at_only_when_its_last_contents_are_known_to_have_landed():
+    """A parity wait returns at once while the phase before the one it is meant for is still open.  For every order of
+    pieces: what the waits before prove covers the last entry in each stage that an issuer, or a softmax warp that
+    clears V rows, looks at."""
+    stages, per_tile = 5, 2
+    rng = random.Random(3)
+    for _ in range(300):
+        pieces = [rng.choice([1, 1, 2, 3, rng.randint(1, 9)]) for _ in range(rng.randint(1, 8))]
+        order = []  # (is V, tile counted over all pieces) of each entry
+        first = 0
+        for n in pieces:
+            entries = {}
+            for j in range(n):
+                entries[0 if j == 0 else 2 * j - 1] = (False, first + j)
+                entries[2 * j + 2 if j + 1 < n else 2 * n - 1] = (True, first + j)
+            order += [entries[i] for i in range(2 * n)]
+            first += n
+        where = {entry: i for i, entry in enumerate(order)}
+        starts = {sum(pieces[:i]) for i in range(len(pieces))}
+        for (is_v, t), i in where.items():
+            for part in range(per_tile):
+                before = i * per_tile + part - stages
+                if before < 0:
+                    continue
+                last_v, last_t = order[before // per_tile]
+                if is_v:  # behind p_full(t): S(t) and so K(t) are done; the issuer itself took V before t
+                    assert last_t < t if last_v else last_t <= t
+                    # a softmax warp at tile t: K(t) used, V up to t - 2 used, at a piece's start V(t - 1) too
+                    if t + 1 in starts or t + 1 == first:  # the piece's last tile may be short
+                        assert last_t <= (t - 1 if t in starts else t - 2) if last_v else last_t <= t
+                else:  # behind pv_done(t - 2); the issuer itself took K before t
+                    assert last_t <= t - 2 if last_v else last_t < t
