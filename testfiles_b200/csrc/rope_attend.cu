@@ -19,12 +19,12 @@
 // do not depend on timing.  Lengths stay on the device: every CTA adds the
 // requests' tiles up for itself, and a captured launch follows new lengths.
 //
-// One CTA on an SM, thirteen warps:
-//   0      TMA producer: K and V, half a tile (128 keys x 128 lanes, 32 KB) at
-//          a time, into a ring of five
-//   1, 12  issue tcgen05.mma: S = Q K^T (128 x 128), and O += P V (128 x 256)
-//   2      brings the piece's Q rows into shared memory (64 KB)
-//   3      adds up the line and lists the CTA's pieces
+// One CTA on an SM, twelve warps:
+//   0      TMA producer: K and V, half a tile (32 KB) at a time, into rings of
+//          three and two
+//   1, 2   issue tcgen05.mma: S = Q K^T (128 x 128), and O += P V (128 x 256)
+//   3      adds up the line, lists the CTA's pieces and brings their Q rows into
+//          shared memory (64 KB)
 //   4..11  softmax: two threads a row, 64 keys each; rescaling of O; results
 // S and O live in TMEM, S twice, so that the softmax of one tile runs beside
 // the products of its neighbours; P (BF16) takes the place of S.  P is rounded
@@ -38,7 +38,11 @@ namespace {
 constexpr int kRows = 128;             // query rows of an item
 constexpr int kKeys = 128;             // keys of a tile
 constexpr int kHalfLanes = kHeadDim / 2;   // lanes of half a K or V tile
-constexpr int kStages = 5;             // ring of halves of K and V tiles
+// Halves of K and V tiles in shared memory.  Each ring has one warp that fills it
+// and one that empties it, each in order, so nobody looks at a stage before its
+// last contents have landed.
+constexpr int kStagesK = 3, kStagesV = 2;
+constexpr int kHalfKeys = kKeys / 2;  // keys of half a V tile
 constexpr int kChunkBytes = kKeys * 128;   // 64 lanes of 128 keys
 constexpr int kStageBytes = 2 * kChunkBytes;
 constexpr int kQChunkBytes = kRows * 128;  // 64 lanes of 128 rows
@@ -50,9 +54,9 @@ constexpr int kQBytes = kRows * kHeadDim * 2;
 // 24.2, 26.5, 26.9, 29.4; 256 requests over 32768 keys 82.4, 83.3, 84.7, 84.9, 96.2.
 constexpr int kItemCost = 2;
 constexpr int kPieces = 4;             // ring of piece descriptors
-constexpr int kThreads = 416;
+constexpr int kThreads = 384;
 constexpr int kSoftmaxWarp0 = 4, kSoftmaxWarps = 8;
-constexpr int kPieceReaders = 4 + kSoftmaxWarps;  // producer, two issuers, Q warp, softmax warps
+constexpr int kPieceReaders = 3 + kSoftmaxWarps;  // producer, two issuers, softmax warps
 constexpr uint32_t kColS = 0, kColO = 256;  // TMEM columns: S (and P) of even and odd tiles, then O
 constexpr long long kWaitClocks = 1ll << 32;  // about two seconds
 constexpr float kRescaleStep = 8.0f;   // O is rescaled when the maximum grows by more than 2^8
@@ -87,7 +91,7 @@ struct AttendArgs {
   Divisor by_group, by_block, by_q_heads;
   int32_t prefix_len, max_len;  // max_len: keys that a row of block_table can name
   int32_t block_size, num_blocks;
-  int32_t box_keys;             // keys of one TMA box: a power of two that divides block_size
+  int32_t box_k, box_v;         // keys of one TMA box: powers of two that divide block_size, up to 128 and 64
   int32_t slot_rows;            // rows of a workspace slot
   int32_t grid;
   int32_t fill;                 // 1: rows of no request become zeros
@@ -215,7 +219,7 @@ struct Piece {
 };
 
 struct Control {
-  uint64_t full[kStages], empty[kStages];
+  uint64_t full_k[kStagesK], empty_k[kStagesK], full_v[kStagesV], empty_v[kStagesV];
   uint64_t s_full[2], p_full[2], pv_done[2];
   uint64_t q_full, q_empty, o_free, drained[2];
   uint64_t swap[4];  // the two warps of 32 rows
@@ -231,7 +235,7 @@ struct Swap {
   float value[2][2][kRows];  // [tile parity][half]
 };
 
-constexpr int kSmemBytes = kQBytes + kStages * kStageBytes + sizeof(Swap) + 768;
+constexpr int kSmemBytes = kQBytes + (kStagesK + kStagesV) * kStageBytes + sizeof(Swap) + 768;
 static_assert(sizeof(Control) <= 768, "control block");
 static_assert(kSmemBytes <= 227 * 1024, "shared memory of one CTA");
 
@@ -359,10 +363,42 @@ struct PieceReader {
   }
 };
 
+// Q rows of a piece: one row of 512 bytes a warp instruction, into the 128-byte
+// swizzle that the products read.  Each lane works out the addresses of four
+// rows beforehand.  Rows past the item's stay as they are: a row of S and O
+// depends on its own Q row alone.
+__device__ __forceinline__ bool load_queries(const AttendArgs& a, Control& ctl, const Piece& p, uint32_t np,
+                                             uint32_t q) {
+  const int lane = threadIdx.x & 31;
+  const uint16_t* mine[kRows / 32];
+#pragma unroll
+  for (int i = 0; i < kRows / 32; ++i) {
+    const int in_item = p.row0 + min(i * 32 + lane, p.rows - 1);
+    const int tok = a.by_group.of(in_item);
+    mine[i] = a.q + (p.first + tok) * a.q_token + (p.head * a.group + in_item - tok * a.group) * a.q_head;
+  }
+  if (!__all_sync(0xffffffffu, mbar_wait(ctl, &ctl.q_empty, (np & 1) ^ 1))) return false;
+  const uint32_t to = q + (lane >> 3) * kQChunkBytes;
+#pragma unroll
+  for (int i = 0; i < kRows / 32; ++i) {
+    const int rows = min(p.rows - i * 32, 32);
+#pragma unroll 8
+    for (int r = 0; r < rows; ++r) {
+      const uint64_t src = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(mine[i]), r) + lane * 16;
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + (i * 32 + r) * 128 +
+                                                                     (((lane & 7) ^ (r & 7)) << 4)),
+                   "l"(src)
+                   : "memory");
+    }
+  }
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&ctl.q_full)) : "memory");
+  return true;
+}
+
 // Adds up the requests' units, finds where this CTA's run begins and lists the
 // run's pieces; CTA 0 also notes the line for the join.  One warp does it all, a
 // request a lane, while the others get ready.
-__device__ void list_pieces(const AttendArgs& a, Control& ctl) {
+__device__ void list_pieces(const AttendArgs& a, Control& ctl, uint32_t q) {
   const int lane = threadIdx.x & 31, cta = blockIdx.x;
   const int used = used_tokens(a);
   const int key_tiles = div_up(a.prefix_len, kKeys), row_tiles = div_up(used * a.group, kRows);
@@ -407,8 +443,10 @@ __device__ void list_pieces(const AttendArgs& a, Control& ctl) {
       ctl.piece[s] = p;
       mbar_arrive(&ctl.piece_full[s]);
     }
+    // this waits for the piece before: the other warps know one piece ahead
+    const bool loaded = p.tiles == 0 || load_queries(a, ctl, p, n, q);
     ++n;
-    return true;
+    return loaded;
   };
   const bool works = cta < line.grid;
   bool ok = true;
@@ -483,6 +521,7 @@ __device__ void list_pieces(const AttendArgs& a, Control& ctl) {
     }
   }
   if (ok) emit(Piece{});
+  asm volatile("cp.async.wait_all;" ::: "memory");
   if (cta != 0) return;
   // for the join: every request's place on the line
   int before = 0;
@@ -502,86 +541,102 @@ __device__ void list_pieces(const AttendArgs& a, Control& ctl) {
   }
 }
 
-// Order of a piece's tiles in the ring: K0, K1, V0, K2, V1, ..., V(n-1), each
-// as its lower and its upper 128 lanes.
-__device__ __forceinline__ int ring_k(int j) { return j == 0 ? 0 : 2 * j - 1; }
-__device__ __forceinline__ int ring_v(int j, int n) { return j + 1 < n ? 2 * j + 2 : 2 * n - 1; }
-
-// The producer warp.  A half tile is [2 chunks of 64 lanes][128 keys][128
-// bytes], filled by boxes of 64 lanes x box_keys keys: pages need not hold
-// whole tiles.  Lane g of the warp looks up the block of the tile's g-th box
-// of keys, one tile ahead, and issues that box's copies.
-__device__ void produce(const AttendArgs& a, Control& ctl, const CUtensorMap* kmap, const CUtensorMap* vmap,
-                        uint32_t ring) {
+// Where lane `lane`'s box of keys of a piece's tile j is in the cache; behind the
+// keys the block past the cache, whose box is filled with zeros.
+__device__ __forceinline__ void look_up(const AttendArgs& a, const Piece& p, const int32_t* table, int j, int box_keys,
+                                        int& block, int& place) {
   const int lane = threadIdx.x & 31;
-  const int boxes = kKeys / a.box_keys;
-  PieceReader pieces;
-  Piece p;
-  uint32_t n = 0;  // half tiles put into the ring
-  bool ok = true;
-  while (ok && pieces.next(ctl, p)) {
-    const int32_t* table = p.own ? a.block_table + p.table_row * a.table_stride : a.prefix_table;
-    // Block and place of this lane's box in tile j; behind the keys the block
-    // past the cache, whose box is filled with zeros.
-    auto look_up = [&](int j, int& block, int& place) {
-      const int key = (p.first_tile + j) * kKeys + lane * a.box_keys;
-      block = a.num_blocks;
-      place = 0;
-      if (j >= p.tiles || lane >= boxes || key >= p.keys) return;
-      const int page = a.by_block.of(key);
-      place = key - page * a.block_size;
-      block = __ldg(table + page);
-      if (block < 0 || block >= a.num_blocks) {
-        raise_status(a.status, WELM_ROPE_DEV_BAD_PAGE);
-        block = a.num_blocks;
-      }
-    };
-    auto load = [&](const CUtensorMap* map, int block, int place) {
-#pragma unroll 1
-      for (int half = 0; half < 2; ++half, ++n) {
-        const uint32_t s = n % kStages;
-        if (!__all_sync(0xffffffffu, mbar_wait(ctl, &ctl.empty[s], ((n / kStages) & 1) ^ 1))) return false;
-        if (lane == 0) mbar_arm(&ctl.full[s], kStageBytes);
-        __syncwarp();
-        if (lane < boxes) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c)
-            asm volatile(
-                "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
-                "%4, %5}], [%6];" ::"r"(ring + s * kStageBytes + c * kChunkBytes + lane * a.box_keys * 128),
-                "l"(map), "r"(half * kHalfLanes + c * 64), "r"(place), "r"(p.head), "r"(block),
-                "r"(smem_u32(&ctl.full[s]))
-                : "memory");
-        }
-      }
-      return true;
-    };
-    int block, place, block_v = 0, place_v = 0, block_next, place_next;
-    look_up(0, block, place);
-    for (int j = 0; j <= p.tiles && ok; ++j) {
-      look_up(j + 1, block_next, place_next);
-      if (j < p.tiles) ok = load(kmap, block, place);
-      if (ok && j > 0) ok = load(vmap, block_v, place_v);
-      block_v = block;
-      place_v = place;
-      block = block_next;
-      place = place_next;
-    }
+  const int key = (p.first_tile + j) * kKeys + lane * box_keys;
+  block = a.num_blocks;
+  place = 0;
+  if (j >= p.tiles || lane * box_keys >= kKeys || key >= p.keys) return;
+  const int page = a.by_block.of(key);
+  place = key - page * a.block_size;
+  block = __ldg(table + page);
+  if (block < 0 || block >= a.num_blocks) {
+    raise_status(a.status, WELM_ROPE_DEV_BAD_PAGE);
+    block = a.num_blocks;
   }
-  // after a failed wait, the copies in flight still have to land
-  if (*reinterpret_cast<volatile int32_t*>(&ctl.failed)) {
-    for (uint32_t i = n > kStages ? n - kStages : 0; i < n; ++i) {
-      const long long t0 = clock64();
-      while (!mbar_poll(&ctl.full[i % kStages], (i / kStages) & 1) && clock64() - t0 < kWaitClocks) {
-      }
+}
+
+// After a failed wait, the copies in flight still have to land.
+template <int kStages>
+__device__ __forceinline__ void await_copies(Control& ctl, uint64_t* full, uint32_t n) {
+  if (*reinterpret_cast<volatile int32_t*>(&ctl.failed) == 0) return;
+  for (uint32_t i = n > kStages ? n - kStages : 0; i < n; ++i) {
+    const long long t0 = clock64();
+    while (!mbar_poll(&full[i % kStages], (i / kStages) & 1) && clock64() - t0 < kWaitClocks) {
     }
   }
 }
 
-// Waits until both halves of a tile of K or V have landed in the ring.
-__device__ __forceinline__ bool landed(Control& ctl, uint32_t entry) {
-  return mbar_wait(ctl, &ctl.full[entry % kStages], (entry / kStages) & 1) &&
-         mbar_wait(ctl, &ctl.full[(entry + 1) % kStages], ((entry + 1) / kStages) & 1);
+// The producer warp.  Half a K tile is [2 chunks of 64 lanes][128 keys][128
+// bytes]: its products take all keys at once.  Half a V tile is 64 keys,
+// [boxes][4 chunks of 64 lanes][box_v keys][128 bytes]: one copy brings all
+// lanes of a box.  Lane g of the warp looks up the block of the tile's g-th box
+// of K, and of V, one tile ahead, and issues that box's copies.
+__device__ void produce(const AttendArgs& a, Control& ctl, const CUtensorMap* kmap, const CUtensorMap* vmap,
+                        uint32_t k_at, uint32_t v_at) {
+  const int lane = threadIdx.x & 31;
+  const int boxes_k = kKeys / a.box_k, boxes_v = kHalfKeys / a.box_v;
+  const int v_half = lane < boxes_v ? 0 : lane < 2 * boxes_v ? 1 : 2;  // the half of V that the lane's box is in
+  const uint32_t my_k = k_at + lane * a.box_k * 128;
+  const uint32_t my_v = v_at + (lane - v_half * boxes_v) * a.box_v * (kHeadDim * 2);
+  PieceReader pieces;
+  Piece p;
+  uint32_t nk = 0, nv = 0;  // halves so far
+  bool ok = true;
+  while (ok && pieces.next(ctl, p)) {
+    const int32_t* table = p.own ? a.block_table + p.table_row * a.table_stride : a.prefix_table;
+    int block_k, place_k, block_v = 0, place_v = 0, next_k, next_place_k, next_v, next_place_v;
+    look_up(a, p, table, 0, a.box_k, block_k, place_k);
+    for (int j = 0; j <= p.tiles && ok; ++j) {
+      look_up(a, p, table, j + 1, a.box_k, next_k, next_place_k);
+      look_up(a, p, table, j, a.box_v, next_v, next_place_v);
+      if (j < p.tiles) {
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half, ++nk) {
+          const uint32_t s = nk % kStagesK;
+          ok = ok && __all_sync(0xffffffffu, mbar_wait(ctl, &ctl.empty_k[s], ((nk / kStagesK) & 1) ^ 1));
+          if (!ok) break;
+          if (lane == 0) mbar_arm(&ctl.full_k[s], kStageBytes);
+          __syncwarp();
+          if (lane < boxes_k) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+              asm volatile(
+                  "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+                  "%3, %4, %5}], [%6];" ::"r"(my_k + s * kStageBytes + c * kChunkBytes),
+                  "l"(kmap), "r"(half * kHalfLanes + c * 64), "r"(place_k), "r"(p.head), "r"(block_k),
+                  "r"(smem_u32(&ctl.full_k[s]))
+                  : "memory");
+          }
+        }
+      }
+      if (j > 0) {
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half, ++nv) {
+          const uint32_t s = nv % kStagesV;
+          ok = ok && __all_sync(0xffffffffu, mbar_wait(ctl, &ctl.empty_v[s], ((nv / kStagesV) & 1) ^ 1));
+          if (!ok) break;
+          if (lane == 0) mbar_arm(&ctl.full_v[s], kStageBytes);
+          __syncwarp();
+          if (v_half == half)
+            asm volatile(
+                "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
+                "%2, %4, %5}], [%6];" ::"r"(my_v + s * kStageBytes),
+                "l"(vmap), "r"(0), "r"(place_v), "r"(p.head), "r"(block_v), "r"(smem_u32(&ctl.full_v[s]))
+                : "memory");
+        }
+      }
+      block_v = next_v;
+      place_v = next_place_v;
+      block_k = next_k;
+      place_k = next_place_k;
+    }
+  }
+  await_copies<kStagesK>(ctl, ctl.full_k, nk);
+  await_copies<kStagesV>(ctl, ctl.full_v, nv);
 }
 
 // No product may outlive the TMEM or the shared memory it works on.
@@ -594,16 +649,12 @@ __device__ __forceinline__ void drain(uint64_t* bar) {
 }
 
 // Two warps issue the products, so that what one waits for does not hold up the
-// other's.  One warp for both left the tensor cores idle for about 1200 of 3900
-// clocks a tile (both waits take some 300 clocks even when they are over).
+// other's (both waits take some 300 clocks even when they are over).
 //
-// A wait for a stage's next phase returns at once while the phase before that
-// one is still open.  So an issuer looks at a stage only when it knows that the
-// stage's last contents, which may have been the other issuer's, had landed:
-// with five stages an entry of the order above follows, in its stages, the two
-// and three entries before it.  For K(t) these are K(t - 1), an older K, or V of
-// a tile up to t - 2, which pv_done(t - 2) proves used; for V(t) they are K up
-// to t, which p_full(t) proves used, or an older V.
+// The products of a tile take 2050 clocks by themselves.  Beside the copies they
+// take some 2600: those of the scores read Q and K from shared memory at 128
+// bytes a clock, all that it has, so that a tile's 128 KB (Q, K), 64 KB (V) and
+// 128 KB of copies written make 2500.
 //
 // S(t) = Q K(t)^T, once P(t - 2), which takes the same columns, has been used.
 __device__ void issue_scores(Control& ctl, uint32_t q, uint32_t ring, uint32_t tmem) {
@@ -611,121 +662,88 @@ __device__ void issue_scores(Control& ctl, uint32_t q, uint32_t ring, uint32_t t
   const uint64_t q_desc = operand_desc(q, 16, 1024);
   PieceReader pieces;
   Piece p;
-  uint32_t base = 0;  // ring entries before this piece, in whole tiles of K or V
-  uint32_t t = 0;     // tiles so far
+  uint32_t t = 0, n = 0;  // tiles and halves of K so far
   bool ok = true;
   for (uint32_t np = 0; ok && pieces.next(ctl, p); ++np) {
     const int tiles = int(uniform(p.tiles));
-    for (int j = 0; j < tiles; ++j, ++t) {
-      const uint32_t e = 2 * (base + ring_k(j)), buf = t & 1;
-      const uint32_t s0 = uniform(e % kStages), s1 = uniform((e + 1) % kStages);
-      const uint64_t k_desc[2] = {operand_desc(ring + s0 * kStageBytes, 16, 1024),
-                                  operand_desc(ring + s1 * kStageBytes, 16, 1024)};
+    for (int j = 0; ok && j < tiles; ++j, ++t) {
+      const uint32_t buf = t & 1;
       const uint32_t d = tmem + kColS + buf * kKeys;
       if (j == 0) {
         ok = mbar_wait(ctl, &ctl.q_full, np & 1);
         // the Q rows came by ordinary asynchronous copies
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
-      ok = ok && (t < 2 || mbar_wait(ctl, &ctl.pv_done[buf], ((t >> 1) & 1) ^ 1)) && landed(ctl, e);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      tmem_fence_after();
-      if (elect_one()) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
+      for (int half = 0; half < 2; ++half, ++n) {
+        const uint32_t s = uniform(n % kStagesK);
+        const uint64_t k_desc = operand_desc(ring + s * kStageBytes, 16, 1024);
+        ok = ok && mbar_wait(ctl, &ctl.full_k[s], (n / kStagesK) & 1);
+        if (half == 0) ok = ok && (t < 2 || mbar_wait(ctl, &ctl.pv_done[buf], ((t >> 1) & 1) ^ 1));
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tmem_fence_after();
+        if (elect_one()) {
 #pragma unroll
           for (int c = 0; c < 2; ++c)
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
               mma_ss(d, q_desc + (((2 * half + c) * kQChunkBytes + kk * 32) >> 4),
-                     k_desc[half] + ((c * kChunkBytes + kk * 32) >> 4), kIdesc, half + c + kk > 0);
-          if (half == 0) mma_commit(&ctl.empty[s0]);
+                     k_desc + ((c * kChunkBytes + kk * 32) >> 4), kIdesc, half + c + kk > 0);
+          if (half == 1) mma_commit(&ctl.s_full[buf]);
+          mma_commit(&ctl.empty_k[s]);
+          if (half == 1 && j == tiles - 1) mma_commit(&ctl.q_empty);
         }
-        mma_commit(&ctl.s_full[buf]);
-        mma_commit(&ctl.empty[s1]);
-        if (j == tiles - 1) mma_commit(&ctl.q_empty);
+        __syncwarp();
       }
-      __syncwarp();
     }
-    base += 2 * tiles;
   }
   if (t > 0) drain(&ctl.drained[0]);
 }
 
 // O += P(t) V(t).
-__device__ void issue_values(Control& ctl, uint32_t ring, uint32_t tmem) {
-  constexpr uint32_t kIdesc = instr_desc(kHalfLanes, true);
+__device__ void issue_values(const AttendArgs& a, Control& ctl, uint32_t ring, uint32_t tmem) {
+  constexpr uint32_t kIdesc = instr_desc(kHeadDim, true);
+  // 16 keys, a product's, lie in one box, or in two boxes of eight
+  const uint32_t box = uniform(a.box_v);
+  const uint32_t lead = box * 128, stride = box > 8 ? 1024 : 4096;
+  const uint32_t per = box > 8 ? box / 16 : 1;  // products of a box
+  uint32_t at[kHalfKeys / 16];
+#pragma unroll
+  for (uint32_t ks = 0; ks < kHalfKeys / 16; ++ks) at[ks] = (ks / per * per * 16 * 512 + ks % per * 16 * 128) >> 4;
   PieceReader pieces;
   Piece p;
-  uint32_t base = 0, t = 0;
+  uint32_t t = 0, n = 0;
   bool ok = true;
   for (uint32_t np = 0; ok && pieces.next(ctl, p); ++np) {
     const int tiles = int(uniform(p.tiles));
-    for (int j = 0; j < tiles; ++j, ++t) {
-      const uint32_t e = 2 * (base + ring_v(j, tiles)), buf = t & 1;
-      const uint32_t s0 = uniform(e % kStages), s1 = uniform((e + 1) % kStages);
-      const uint64_t v_desc[2] = {operand_desc(ring + s0 * kStageBytes, kChunkBytes, 1024),
-                                  operand_desc(ring + s1 * kStageBytes, kChunkBytes, 1024)};
+    for (int j = 0; ok && j < tiles; ++j, ++t) {
+      const uint32_t buf = t & 1;
       // P: keys 0..63 in the first 32 columns of S, keys 64..127 in those from column 64
       const uint32_t p_at = tmem + kColS + buf * kKeys;
-      ok = (j > 0 || mbar_wait(ctl, &ctl.o_free, (np & 1) ^ 1)) && mbar_wait(ctl, &ctl.p_full[buf], (t >> 1) & 1) &&
-           landed(ctl, e);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      tmem_fence_after();
-      if (elect_one()) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
+      for (int half = 0; half < 2; ++half, ++n) {
+        const uint32_t s = uniform(n % kStagesV);
+        const uint64_t v_desc = operand_desc(ring + s * kStageBytes, lead, stride);
+        ok = ok && mbar_wait(ctl, &ctl.full_v[s], (n / kStagesV) & 1);
+        if (half == 0)
+          ok = ok && (j > 0 || mbar_wait(ctl, &ctl.o_free, (np & 1) ^ 1)) &&
+               mbar_wait(ctl, &ctl.p_full[buf], (t >> 1) & 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tmem_fence_after();
+        if (elect_one()) {
 #pragma unroll
-          for (int ks = 0; ks < kKeys / 16; ++ks)
-            mma_ts(tmem + kColO + half * kHalfLanes, p_at + (ks >> 2) * 64 + (ks & 3) * 8,
-                   v_desc[half] + ((ks * 16 * 128) >> 4), kIdesc, j > 0 || ks > 0);
-          if (half == 0) mma_commit(&ctl.empty[s0]);
+          for (int ks = 0; ks < kHalfKeys / 16; ++ks)
+            mma_ts(tmem + kColO, p_at + half * 64 + ks * 8, v_desc + at[ks], kIdesc, j + half + ks > 0);
+          if (half == 1) mma_commit(&ctl.pv_done[buf]);
+          mma_commit(&ctl.empty_v[s]);
         }
-        mma_commit(&ctl.pv_done[buf]);
-        mma_commit(&ctl.empty[s1]);
+        __syncwarp();
       }
-      __syncwarp();
     }
-    base += 2 * tiles;
   }
   if (t > 0) drain(&ctl.drained[1]);
-}
-
-// Q rows of each piece: one row of 512 bytes a warp instruction, into the
-// 128-byte swizzle that the products read.  Each lane works out the addresses
-// of four rows beforehand.  Rows past the item's stay as they are: a row of S
-// and O depends on its own Q row alone.
-__device__ void load_queries(const AttendArgs& a, Control& ctl, uint32_t q) {
-  const int lane = threadIdx.x & 31;
-  PieceReader pieces;
-  Piece p;
-  for (uint32_t np = 0; pieces.next(ctl, p); ++np) {
-    const uint16_t* mine[kRows / 32];
-#pragma unroll
-    for (int i = 0; i < kRows / 32; ++i) {
-      const int in_item = p.row0 + min(i * 32 + lane, p.rows - 1);
-      const int tok = a.by_group.of(in_item);
-      mine[i] = a.q + (p.first + tok) * a.q_token + (p.head * a.group + in_item - tok * a.group) * a.q_head;
-    }
-    if (!__all_sync(0xffffffffu, mbar_wait(ctl, &ctl.q_empty, (np & 1) ^ 1))) break;
-    const uint32_t to = q + (lane >> 3) * kQChunkBytes;
-#pragma unroll
-    for (int i = 0; i < kRows / 32; ++i) {
-      const int rows = min(p.rows - i * 32, 32);
-#pragma unroll 8
-      for (int r = 0; r < rows; ++r) {
-        const uint64_t src = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(mine[i]), r) + lane * 16;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + (i * 32 + r) * 128 +
-                                                                       (((lane & 7) ^ (r & 7)) << 4)),
-                     "l"(src)
-                     : "memory");
-      }
-    }
-    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&ctl.q_full)) : "memory");
-  }
-  asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 // Softmax of the tiles, rescaling of O, and the results.  Two threads hold a
@@ -741,7 +759,7 @@ __device__ void softmax_rows(const AttendArgs& a, Control& ctl, Swap& swap, uint
   const float c = a.scale;
   PieceReader pieces;
   Piece p;
-  uint32_t base = 0, tile = 0, swaps = 0;
+  uint32_t tile = 0, swaps = 0;
   // hands `value` to the row's other thread and returns that thread's
   auto trade = [&](float value, float& other) {
     const uint32_t parity = swaps & 1;
@@ -753,7 +771,7 @@ __device__ void softmax_rows(const AttendArgs& a, Control& ctl, Swap& swap, uint
     ++swaps;
     return true;
   };
-  for (; pieces.next(ctl, p); base += 2 * p.tiles, tile += p.tiles) {
+  for (; pieces.next(ctl, p); tile += p.tiles) {
     const bool busy = warp * 32 < p.rows;  // some lane of the warp has a row
     const int in_item = p.row0 + row;
     const int tok = a.by_group.of(in_item);
@@ -783,7 +801,8 @@ __device__ void softmax_rows(const AttendArgs& a, Control& ctl, Swap& swap, uint
         top = fmaxf(top, other);
         // The maximum in use only moves when it has grown enough to matter:
         // until then p stays at or below 2^8, well inside BF16 and FP32.
-        const bool grown = (top - m) * c > kRescaleStep;
+        // Rows past the item's, whose scores may be anything, do not ask for it.
+        const bool grown = row < p.rows && (top - m) * c > kRescaleStep;
         if (j > 0 && __any_sync(0xffffffffu, grown)) {
           const uint32_t tp = t - 1;
           if (!__all_sync(0xffffffffu, mbar_wait(ctl, &ctl.pv_done[tp & 1], (tp >> 1) & 1))) return;
@@ -823,15 +842,19 @@ __device__ void softmax_rows(const AttendArgs& a, Control& ctl, Swap& swap, uint
       // V rows past the keys weigh nothing, but what their page holds may be
       // no number, and 0 times that is none either: they are cleared.  Boxes
       // that begin behind the keys were filled with zeros.
-      const int whole = p.keys - (p.first_tile + j) * kKeys;
-      if (whole < kKeys) {
-        const uint32_t e = 2 * (base + ring_v(j, p.tiles)) + half, st = e % kStages;
-        if (!__all_sync(0xffffffffu, mbar_wait(ctl, &ctl.full[st], (e / kStages) & 1))) return;
-        uint8_t* v = ring + st * kStageBytes;
-        const int end = div_up(whole, a.box_keys) * a.box_keys;
-        for (int i = whole * 16 + row; i < end * 16; i += kRows)
-          *reinterpret_cast<uint4*>(v + ((i >> 3) & 1) * kChunkBytes + (i >> 4) * 128 + (i & 7) * 16) =
+      const int whole = p.keys - (p.first_tile + j) * kKeys - half * kHalfKeys;
+      if (whole < kHalfKeys) {
+        // V(t - 1), the stage's last contents, has landed if it has been used
+        if (t > 0 && !__all_sync(0xffffffffu, mbar_wait(ctl, &ctl.pv_done[buf ^ 1], ((t - 1) >> 1) & 1))) return;
+        const uint32_t n = 2 * t + half, st = n % kStagesV;
+        if (!__all_sync(0xffffffffu, mbar_wait(ctl, &ctl.full_v[st], (n / kStagesV) & 1))) return;
+        uint8_t* v = ring + (kStagesK + st) * kStageBytes;
+        const int begin = max(whole, 0), end = div_up(begin, a.box_v) * a.box_v;
+        for (int i = begin * 32 + row; i < end * 32; i += kRows) {
+          const int key = i >> 5, box = key & ~(a.box_v - 1);
+          *reinterpret_cast<uint4*>(v + box * 512 + ((i >> 3) & 3) * a.box_v * 128 + (key - box) * 128 + (i & 7) * 16) =
               make_uint4(0, 0, 0, 0);
+        }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
       tmem_fence_before();
@@ -912,13 +935,17 @@ __global__ void __launch_bounds__(kThreads, 1)
                        const __grid_constant__ AttendArgs a) {
   extern __shared__ __align__(1024) uint8_t smem[];  // the 128-byte swizzle repeats every 1024 bytes
   uint8_t* ring = smem + kQBytes;
-  Swap& swap = *reinterpret_cast<Swap*>(ring + kStages * kStageBytes);
+  Swap& swap = *reinterpret_cast<Swap*>(ring + (kStagesK + kStagesV) * kStageBytes);
   Control& ctl = *reinterpret_cast<Control*>(&swap + 1);
   const int tid = threadIdx.x, warp = tid >> 5;
   if (tid == 0) {
-    for (int s = 0; s < kStages; ++s) {
-      mbar_init(&ctl.full[s], 1);
-      mbar_init(&ctl.empty[s], 1);
+    for (int s = 0; s < kStagesK; ++s) {
+      mbar_init(&ctl.full_k[s], 1);
+      mbar_init(&ctl.empty_k[s], 1);
+    }
+    for (int s = 0; s < kStagesV; ++s) {
+      mbar_init(&ctl.full_v[s], 1);
+      mbar_init(&ctl.empty_v[s], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&ctl.s_full[i], 1);
@@ -947,19 +974,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   tmem_fence_after();
   pdl_enter();
   const uint32_t tmem = ctl.tmem;
-  const uint32_t q_at = smem_u32(smem), ring_at = smem_u32(ring);
+  const uint32_t q_at = smem_u32(smem), k_at = smem_u32(ring), v_at = k_at + kStagesK * kStageBytes;
   if (warp == 0) {
-    produce(a, ctl, &kmap, &vmap, ring_at);
+    produce(a, ctl, &kmap, &vmap, k_at, v_at);
   } else if (warp == 1) {
-    issue_scores(ctl, q_at, ring_at, uniform(tmem));
+    issue_scores(ctl, q_at, k_at, uniform(tmem));
   } else if (warp == 2) {
-    load_queries(a, ctl, q_at);
+    issue_values(a, ctl, v_at, uniform(tmem));
   } else if (warp == 3) {
-    list_pieces(a, ctl);
-  } else if (warp < kSoftmaxWarp0 + kSoftmaxWarps) {
-    softmax_rows(a, ctl, swap, ring, tmem);
+    list_pieces(a, ctl, q_at);
   } else {
-    issue_values(ctl, ring_at, uniform(tmem));
+    softmax_rows(a, ctl, swap, ring, tmem);
   }
   tmem_fence_before();
   __syncthreads();
@@ -1172,19 +1197,25 @@ Workspace attend_workspace(int64_t tokens, int64_t batch, int64_t q_heads, int64
   return w;
 }
 
-// Tensor map of a cache as {256 lanes, slot, head, block}, boxes of 64 lanes
-// and `box_keys` slots.
+// Tensor map of a cache.  K: {256 lanes, slot, head, block}, boxes of 64 lanes
+// and `box_keys` slots.  V: {64 lanes, slot, chunk of 64 lanes, head, block},
+// boxes of all lanes and `box_keys` slots.
 bool encode_cache_map(CUtensorMap& map, const void* base, int64_t blocks, int64_t block_size, int64_t heads,
-                      const int64_t* strides, int box_keys) {
+                      const int64_t* strides, int box_keys, bool chunks) {
   const PFN_cuTensorMapEncodeTiled_v12000 encode = tensor_map_encoder();
   if (encode == nullptr) return false;
-  const cuuint64_t dim[4] = {kHeadDim, cuuint64_t(block_size), cuuint64_t(heads), cuuint64_t(blocks)};
   // the stride of a dimension of one is not used, but has to be one
   auto step = [](int64_t extent, int64_t stride) { return cuuint64_t(extent > 1 ? stride : kHeadDim) * 2; };
-  const cuuint64_t stride[3] = {step(block_size, strides[1]), step(heads, strides[2]), step(blocks, strides[0])};
-  const cuuint32_t box[4] = {64, cuuint32_t(box_keys), 1, 1};
-  const cuuint32_t unit[4] = {1, 1, 1, 1};
-  return encode(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dim, stride, box, unit,
+  const cuuint64_t slot = step(block_size, strides[1]), head = step(heads, strides[2]);
+  const cuuint64_t block = step(blocks, strides[0]);
+  const cuuint64_t n = cuuint64_t(block_size), h = cuuint64_t(heads), b = cuuint64_t(blocks);
+  const cuuint64_t dim_k[4] = {kHeadDim, n, h, b}, dim_v[5] = {64, n, kHeadDim / 64, h, b};
+  const cuuint64_t stride_k[3] = {slot, head, block}, stride_v[4] = {slot, 128, head, block};
+  const cuuint32_t box_k[4] = {64, cuuint32_t(box_keys), 1, 1};
+  const cuuint32_t box_v[5] = {64, cuuint32_t(box_keys), kHeadDim / 64, 1, 1};
+  const cuuint32_t unit[5] = {1, 1, 1, 1, 1};
+  return encode(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, chunks ? 5 : 4, const_cast<void*>(base),
+                chunks ? dim_v : dim_k, chunks ? stride_v : stride_k, chunks ? box_v : box_k, unit,
                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -1244,7 +1275,8 @@ int welm_rope_attend(const void* q, void* out, float* lse, const void* key_cache
     return WELM_ROPE_ERR_BAD_SIZE;
   const __int128 row_tiles = (n_tokens * (num_q_heads / num_k_heads) + kRows - 1) / kRows;
   if ((row_tiles * ((prefix_len + kKeys - 1) / kKeys + kItemCost) +
-       (row_tiles + batch_size) * ((table_width * block_size + kKeys - 1) / kKeys + kItemCost)) * num_k_heads >= INT32_MAX)
+       (row_tiles + batch_size) * ((table_width * block_size + kKeys - 1) / kKeys + kItemCost)) * num_k_heads >=
+      INT32_MAX)
     return WELM_ROPE_ERR_BAD_SIZE;
   if (!(scale > 0.0f) || scale > 3.0e38f || (fill_unused != 0 && fill_unused != 1)) return WELM_ROPE_ERR_BAD_MODE;
   if (n_tokens == 0 || batch_size == 0) return WELM_ROPE_OK;
@@ -1279,8 +1311,9 @@ int welm_rope_attend(const void* q, void* out, float* lse, const void* key_cache
   int box = 8;
   while (box < kKeys && block_size % (2 * box) == 0) box *= 2;
   CUtensorMap kmap, vmap;
-  if (!encode_cache_map(kmap, key_cache, num_blocks, block_size, num_k_heads, key_cache_strides, box) ||
-      !encode_cache_map(vmap, value_cache, num_blocks, block_size, num_k_heads, value_cache_strides, box))
+  if (!encode_cache_map(kmap, key_cache, num_blocks, block_size, num_k_heads, key_cache_strides, box, false) ||
+      !encode_cache_map(vmap, value_cache, num_blocks, block_size, num_k_heads, value_cache_strides,
+                        box < kHalfKeys ? box : kHalfKeys, true))
     return WELM_ROPE_ERR_CUDA;
   AttendArgs a{};
   a.q = static_cast<const uint16_t*>(q);
@@ -1307,7 +1340,8 @@ int welm_rope_attend(const void* q, void* out, float* lse, const void* key_cache
   a.max_len = int32_t(table_width * block_size);
   a.block_size = int32_t(block_size);
   a.num_blocks = int32_t(num_blocks);
-  a.box_keys = box;
+  a.box_k = box;
+  a.box_v = box < kHalfKeys ? box : kHalfKeys;
   a.slot_rows = int32_t(n_tokens * group < kRows ? n_tokens * group : kRows);
   a.grid = sms;
   a.fill = int32_t(fill_unused);
