@@ -11,7 +11,9 @@
 // Work.  An item is 128 query rows (tokens x the query heads of one KV head)
 // against a run of keys.  The prefix's items take their rows from all requests
 // together, so a prefix key is read once for every 128 rows instead of once
-// for every request; a request's own items hold its own rows.  All items'
+// for every request; a request's own items hold its own rows.  Where requests
+// fill their row tiles by themselves that gains nothing, and an item is a
+// request's rows against the prefix and its own keys in one.  All items'
 // 128-key tiles form one line, cut into equal runs, one for each CTA; a CTA
 // walks the pieces of items in its run.  An item that is cut, or whose rows
 // also have the other part, leaves FP32 partial results in the workspace, and
@@ -48,10 +50,9 @@ constexpr int kStageBytes = 2 * kChunkBytes;
 constexpr int kQChunkBytes = kRows * 128;  // 64 lanes of 128 rows
 constexpr int kQBytes = kRows * kHeadDim * 2;
 // What an item costs beside its tiles (its Q rows, its results), in tiles.
-// Measured with 0, 1, 2, 3 and 6 on one B200 (graph replay, us): 2560 query
-// tokens over 8192 shared and 900 own keys, whose own items are short and
-// numerous, 171.7, 145.8, 130.5, 131.3, 136.0; 24 requests' verification 24.3,
-// 24.2, 26.5, 26.9, 29.4; 256 requests over 32768 keys 82.4, 83.3, 84.7, 84.9, 96.2.
+// Measured with 1, 2 and 3 on one B200 (graph replay, us): 128 requests over a
+// prefix 35.8, 34.9, 34.9; 24 requests' verification 24.8, 24.1, 24.6; 48
+// requests without a prefix 27.6, 27.4, 27.4.
 constexpr int kItemCost = 2;
 constexpr int kPieces = 4;             // ring of piece descriptors
 constexpr int kThreads = 384;
@@ -113,7 +114,8 @@ __device__ __forceinline__ int64_t clamp64(int64_t v, int64_t lo, int64_t hi) {
 }
 
 // One request's own part: `count` query tokens from token `first`, the last of
-// them at the last of `len` keys.
+// them at the last of `len` keys.  `joint` is the number of the prefix's key tiles
+// where its items hold the prefix too, and -1 where they do not.
 struct Request {
   int first, count, len;
   __device__ __forceinline__ int row_tiles(const AttendArgs& a) const { return div_up(count * a.group, kRows); }
@@ -138,17 +140,24 @@ struct Request {
     };
     return sum(rt + c) - sum(c);
   }
-  // Units of the line that one head's row tiles before rt take: their tiles,
-  // and kItemCost for each that has any (tile x has none while x + c < G).
-  __device__ __forceinline__ int units_before(const AttendArgs& a, int rt) const {
+  // Row tiles before rt that see own keys (tile x does not while x + c < G).
+  __device__ __forceinline__ int seeing_before(const AttendArgs& a, int rt) const {
     if (rt == 0) return 0;
     const int c = int((127 + int64_t(a.group) * (len - count + 128)) >> 7);
-    const int none = min(max(a.group - c, 0), rt);
-    return tiles_before(a, rt) + (rt - none) * kItemCost;
+    return rt - min(max(a.group - c, 0), rt);
   }
-  __device__ __forceinline__ int all_units(const AttendArgs& a) const {
+  // Units of the line that one head's row tiles before rt take: their tiles,
+  // and kItemCost for each that has any.
+  __device__ __forceinline__ int units_before(const AttendArgs& a, int rt, int joint) const {
+    return tiles_before(a, rt) + (joint >= 0 ? rt * (joint + kItemCost) : seeing_before(a, rt) * kItemCost);
+  }
+  __device__ __forceinline__ int all_units(const AttendArgs& a, int joint) const {
     const int n = row_tiles(a);
-    return n == 0 ? 0 : units_before(a, n - 1) + (len > 0 ? div_up(len, kKeys) + kItemCost : 0);
+    return n == 0 ? 0 : units_before(a, n - 1, joint) + units(len > 0 ? div_up(len, kKeys) : 0, joint);
+  }
+  // Units of an item with `tiles` own tiles.
+  static __device__ __forceinline__ int units(int tiles, int joint) {
+    return joint >= 0 ? joint + tiles + kItemCost : tiles > 0 ? tiles + kItemCost : 0;
   }
 };
 
@@ -188,7 +197,7 @@ struct Line {
 
 // The line as the join kernel reads it; divisions are by each and each + 1.
 struct LineNote {
-  int32_t pre, each, more;
+  int32_t pre, joint, each, more;
   Divisor by_each, by_longer;
   __device__ __forceinline__ int cta_of(int u) const {
     const int longer = more * (each + 1);
@@ -212,7 +221,8 @@ struct Piece {
   int32_t rows;
   int32_t first;       // token that rows are counted from
   int32_t seen0;       // keys that token `first` sees; a later token sees one more each, or `keys` in the prefix
-  int32_t own;         // 1: a request's own keys; 0: the prefix
+  int32_t own;         // 1: a request's own keys, behind the prefix's if the item has them; 0: the prefix
+  int32_t shared_tiles;  // the item's tiles of the prefix, which come first
   int32_t table_row;   // row of block_table
   int32_t to;          // Destination
   int32_t slot;
@@ -221,7 +231,7 @@ struct Piece {
 struct Control {
   uint64_t full_k[kStagesK], empty_k[kStagesK], full_v[kStagesV], empty_v[kStagesV];
   uint64_t s_full[2], p_full[2], pv_done[2];
-  uint64_t q_full, q_empty, o_free, drained[2];
+  uint64_t q_first, q_full, q_empty, o_free, drained[2];
   uint64_t swap[4];  // the two warps of 32 rows
   uint64_t piece_full[kPieces], piece_empty[kPieces];
   Piece piece[kPieces];
@@ -235,8 +245,8 @@ struct Swap {
   float value[2][2][kRows];  // [tile parity][half]
 };
 
-constexpr int kSmemBytes = kQBytes + (kStagesK + kStagesV) * kStageBytes + sizeof(Swap) + 768;
-static_assert(sizeof(Control) <= 768, "control block");
+constexpr int kSmemBytes = kQBytes + (kStagesK + kStagesV) * kStageBytes + sizeof(Swap) + 800;
+static_assert(sizeof(Control) <= 800, "control block");
 static_assert(kSmemBytes <= 227 * 1024, "shared memory of one CTA");
 
 // Waits for a phase of `bar`; false once any warp of the CTA has given up.
@@ -364,9 +374,26 @@ struct PieceReader {
 };
 
 // Q rows of a piece: one row of 512 bytes a warp instruction, into the 128-byte
-// swizzle that the products read.  Each lane works out the addresses of four
-// rows beforehand.  Rows past the item's stay as they are: a row of S and O
-// depends on its own Q row alone.
+// swizzle that the products read.  The softmax warps, which have nothing to do
+// yet, bring the first piece's rows, a share each; the listing warp brings those
+// of the pieces after it, with the addresses of four rows worked out by each lane
+// beforehand.  Rows past the item's stay as they are: a row of S and O depends
+// on its own Q row alone.
+__device__ __forceinline__ void load_first_queries(const AttendArgs& a, Control& ctl, const Piece& p, int warp,
+                                                   uint32_t q) {
+  const int lane = threadIdx.x & 31;
+  const uint32_t to = q + (lane >> 3) * kQChunkBytes;
+  const uint16_t* rows_at = a.q + p.first * a.q_token + p.head * a.group * a.q_head + lane * 8;
+#pragma unroll 4
+  for (int r = warp; r < p.rows; r += kSoftmaxWarps) {
+    const int in_item = p.row0 + r, tok = a.by_group.of(in_item);
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to + r * 128 + (((lane & 7) ^ (r & 7)) << 4)),
+                 "l"(rows_at + tok * a.q_token + (in_item - tok * a.group) * a.q_head)
+                 : "memory");
+  }
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&ctl.q_first)) : "memory");
+}
+
 __device__ __forceinline__ bool load_queries(const AttendArgs& a, Control& ctl, const Piece& p, uint32_t np,
                                              uint32_t q) {
   const int lane = threadIdx.x & 31;
@@ -402,10 +429,9 @@ __device__ void list_pieces(const AttendArgs& a, Control& ctl, uint32_t q) {
   const int lane = threadIdx.x & 31, cta = blockIdx.x;
   const int used = used_tokens(a);
   const int key_tiles = div_up(a.prefix_len, kKeys), row_tiles = div_up(used * a.group, kRows);
-  const int pre = prefix_units(a, used);
   // The 32 requests from `held` on, one a lane: its units, and with those before it in the 32.
   Request mine{0, 0, 0};
-  int held = 0, my_units = 0, my_sum = 0;
+  int held = 0, my_units = 0, my_sum = 0, joint = -1;
   auto hold = [&](int b0) {
     held = b0;
     mine = Request{0, 0, 0};
@@ -414,14 +440,14 @@ __device__ void list_pieces(const AttendArgs& a, Control& ctl, uint32_t q) {
       raw.load(a, b0 + lane);
       mine = raw.checked(a, false);
     }
-    my_units = my_sum = mine.all_units(a) * a.k_heads;
+    my_units = my_sum = mine.all_units(a, joint) * a.k_heads;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const int x = __shfl_up_sync(0xffffffffu, my_sum, d);
       if (lane >= d) my_sum += x;
     }
   };
-  int total = 0;
+  int total = 0, row_tiles_alone = 0, seeing = 0;
   for (int b0 = lane; b0 < a.batch; b0 += 256) {  // eight loads in flight
     RawRequest raw[8];
 #pragma unroll
@@ -429,10 +455,31 @@ __device__ void list_pieces(const AttendArgs& a, Control& ctl, uint32_t q) {
       if (b0 + 32 * i < a.batch) raw[i].load(a, b0 + 32 * i);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (b0 + 32 * i < a.batch) total += raw[i].checked(a, cta == 0).all_units(a) * a.k_heads;
+      if (b0 + 32 * i < a.batch) {
+        const Request r = raw[i].checked(a, cta == 0);
+        const int n = r.row_tiles(a);
+        total += r.all_units(a, -1);
+        row_tiles_alone += n;
+        seeing += n == 0 ? 0 : r.seeing_before(a, n - 1) + (r.len > 0);
+      }
   }
   total = __reduce_add_sync(0xffffffffu, total);
-  const Line line(pre + total, a.grid);
+  int pre = prefix_units(a, used);
+  if (pre > 0) {
+    // The shorter line: row tiles of all requests together against the prefix and of
+    // each against its own keys, or of each against both.  2560 query tokens of four
+    // requests over 8192 shared keys: 136 us apart, 119 in one, with no partial results
+    // but of cut items.
+    row_tiles_alone = __reduce_add_sync(0xffffffffu, row_tiles_alone);
+    seeing = __reduce_add_sync(0xffffffffu, seeing);
+    const int64_t both = int64_t(row_tiles_alone) * (key_tiles + kItemCost) - int64_t(seeing) * kItemCost;
+    if (both * a.k_heads <= pre) {
+      joint = key_tiles;
+      total += int(both);
+      pre = 0;
+    }
+  }
+  const Line line(pre + total * a.k_heads, a.grid);
   int n = 0;
   // every lane holds the piece; lane 0 writes it
   auto emit = [&](const Piece& p) {
@@ -444,7 +491,7 @@ __device__ void list_pieces(const AttendArgs& a, Control& ctl, uint32_t q) {
       mbar_arrive(&ctl.piece_full[s]);
     }
     // this waits for the piece before: the other warps know one piece ahead
-    const bool loaded = p.tiles == 0 || load_queries(a, ctl, p, n, q);
+    const bool loaded = n == 0 || p.tiles == 0 || load_queries(a, ctl, p, n, q);
     ++n;
     return loaded;
   };
@@ -467,6 +514,7 @@ __device__ void list_pieces(const AttendArgs& a, Control& ctl, uint32_t q) {
     p.first = 0;
     p.seen0 = a.prefix_len;
     p.own = 0;
+    p.shared_tiles = key_tiles;
     p.table_row = 0;
     p.to = p.tiles == key_tiles ? kToPart : kToSlot;
     p.slot = 2 * cta + (p.first_tile > 0 ? 0 : 1);
@@ -492,12 +540,12 @@ __device__ void list_pieces(const AttendArgs& a, Control& ctl, uint32_t q) {
       int hi = rts;
       while (hi - rt > 1) {
         const int mid = (rt + hi) >> 1;
-        if (base + a.k_heads * r.units_before(a, mid) <= u) rt = mid; else hi = mid;
+        if (base + a.k_heads * r.units_before(a, mid, joint) <= u) rt = mid; else hi = mid;
       }
-      base += a.k_heads * r.units_before(a, rt);
+      base += a.k_heads * r.units_before(a, rt, joint);
     }
     for (; ok && rt < rts && u < end; ++rt) {
-      const int t = r.tiles(a, rt), cost = t > 0 ? t + kItemCost : 0;
+      const int cost = Request::units(r.tiles(a, rt), joint);
       for (int h = 0; ok && h < a.k_heads && u < end; ++h, base += cost) {
         if (u >= base + cost) continue;
         const int at = u - base, step = min(end - u, cost - at);
@@ -513,8 +561,9 @@ __device__ void list_pieces(const AttendArgs& a, Control& ctl, uint32_t q) {
         p.first = r.first;
         p.seen0 = r.len - r.count + 1;
         p.own = 1;
+        p.shared_tiles = max(joint, 0);
         p.table_row = b;
-        p.to = p.tiles < t ? kToSlot : a.prefix_len > 0 ? kToPart : kToOutput;
+        p.to = p.tiles < cost - kItemCost ? kToSlot : pre > 0 ? kToPart : kToOutput;
         p.slot = 2 * cta + (p.first_tile > 0 ? 0 : 1);
         ok = emit(p);
       }
@@ -533,6 +582,7 @@ __device__ void list_pieces(const AttendArgs& a, Control& ctl, uint32_t q) {
   if (lane == 0) {
     LineNote note;
     note.pre = pre;
+    note.joint = joint;
     note.each = line.each;
     note.more = line.more;
     note.by_each = Divisor(max(line.each, 1));
@@ -541,23 +591,28 @@ __device__ void list_pieces(const AttendArgs& a, Control& ctl, uint32_t q) {
   }
 }
 
-// Where lane `lane`'s box of keys of a piece's tile j is in the cache; behind the
-// keys the block past the cache, whose box is filled with zeros.
-__device__ __forceinline__ void look_up(const AttendArgs& a, const Piece& p, const int32_t* table, int j, int box_keys,
-                                        int& block, int& place) {
-  const int lane = threadIdx.x & 31;
-  const int key = (p.first_tile + j) * kKeys + lane * box_keys;
-  block = a.num_blocks;
-  place = 0;
-  if (j >= p.tiles || lane * box_keys >= kKeys || key >= p.keys) return;
-  const int page = a.by_block.of(key);
-  place = key - page * a.block_size;
-  block = __ldg(table + page);
-  if (block < 0 || block >= a.num_blocks) {
-    raise_status(a.status, WELM_ROPE_DEV_BAD_PAGE);
-    block = a.num_blocks;
+// Where a box of keys is in the cache.  The block is looked at when its copies
+// are issued, a tile after it was asked for, and not as soon as it is there.
+struct BoxPlace {
+  int block = 0, place = 0;
+  bool keys = false;  // some row sees keys of the box
+  __device__ __forceinline__ void ask(const AttendArgs& a, const Piece& p, const int32_t* own, int j, int box_keys) {
+    const int tile = p.first_tile + j, at = (threadIdx.x & 31) * box_keys;
+    const bool shared = tile < p.shared_tiles;
+    const int key = (shared ? tile : tile - p.shared_tiles) * kKeys + at;
+    keys = j < p.tiles && at < kKeys && key < (shared ? a.prefix_len : p.keys);
+    if (!keys) return;
+    const int page = a.by_block.of(key);
+    place = key - page * a.block_size;
+    block = __ldg((shared ? a.prefix_table : own) + page);
   }
-}
+  // The block past the cache, whose box is filled with zeros, for boxes behind the keys and blocks that do not exist.
+  __device__ __forceinline__ int checked(const AttendArgs& a) const {
+    const bool there = uint32_t(block) < uint32_t(a.num_blocks);
+    if (keys && !there) raise_status(a.status, WELM_ROPE_DEV_BAD_PAGE);
+    return keys && there ? block : a.num_blocks;
+  }
+};
 
 // After a failed wait, the copies in flight still have to land.
 template <int kStages>
@@ -587,13 +642,14 @@ __device__ void produce(const AttendArgs& a, Control& ctl, const CUtensorMap* km
   uint32_t nk = 0, nv = 0;  // halves so far
   bool ok = true;
   while (ok && pieces.next(ctl, p)) {
-    const int32_t* table = p.own ? a.block_table + p.table_row * a.table_stride : a.prefix_table;
-    int block_k, place_k, block_v = 0, place_v = 0, next_k, next_place_k, next_v, next_place_v;
-    look_up(a, p, table, 0, a.box_k, block_k, place_k);
+    const int32_t* own = a.block_table + p.table_row * a.table_stride;
+    BoxPlace at_k, at_v, next_k, next_v;
+    at_k.ask(a, p, own, 0, a.box_k);
     for (int j = 0; j <= p.tiles && ok; ++j) {
-      look_up(a, p, table, j + 1, a.box_k, next_k, next_place_k);
-      look_up(a, p, table, j, a.box_v, next_v, next_place_v);
+      next_k.ask(a, p, own, j + 1, a.box_k);
+      next_v.ask(a, p, own, j, a.box_v);
       if (j < p.tiles) {
+        const int block = at_k.checked(a);
 #pragma unroll 1
         for (int half = 0; half < 2; ++half, ++nk) {
           const uint32_t s = nk % kStagesK;
@@ -607,13 +663,14 @@ __device__ void produce(const AttendArgs& a, Control& ctl, const CUtensorMap* km
               asm volatile(
                   "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
                   "%3, %4, %5}], [%6];" ::"r"(my_k + s * kStageBytes + c * kChunkBytes),
-                  "l"(kmap), "r"(half * kHalfLanes + c * 64), "r"(place_k), "r"(p.head), "r"(block_k),
+                  "l"(kmap), "r"(half * kHalfLanes + c * 64), "r"(at_k.place), "r"(p.head), "r"(block),
                   "r"(smem_u32(&ctl.full_k[s]))
                   : "memory");
           }
         }
       }
       if (j > 0) {
+        const int block = at_v.checked(a);
 #pragma unroll 1
         for (int half = 0; half < 2; ++half, ++nv) {
           const uint32_t s = nv % kStagesV;
@@ -625,14 +682,12 @@ __device__ void produce(const AttendArgs& a, Control& ctl, const CUtensorMap* km
             asm volatile(
                 "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, "
                 "%2, %4, %5}], [%6];" ::"r"(my_v + s * kStageBytes),
-                "l"(vmap), "r"(0), "r"(place_v), "r"(p.head), "r"(block_v), "r"(smem_u32(&ctl.full_v[s]))
+                "l"(vmap), "r"(0), "r"(at_v.place), "r"(p.head), "r"(block), "r"(smem_u32(&ctl.full_v[s]))
                 : "memory");
         }
       }
-      block_v = next_v;
-      place_v = next_place_v;
-      block_k = next_k;
-      place_k = next_place_k;
+      at_k = next_k;
+      at_v = next_v;
     }
   }
   await_copies<kStagesK>(ctl, ctl.full_k, nk);
@@ -670,7 +725,7 @@ __device__ void issue_scores(Control& ctl, uint32_t q, uint32_t ring, uint32_t t
       const uint32_t buf = t & 1;
       const uint32_t d = tmem + kColS + buf * kKeys;
       if (j == 0) {
-        ok = mbar_wait(ctl, &ctl.q_full, np & 1);
+        ok = np == 0 ? mbar_wait(ctl, &ctl.q_first, 0) : mbar_wait(ctl, &ctl.q_full, (np & 1) ^ 1);
         // the Q rows came by ordinary asynchronous copies
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
@@ -749,7 +804,8 @@ __device__ void issue_values(const AttendArgs& a, Control& ctl, uint32_t ring, u
 // Softmax of the tiles, rescaling of O, and the results.  Two threads hold a
 // row: the first four warps its keys 0..63 of a tile and lanes 0..127 of O,
 // the others the rest; they swap maxima, so both come to the same ones.
-__device__ void softmax_rows(const AttendArgs& a, Control& ctl, Swap& swap, uint8_t* ring, uint32_t tmem) {
+__device__ void softmax_rows(const AttendArgs& a, Control& ctl, Swap& swap, uint32_t q, uint8_t* ring,
+                             uint32_t tmem) {
   const int lane = threadIdx.x & 31;
   const int warp = ((threadIdx.x >> 5) - kSoftmaxWarp0) & 3;
   const int half = (threadIdx.x >> 5) >= kSoftmaxWarp0 + 4;
@@ -772,11 +828,17 @@ __device__ void softmax_rows(const AttendArgs& a, Control& ctl, Swap& swap, uint
     return true;
   };
   for (; pieces.next(ctl, p); tile += p.tiles) {
+    if (tile == 0) load_first_queries(a, ctl, p, (threadIdx.x >> 5) - kSoftmaxWarp0, q);
     const bool busy = warp * 32 < p.rows;  // some lane of the warp has a row
     const int in_item = p.row0 + row;
     const int tok = a.by_group.of(in_item);
     int seen = p.own ? p.seen0 + tok : p.seen0;
     if (seen > p.keys) seen = p.keys;
+    // keys from the piece's first tile on, counted from this thread's half of a tile:
+    // the prefix's, the request's that the row sees, the request's that any row sees
+    const int in_shared = p.shared_tiles - p.first_tile, behind = p.first_tile * kKeys + half * kHalfKeys;
+    const int shared_left = a.prefix_len - behind;
+    const int own_left = seen - behind + p.shared_tiles * kKeys, all_left = own_left - seen + p.keys;
     float m = -INFINITY, l = 0.0f;
     for (int j = 0; j < p.tiles; ++j) {
       const uint32_t t = tile + j, buf = t & 1, ph = (t >> 1) & 1;
@@ -787,7 +849,8 @@ __device__ void softmax_rows(const AttendArgs& a, Control& ctl, Swap& swap, uint
         tmem_load32(my_s + buf * kKeys, s[0]);
         tmem_load32(my_s + buf * kKeys + 32, s[1]);
         tmem_load_wait();
-        const int left = seen - (p.first_tile + j) * kKeys - half * 64;  // of these 64 keys, those that the row sees
+        // of these 64 keys, those that the row sees
+        const int left = (j < in_shared ? shared_left : own_left) - j * kKeys;
         if (left < 64) {
 #pragma unroll
           for (int i = 0; i < 64; ++i)
@@ -842,7 +905,7 @@ __device__ void softmax_rows(const AttendArgs& a, Control& ctl, Swap& swap, uint
       // V rows past the keys weigh nothing, but what their page holds may be
       // no number, and 0 times that is none either: they are cleared.  Boxes
       // that begin behind the keys were filled with zeros.
-      const int whole = p.keys - (p.first_tile + j) * kKeys - half * kHalfKeys;
+      const int whole = (j < in_shared ? shared_left : all_left) - j * kKeys;
       if (whole < kHalfKeys) {
         // V(t - 1), the stage's last contents, has landed if it has been used
         if (t > 0 && !__all_sync(0xffffffffu, mbar_wait(ctl, &ctl.pv_done[buf ^ 1], ((t - 1) >> 1) & 1))) return;
@@ -952,6 +1015,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&ctl.p_full[i], kSoftmaxWarps);
       mbar_init(&ctl.pv_done[i], 1);
     }
+    mbar_init(&ctl.q_first, 32 * kSoftmaxWarps);
     mbar_init(&ctl.q_full, 32);
     mbar_init(&ctl.q_empty, 1);
     mbar_init(&ctl.o_free, kSoftmaxWarps);
@@ -963,6 +1027,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     ctl.failed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 0 && elect_one()) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&kmap) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&ctl.tmem))
@@ -984,7 +1052,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == 3) {
     list_pieces(a, ctl, q_at);
   } else {
-    softmax_rows(a, ctl, swap, ring, tmem);
+    softmax_rows(a, ctl, swap, q_at, ring, tmem);
+    asm volatile("cp.async.wait_all;" ::: "memory");
   }
   tmem_fence_before();
   __syncthreads();
@@ -1062,8 +1131,9 @@ __device__ __forceinline__ RowParts find_parts(const AttendArgs& a, int flat, in
     place(0, (h * div_up(used * a.group, kRows) + packed / kRows) * (key_tiles + kItemCost), key_tiles, packed % kRows);
   }
   const int packed = (token - q.first) * a.group + g, rt = packed / kRows;
-  const int t = q.tiles(a, rt);
-  place(1, pre + a.units_before[b] + q.units_before(a, rt) * a.k_heads + h * (t + kItemCost), t, packed % kRows);
+  const int units = Request::units(q.tiles(a, rt), note.joint);
+  place(1, pre + a.units_before[b] + q.units_before(a, rt, note.joint) * a.k_heads + h * units,
+        max(units - kItemCost, 0), packed % kRows);
   r.live = pre > 0 || r.count[1] != 1;  // otherwise the first kernel wrote the row
   return r;
 }

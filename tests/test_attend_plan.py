@@ -26,7 +26,14 @@ class Plan:
             self.starts.append(self.starts[-1] + n)
         self.tokens = self.starts[-1]
         self.row_tiles = div_up(self.tokens * self.group, ROWS)
-        self.pre = self.row_tiles * k_heads * (div_up(prefix, KEYS) + COST) if prefix else 0
+        self.key_tiles = div_up(prefix, KEYS)
+        self.pre = self.row_tiles * k_heads * (self.key_tiles + COST) if prefix else 0
+        # the shorter line: requests' items with the prefix in them, or apart from it
+        self.joint = -1
+        alone = sum(self.own_tiles(b) for b in range(len(counts)))
+        seeing = sum(self.tiles(b, rt) > 0 for b in range(len(counts)) for rt in range(self.own_tiles(b)))
+        if prefix and (alone * (self.key_tiles + COST) - seeing * COST) * k_heads <= self.pre:
+            self.joint, self.pre = self.key_tiles, 0
         self.before = [0]
         for b in range(len(counts)):
             self.before.append(self.before[-1] + k_heads * sum(self.cost(b, rt) for rt in range(self.own_tiles(b))))
@@ -46,13 +53,17 @@ class Plan:
 
     def cost(self, b, rt):
         t = self.tiles(b, rt)
-        return t + COST if t else 0
+        return self.joint + t + COST if self.joint >= 0 else t + COST if t else 0
 
-    def units_before(self, b, rt):
+    def seeing_before(self, b, rt):
         if rt == 0:
             return 0
         c = (127 + self.group * (self.lens[b] - self.counts[b] + 128)) >> 7
-        return self.tiles_before(b, rt) + (rt - min(max(self.group - c, 0), rt)) * COST
+        return rt - min(max(self.group - c, 0), rt)
+
+    def units_before(self, b, rt):
+        return self.tiles_before(b, rt) + (
+            rt * (self.joint + COST) if self.joint >= 0 else self.seeing_before(b, rt) * COST)
 
     def tiles_before(self, b, rt):
         """The closed form of sum(tiles(b, x) for x < rt), rt below own_tiles(b)."""
@@ -80,7 +91,7 @@ class Plan:
     def pieces(self, cta):
         """(item, first tile, tiles, destination) in the order of list_pieces."""
         u, end = self.begin(cta), self.begin(cta + 1)
-        key_tiles = div_up(self.prefix, KEYS)
+        key_tiles = self.key_tiles
         while u < end and u < self.pre:
             item, at = divmod(u, key_tiles + COST)
             step = min(end - u, key_tiles + COST - at)
@@ -98,7 +109,7 @@ class Plan:
         base = self.pre + (self.before[start] if start < len(self.counts) else 0)
         for b in range(start, len(self.counts)):
             for rt in range(self.own_tiles(b)):
-                t, cost = self.tiles(b, rt), self.cost(b, rt)
+                cost = self.cost(b, rt)
                 for h in range(self.k_heads):
                     if u < end and u < base + cost:
                         at = u - base
@@ -107,8 +118,8 @@ class Plan:
                         u += step
                         first = max(at - COST, 0)
                         n = at + step - COST - first
-                        to = ("slot", 2 * cta + (0 if first > 0 else 1)) if n < t else (
-                            ("part", 1) if self.prefix else ("out", 0))
+                        to = ("slot", 2 * cta + (0 if first > 0 else 1)) if n < cost - COST else (
+                            ("part", 1) if self.pre else ("out", 0))
                         if n > 0:
                             yield ("own", b, rt, h), first, n, to
                     base += cost
@@ -122,14 +133,14 @@ class Plan:
         ranges = []
         if self.pre:
             packed = token * self.group + g
-            key_tiles = div_up(self.prefix, KEYS)
+            key_tiles = self.key_tiles
             lo = (h * self.row_tiles + packed // ROWS) * (key_tiles + COST) + COST
             ranges.append((0, lo, lo + key_tiles, packed % ROWS))
         packed = (token - self.starts[b]) * self.group + g
         rt = packed // ROWS
-        lo = self.pre + self.before[b] + self.k_heads * self.units_before(b, rt) + (
-            h * (self.tiles(b, rt) + COST) + COST)
-        ranges.append((1, lo, lo + self.tiles(b, rt), packed % ROWS))
+        cost = self.cost(b, rt)
+        lo = self.pre + self.before[b] + self.k_heads * self.units_before(b, rt) + h * cost + COST
+        ranges.append((1, lo, lo + max(cost - COST, 0), packed % ROWS))
         for x, lo, hi, row in ranges:
             if lo == hi:
                 continue
@@ -167,15 +178,15 @@ def check(plan):
                         "part", to[1], key[0] * plan.q_heads + key[1])
                     held.setdefault(key, []).append(place)
     expected = {}
-    if plan.prefix:
+    if plan.pre:
         for h in range(plan.k_heads):
             for t in range(plan.row_tiles):
-                expected["prefix", h, t] = div_up(plan.prefix, KEYS)
+                expected["prefix", h, t] = plan.key_tiles
     for b in range(len(plan.counts)):
         for rt in range(plan.own_tiles(b)):
             for h in range(plan.k_heads):
-                if plan.tiles(b, rt):
-                    expected["own", b, rt, h] = plan.tiles(b, rt)
+                if plan.cost(b, rt):
+                    expected["own", b, rt, h] = plan.cost(b, rt) - COST
     assert covered.keys() == expected.keys()
     for item, runs in covered.items():
         runs.sort()
@@ -193,21 +204,25 @@ def check(plan):
 @pytest.mark.parametrize("counts,lens,prefix,heads,grid", [
     ([1], [300], 0, (6, 1), 148), ([1], [0], 0, (6, 1), 148), ([1], [0], 1, (6, 1), 148),
     ([1] * 40, [50] * 40, 1000, (6, 1), 148), ([5, 0, 3], [7, 9, 1], 65, (8, 2), 148),
-    ([100, 40], [100, 300], 200, (6, 1), 16), ([3], [5000], 0, (130, 1), 7), ([1] * 300, [1] * 300, 0, (6, 1), 148),
+    ([100, 40], [100, 300], 200, (6, 1), 16), ([100, 41], [100, 0], 900, (12, 2), 16), ([3], [3], 5000, (6, 1), 7),
+    ([64, 0, 128], [0, 70, 500], 128, (4, 2), 11), ([3], [5000], 0, (130, 1), 7), ([1] * 300, [1] * 300, 0, (6, 1), 148),
 ])
 def test_pieces_cover_every_tile_and_the_join_finds_them(counts, lens, prefix, heads, grid):
     check(Plan(counts, lens, prefix, *heads, grid))
 
 
 def test_random_batches():
-    rng = random.Random(5)
+    rng, joint = random.Random(5), set()
     for _ in range(60):
         batch = rng.randint(1, 20)
         counts = [rng.choice([0, 1, 1, rng.randint(1, 60)]) for _ in range(batch)]
         lens = [rng.choice([0, 1, 63, 64, 65, rng.randint(0, 2000)]) for _ in range(batch)]
         prefix = rng.choice([0, 1, 64, rng.randint(1, 3000)])
         heads = rng.choice([(6, 1), (8, 2), (4, 4), (12, 2)])
-        check(Plan(counts, lens, prefix, *heads, rng.choice([1, 5, 20, 148])))
+        plan = Plan(counts, lens, prefix, *heads, rng.choice([1, 5, 20, 148]))
+        joint.add(plan.joint >= 0)
+        check(plan)
+    assert joint == {False, True}
 
 
 def test_ring_order_names_every_entry_once():
@@ -243,8 +258,11 @@ def test_closed_form_of_a_requests_tiles():
         for rt in sorted({0, 1, n // 2, n - 1, rng.randrange(n)} & set(range(n))):
             assert plan.tiles_before(0, rt) == sum(plan.tiles(0, x) for x in range(rt)), (count, length, group, rt)
             assert plan.units_before(0, rt) == sum(plan.cost(0, x) for x in range(rt)), (count, length, group, rt)
+            assert plan.seeing_before(0, rt) == sum(plan.tiles(0, x) > 0 for x in range(rt))
         last = div_up(length, KEYS) + COST if length else 0
         assert plan.units_before(0, n - 1) + last == plan.units
+        plan = Plan([count], [length], 1000, group, 1, 148)  # one request: the prefix in its items
+        assert plan.joint == 8 and plan.units_before(0, n - 1) + plan.cost(0, n - 1) == plan.units
 
 
 def test_division_by_multiplication():

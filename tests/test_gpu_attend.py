@@ -115,6 +115,35 @@ def test_query_runs(counts, lens, prefix):
     agree(batch, batch.run())
 
 
+@pytest.mark.parametrize("block", [8, 48, 64])
+@pytest.mark.parametrize("counts,lens,prefix", [
+    ([64, 0, 128], [64, 70, 500], 130), ([64, 64], [0, 1], 1), ([128, 64], [100, 600], 1000), ([192], [300], 127),
+    ([3], [0], 300), ([2], [200], 5000), ([1], [1], 129),
+])
+def test_requests_that_fill_their_row_tiles(counts, lens, prefix, block):
+    """The prefix and a request's own keys in one item: its tiles end inside the prefix and inside the own keys."""
+    batch = Batch(lens, counts=counts, prefix=prefix, heads=(4, 2), block=block)
+    agree(batch, batch.run())
+    assert batch.status.item() == 0
+
+
+def test_captured_call_follows_query_starts():
+    """The same launch with the prefix in the requests' items and apart from them."""
+    batch = Batch([300, 400], counts=[64, 128], prefix=700, heads=(4, 2))
+    starts = torch.tensor(batch.starts, dtype=torch.int64, device=DEV)
+    args = {**batch.args(), "query_starts": starts, "return_lse": True}
+    call = lambda: welm.attend_shared_prefix(batch.q, batch.keys, batch.values, **args)  # noqa: E731
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, lse = call()
+    for new in ([0, 64, 192], [0, 65, 192], [0, 0, 192], [0, 191, 192]):
+        starts.copy_(torch.tensor(new))
+        graph.replay()
+        batch.starts = new
+        agree(batch, (out, lse))
+
+
 @pytest.mark.parametrize("scale,spread", [(1.0, 1.0), (1 / 16, 8.0), (1e-3, 1.0), (0.25, 3.0)])
 def test_scales(scale, spread):
     """Peaked and flat rows; with peaked ones the running maximum moves often."""
