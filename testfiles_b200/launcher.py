@@ -40,7 +40,10 @@ the timed region, µs per call and GB/s each way over the bus.
 ``--kv-write N,BS`` times the fused KV-mirror cache write (with ``--time``;
 with ``--iters`` it only launches it, for ncu).  ``--fused-qkv M`` times
 prefill on strided Q/K views of a fused QKV projection output beside a
-contiguous Q copy followed by the op.
+contiguous Q copy followed by the op.  ``--paged-decode BS,PREFIX,LEN`` times a
+decode step's rotation, append to the paged cache and attention, and
+``--multi-axis M`` the multi-axis rotation of an image's tokens; both only
+launch with ``--iters`` and without ``--time``.
 """
 
 from __future__ import annotations
@@ -55,7 +58,7 @@ from typing import Iterable, Optional
 
 import torch
 
-from . import _native, ops, workloads
+from . import _native, ops, paged, workloads
 from .clocks import ClockSampler
 
 L2_BYTES = 126 * 1024 * 1024
@@ -529,6 +532,118 @@ def time_fused_qkv(n_tokens: int, device: torch.device, trials: int = 7, graph_l
     }
 
 
+def _timed(call, sets: int, nbytes: int, record: dict, device: torch.device, trials: int, graph_launches: int,
+           replays: int) -> dict:
+    """``record`` with the time of ``call(i)``, graph-replayed over ``sets`` rotating buffer sets."""
+    for i in range(3):
+        call(i)
+    torch.cuda.synchronize(device)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for i in range(graph_launches):
+            call(i)
+    us = _replay_us(graph, device, trials, replays, graph_launches)
+    peak, kind = measured_hbm_peak()
+    return {"record_type": "timing", **record, "us_per_launch": round(us, 3), "bytes_per_launch": nbytes,
+            "gb_s": round(nbytes / (us * 1e3), 1), "hbm_frac": round(nbytes / (us * 1e3) / peak, 4),
+            "hbm_peak_gbs": peak, "hbm_peak_source": kind, "buffer_sets": sets,
+            "l2_cold": sets * nbytes > 2 * L2_BYTES, "device_name": torch.cuda.get_device_name(device)}
+
+
+def multi_axis_bytes(n_tokens: int) -> int:
+    """Algorithmic bytes of a three-axis rotation in place: per token the rope
+    slices of 6 Q heads and the K head read and written (7 x 256), three
+    positions (24) and a cos/sin row (256)."""
+    return 2072 * n_tokens
+
+
+def time_multi_axis(n_tokens: int, device: torch.device, trials: int = 7, graph_launches: int = 32,
+                    replays: int = 20, sets: Optional[int] = None, iters: int = 0) -> dict:
+    """µs per rope_multi_axis_inplace on strided Q / K views of a fused QKV
+    output [N, 8 x 256]: the tokens of an image as wide as high, sections 16,
+    8 and 8.  ``iters`` > 0 only launches that many times (for ncu captures)."""
+    nbytes = multi_axis_bytes(n_tokens)
+    if sets is None:
+        sets = int(min(16, max(2, -(-2 * L2_BYTES // max(nbytes, 1)))))
+    side = max(1, round(n_tokens ** 0.5))
+    cache = workloads.make_cos_sin_cache(n_tokens // side + side + 1, 10000.0, device=device)
+    g = torch.Generator(device=device).manual_seed(0)
+    at = torch.arange(n_tokens, dtype=torch.int64, device=device)
+    positions = torch.stack([torch.zeros_like(at), at // side, at % side])
+    bufs = [(torch.randn((n_tokens, 8 * 256), generator=g, device=device).to(torch.bfloat16), positions.clone())
+            for _ in range(1 if iters else sets)]
+
+    def call(i: int) -> None:
+        qkv, pos = bufs[i % len(bufs)]
+        paged.rope_multi_axis_inplace(qkv[:, :1536].view(n_tokens, 6, 256), qkv[:, 1536:1792].view(n_tokens, 1, 256),
+                                      pos, cache, (16, 8, 8))
+
+    if iters:
+        for i in range(iters):
+            call(i)
+        torch.cuda.synchronize(device)
+        return {"record_type": "launch", "kernel_name": "rope_multi_axis_kernel", "n_tokens": n_tokens, "iters": iters}
+    return _timed(call, sets, nbytes, {"case": f"multi_axis_m{n_tokens}", "phase": "prefill", "path": "multi_axis",
+                                       "n_tokens": n_tokens}, device, trials, graph_launches, replays)
+
+
+def paged_decode_bytes(batch: int, prefix_len: int, length: int) -> int:
+    """Algorithmic bytes of a decode step's append and attention: the shared and
+    the own keys and values (2 x 512 a key); per request 6 rope slices read and
+    written (2 x 128), 6 Q rows read and outputs written (2 x 512), the new key
+    and value read and written (4 x 512), a cos/sin row (256), position, slot
+    and length (24)."""
+    return 1024 * (prefix_len + batch * length) + batch * (2 * 6 * 128 + 2 * 6 * 512 + 4 * 512 + 256 + 24)
+
+
+def time_paged_decode(batch: int, prefix_len: int, length: int, device: torch.device, trials: int = 7,
+                      graph_launches: int = 8, replays: int = 20, sets: Optional[int] = None, iters: int = 0) -> dict:
+    """µs per decode step of ``batch`` requests: rope_kv_append of their new
+    tokens into a paged cache of 64-key blocks, then attend_shared_prefix over
+    ``prefix_len`` keys that all share and ``length`` own ones.  ``iters`` > 0
+    only launches that many times (for ncu captures)."""
+    if batch < 1 or prefix_len < 0 or length < 1:
+        raise ValueError("a decode step needs at least one request, and one own key for each")
+    nbytes = paged_decode_bytes(batch, prefix_len, length)
+    if sets is None:
+        sets = int(min(8, max(2, -(-2 * L2_BYTES // nbytes))))
+    shared, own = -(-prefix_len // 64), -(-length // 64)
+    blocks = shared + batch * own
+    cos_sin = workloads.make_cos_sin_cache(prefix_len + length, 10000.0, device=device)
+    g = torch.Generator(device=device).manual_seed(0)
+    bufs = []
+    for _ in range(1 if iters else sets):
+        order = torch.randperm(blocks, generator=g, device=device).to(torch.int32)
+        table = order[shared:].view(batch, own)
+        caches = [torch.randn((blocks, 64, 1, 256), generator=g, device=device).to(torch.bfloat16) for _ in range(2)]
+        qkv = torch.randn((batch, 8 * 256), generator=g, device=device).to(torch.bfloat16)
+        slots = table[:, (length - 1) // 64].long() * 64 + (length - 1) % 64
+        bufs.append((qkv, slots, table, order[:shared], *caches))
+    positions = torch.full((batch,), prefix_len + length - 1, dtype=torch.int64, device=device)
+    lens = torch.full((batch,), length, dtype=torch.int64, device=device)
+    out = torch.empty((batch, 6, 256), dtype=torch.bfloat16, device=device)
+    workspace = torch.empty(paged.attend_workspace_bytes(batch, batch, 6, 1, prefix_len, device=device),
+                            dtype=torch.uint8, device=device)
+
+    def call(i: int) -> None:
+        qkv, slots, table, prefix_table, keys, values = bufs[i % len(bufs)]
+        q = qkv[:, :1536].view(batch, 6, 256)
+        paged.rope_kv_append(q, qkv[:, 1536:1792].view(batch, 1, 256), qkv[:, 1792:].view(batch, 1, 256), positions,
+                             cos_sin, slots, keys, values)
+        paged.attend_shared_prefix(q, keys, values, table, lens, prefix_table=prefix_table if shared else None,
+                                   prefix_len=prefix_len, out=out, workspace=workspace)
+
+    if iters:
+        for i in range(iters):
+            call(i)
+        torch.cuda.synchronize(device)
+        return {"record_type": "launch", "kernel_name": "rope_attend_kernel", "batch_size": batch,
+                "prefix_len": prefix_len, "length": length, "iters": iters}
+    return _timed(call, sets, nbytes, {"case": f"paged_decode_bs{batch}_p{prefix_len}_l{length}", "phase": "decode",
+                                       "path": "paged_attend", "batch_size": batch, "prefix_len": prefix_len,
+                                       "length": length}, device, trials, graph_launches, replays)
+
+
 # Dense ordinary launches of at most this many tokens run one head per thread
 # (kHeadSplitMaxTokens in csrc/rope_host.cuh).
 HEAD_SPLIT_MAX_TOKENS = 3328
@@ -636,6 +751,11 @@ def main(argv: Optional[list[str]] = None) -> int:
     parser.add_argument("--fused-qkv", type=int, default=None, metavar="M",
                         help="time prefill on strided Q/K views of an [M, 8 x 256] QKV output against a "
                              "contiguous Q copy followed by the op")
+    parser.add_argument("--paged-decode", default=None, metavar="BS,PREFIX,LEN",
+                        help="time a decode step of BS requests over PREFIX shared and LEN own keys each: rotation, "
+                             "append to the paged cache, attention (without --time: only launch it)")
+    parser.add_argument("--multi-axis", type=int, default=None, metavar="M",
+                        help="time the multi-axis rotation of an image's M tokens (without --time: only launch it)")
     args = parser.parse_args(argv)
     if args.sets is not None and args.sets < 1:
         parser.error("--sets needs at least 1")
@@ -644,14 +764,21 @@ def main(argv: Optional[list[str]] = None) -> int:
         return 2
     device = torch.device(args.device)
     torch.cuda.set_device(device)
-    if args.kv_write or args.fused_qkv:
-        if args.fused_qkv:
+    if args.kv_write or args.fused_qkv or args.paged_decode or args.multi_axis:
+        iters = 0 if args.time else args.iters
+        if args.paged_decode:
+            rec = time_paged_decode(*(int(x) for x in args.paged_decode.split(",")), device, sets=args.sets, iters=iters)
+        elif args.multi_axis:
+            if args.multi_axis <= 0:
+                parser.error("--multi-axis needs a positive token count")
+            rec = time_multi_axis(args.multi_axis, device, sets=args.sets, iters=iters)
+        elif args.fused_qkv:
             if args.fused_qkv <= 0:
                 parser.error("--fused-qkv needs a positive token count")
             rec = time_fused_qkv(args.fused_qkv, device)
         else:
             n, bs = (int(x) for x in args.kv_write.split(","))
-            rec = time_kv_write(n, bs, device, iters=0 if args.time else args.iters)
+            rec = time_kv_write(n, bs, device, iters=iters)
         print(json.dumps(rec), flush=True)
         if args.json:
             with open(args.json, "a") as fh:

@@ -143,3 +143,22 @@ def test_gather_ceiling_reads_without_writing():
         launcher.ceiling_gather(pos.to(torch.int32), cache)
     with pytest.raises(ValueError):
         launcher.ceiling_gather(pos[::2], cache)
+
+
+def test_time_multi_axis_record():
+    rec = launcher.time_multi_axis(1000, DEV, trials=2, graph_launches=4, replays=3, sets=2)
+    assert rec["us_per_launch"] > 0 and rec["bytes_per_launch"] == launcher.multi_axis_bytes(1000)
+    assert launcher.time_multi_axis(500, DEV, iters=2)["record_type"] == "launch"
+
+
+@pytest.mark.parametrize("prefix", [0, 130])
+def test_time_paged_decode_record(prefix):
+    rec = launcher.time_paged_decode(5, prefix, 65, DEV, trials=2, graph_launches=4, replays=3, sets=2)
+    assert rec["us_per_launch"] > 0 and rec["bytes_per_launch"] == launcher.paged_decode_bytes(5, prefix, 65)
+    assert launcher.time_paged_decode(3, prefix, 64, DEV, iters=2)["record_type"] == "launch"
+
+
+def test_paged_options_print_a_record(capsys):
+    for args in (["--paged-decode", "4,200,70"], ["--multi-axis", "300"]):
+        assert launcher.main(args + ["--iters", "1"]) == 0
+        assert json.loads(capsys.readouterr().out)["record_type"] == "launch"
