@@ -1093,8 +1093,7 @@ __device__ __forceinline__ int find_request(const AttendArgs& a, int token, int&
 }
 
 // `b`: a request that begins at or before the row's token, not far before.
-__device__ __forceinline__ RowParts find_parts(const AttendArgs& a, int flat, int b) {
-  const int used = used_tokens(a);
+__device__ __forceinline__ RowParts find_parts(const AttendArgs& a, const LineNote& note, int used, int flat, int b) {
   RowParts r{};
   if (flat >= a.tokens * a.q_heads) return r;
   const int token = a.by_q_heads.of(flat), hq = flat - token * a.q_heads;
@@ -1106,17 +1105,15 @@ __device__ __forceinline__ RowParts find_parts(const AttendArgs& a, int flat, in
   } else {
     while (b + 1 < a.batch && __ldg(a.query_starts + b + 1) <= token) ++b;
   }
-  Request q{0, 0, 0};
-  if (token < used) {
-    RawRequest raw;
-    raw.load(a, b);
-    q = raw.checked(a, false);
-  }
-  if (token < q.first || token >= q.first + q.count) {  // a row of no request
+  // all that has to be read at once, before any of it is looked at
+  RawRequest raw;
+  raw.load(a, b);
+  const int units_before = a.units_before[b];
+  const Request q = raw.checked(a, false);
+  if (token >= used || token < q.first || token >= q.first + q.count) {  // a row of no request
     r.live = a.fill;
     return r;
   }
-  const LineNote note = *a.note;
   const int pre = note.pre;
   auto place = [&](int x, int first, int tiles, int in_tile) {
     r.in_tile[x] = in_tile;
@@ -1132,7 +1129,7 @@ __device__ __forceinline__ RowParts find_parts(const AttendArgs& a, int flat, in
   }
   const int packed = (token - q.first) * a.group + g, rt = packed / kRows;
   const int units = Request::units(q.tiles(a, rt), note.joint);
-  place(1, pre + a.units_before[b] + q.units_before(a, rt, note.joint) * a.k_heads + h * units,
+  place(1, pre + units_before + q.units_before(a, rt, note.joint) * a.k_heads + h * units,
         max(units - kItemCost, 0), packed % kRows);
   r.live = pre > 0 || r.count[1] != 1;  // otherwise the first kernel wrote the row
   return r;
@@ -1161,18 +1158,21 @@ __device__ __forceinline__ void load8f(const float* p, float (&v)[8]) {
                : "memory");
 }
 
-template <int kGroups>
-__global__ void __launch_bounds__(kGroups == 1 ? 256 : 128 * kGroups)
+template <int kGroups, int kUnroll, int kResident>
+__global__ void __launch_bounds__(kGroups == 1 ? 256 : 128 * kGroups, kResident)
     rope_attend_join_kernel(const __grid_constant__ AttendArgs a) {
-  constexpr int kRowsPerCta = kGroups == 1 ? 32 : 4, kUnroll = 4;
+  constexpr int kRowsPerCta = kGroups == 1 ? 32 : 4;
   __shared__ RowParts parts[kRowsPerCta];
   __shared__ int s_request;
   __shared__ float s_o[kGroups == 1 ? 1 : kGroups - 1][kGroups == 1 ? 1 : 10][128];
   const int grp = threadIdx.x >> 7, in_grp = threadIdx.x & 127;
   const int lanes8 = in_grp >> 2;  // eight lanes of the head
   pdl_enter();
+  const LineNote note = *a.note;
+  const int used = used_tokens(a);
   const int request = find_request(a, a.by_q_heads.of(blockIdx.x * kRowsPerCta), s_request);
-  if (threadIdx.x < kRowsPerCta) parts[threadIdx.x] = find_parts(a, blockIdx.x * kRowsPerCta + threadIdx.x, request);
+  if (threadIdx.x < kRowsPerCta)
+    parts[threadIdx.x] = find_parts(a, note, used, blockIdx.x * kRowsPerCta + threadIdx.x, request);
   __syncthreads();
   const int64_t all = int64_t(a.tokens) * a.q_heads;
   for (int row = (kGroups == 1 ? 4 * grp : 0) + (in_grp & 3); row < kRowsPerCta; row += 8) {
@@ -1305,9 +1305,14 @@ int launch_attend(const CUtensorMap& kmap, const CUtensorMap& vmap, const Attend
   int rc = launch(rope_attend_kernel, unsigned(a.grid), kThreads, kSmemBytes, stream, kmap, vmap, a);
   if (rc != WELM_ROPE_OK) return rc;
   const int64_t rows = int64_t(a.tokens) * a.q_heads;
-  if (rows <= 4 * a.grid) return launch(rope_attend_join_kernel<4>, unsigned((rows + 3) / 4), 512, 0, stream, a);
-  if (rows <= 4096) return launch(rope_attend_join_kernel<2>, unsigned((rows + 3) / 4), 256, 0, stream, a);
-  return launch(rope_attend_join_kernel<1>, unsigned((rows + 31) / 32), 256, 0, stream, a);
+  // Few rows may have many partial results each: four groups of threads to a row's,
+  // with as many loads in flight as registers allow for one CTA or two on an SM.
+  // 768 rows of some 20 partial results: 34.7 us for both kernels with two groups,
+  // 33.0 with four; 288 rows of three: 27.0 with four loads in flight, 27.7 with three.
+  if (rows <= 4 * a.grid) return launch(rope_attend_join_kernel<4, 4, 1>, unsigned((rows + 3) / 4), 512, 0, stream, a);
+  if (rows <= 8 * a.grid) return launch(rope_attend_join_kernel<4, 3, 2>, unsigned((rows + 3) / 4), 512, 0, stream, a);
+  if (rows <= 4096) return launch(rope_attend_join_kernel<2, 3, 1>, unsigned((rows + 3) / 4), 256, 0, stream, a);
+  return launch(rope_attend_join_kernel<1, 2, 1>, unsigned((rows + 31) / 32), 256, 0, stream, a);
 }
 
 }  // namespace
