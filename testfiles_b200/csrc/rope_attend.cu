@@ -27,7 +27,8 @@
 //   1, 2   issue tcgen05.mma: S = Q K^T (128 x 128), and O += P V (128 x 256)
 //   3      adds up the line, lists the CTA's pieces and brings their Q rows into
 //          shared memory (64 KB)
-//   4..11  softmax: two threads a row, 64 keys each; rescaling of O; results
+//   4..11  softmax: two threads a row, 64 keys each; rescaling of O; results.
+//          At first they help to add up the line and bring the first Q rows
 // S and O live in TMEM, S twice, so that the softmax of one tile runs beside
 // the products of its neighbours; P (BF16) takes the place of S.  P is rounded
 // to BF16 because the product with the BF16 values takes both operands in one
@@ -228,13 +229,20 @@ struct Piece {
   int32_t slot;
 };
 
+// What the line is made of, of one head of some requests.
+struct LineSums {
+  int units, row_tiles, seeing;  // own items' units; row tiles, and those that see own keys
+};
+
 struct Control {
   uint64_t full_k[kStagesK], empty_k[kStagesK], full_v[kStagesV], empty_v[kStagesV];
   uint64_t s_full[2], p_full[2], pv_done[2];
   uint64_t q_first, q_full, q_empty, o_free, drained[2];
   uint64_t swap[4];  // the two warps of 32 rows
   uint64_t piece_full[kPieces], piece_empty[kPieces];
+  uint64_t added;
   Piece piece[kPieces];
+  LineSums sums[kSoftmaxWarps];
   uint32_t tmem;
   int32_t failed;
 };
@@ -245,8 +253,8 @@ struct Swap {
   float value[2][2][kRows];  // [tile parity][half]
 };
 
-constexpr int kSmemBytes = kQBytes + (kStagesK + kStagesV) * kStageBytes + sizeof(Swap) + 800;
-static_assert(sizeof(Control) <= 800, "control block");
+constexpr int kSmemBytes = kQBytes + (kStagesK + kStagesV) * kStageBytes + sizeof(Swap) + 896;
+static_assert(sizeof(Control) <= 896, "control block");
 static_assert(kSmemBytes <= 227 * 1024, "shared memory of one CTA");
 
 // Waits for a phase of `bar`; false once any warp of the CTA has given up.
@@ -422,23 +430,51 @@ __device__ __forceinline__ bool load_queries(const AttendArgs& a, Control& ctl, 
   return true;
 }
 
+// Units of the requests from `first` on, a request a lane and then every `step`th
+// after it, one copy of the code, which nobody has run yet, for all of them.
+// `kept` becomes the lane's first request.
+__device__ __forceinline__ LineSums add_up(const AttendArgs& a, int first, int step, Request& kept) {
+  const int lane = threadIdx.x & 31;
+  LineSums sums{0, 0, 0};
+  RawRequest next;
+  if (first + lane < a.batch) next.load(a, first + lane);
+#pragma unroll 1
+  for (int b = first + lane; b < a.batch; b += step) {
+    const RawRequest raw = next;
+    if (b + step < a.batch) next.load(a, b + step);
+    const Request r = raw.checked(a, blockIdx.x == 0);
+    const int n = r.row_tiles(a);
+    sums.units += r.all_units(a, -1);
+    sums.row_tiles += n;
+    sums.seeing += n == 0 ? 0 : r.seeing_before(a, n - 1) + (r.len > 0);
+    if (b == first + lane) kept = r;
+  }
+  sums.units = __reduce_add_sync(0xffffffffu, sums.units);
+  sums.row_tiles = __reduce_add_sync(0xffffffffu, sums.row_tiles);
+  sums.seeing = __reduce_add_sync(0xffffffffu, sums.seeing);
+  return sums;
+}
+
 // Adds up the requests' units, finds where this CTA's run begins and lists the
-// run's pieces; CTA 0 also notes the line for the join.  One warp does it all, a
-// request a lane, while the others get ready.
+// run's pieces; CTA 0 also notes the line for the join.  The softmax warps, which
+// have nothing to do yet, add up what is past the first 32 requests: 128 requests
+// over a prefix 33.0 us with one warp for all, eight requests a lane at once, and
+// 32.0 so; one request 11.1 and 10.5.
 __device__ void list_pieces(const AttendArgs& a, Control& ctl, uint32_t q) {
   const int lane = threadIdx.x & 31, cta = blockIdx.x;
-  const int used = used_tokens(a);
-  const int key_tiles = div_up(a.prefix_len, kKeys), row_tiles = div_up(used * a.group, kRows);
+  const int key_tiles = div_up(a.prefix_len, kKeys);
   // The 32 requests from `held` on, one a lane: its units, and with those before it in the 32.
   Request mine{0, 0, 0};
   int held = 0, my_units = 0, my_sum = 0, joint = -1;
   auto hold = [&](int b0) {
-    held = b0;
-    mine = Request{0, 0, 0};
-    if (b0 + lane < a.batch) {
-      RawRequest raw;
-      raw.load(a, b0 + lane);
-      mine = raw.checked(a, false);
+    if (b0 != held) {
+      held = b0;
+      mine = Request{0, 0, 0};
+      if (b0 + lane < a.batch) {
+        RawRequest raw;
+        raw.load(a, b0 + lane);
+        mine = raw.checked(a, false);
+      }
     }
     my_units = my_sum = mine.all_units(a, joint) * a.k_heads;
 #pragma unroll
@@ -447,32 +483,26 @@ __device__ void list_pieces(const AttendArgs& a, Control& ctl, uint32_t q) {
       if (lane >= d) my_sum += x;
     }
   };
-  int total = 0, row_tiles_alone = 0, seeing = 0;
-  for (int b0 = lane; b0 < a.batch; b0 += 256) {  // eight loads in flight
-    RawRequest raw[8];
+  const int64_t end_of_last = a.query_starts != nullptr ? __ldg(a.query_starts + a.batch) : a.tokens;
+  LineSums sums = add_up(a, 0, 32 * (1 + kSoftmaxWarps), mine);
+  if (a.batch > 32) {
+    if (!__all_sync(0xffffffffu, mbar_wait(ctl, &ctl.added, 0))) return;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (b0 + 32 * i < a.batch) raw[i].load(a, b0 + 32 * i);
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (b0 + 32 * i < a.batch) {
-        const Request r = raw[i].checked(a, cta == 0);
-        const int n = r.row_tiles(a);
-        total += r.all_units(a, -1);
-        row_tiles_alone += n;
-        seeing += n == 0 ? 0 : r.seeing_before(a, n - 1) + (r.len > 0);
-      }
+    for (int w = 0; w < kSoftmaxWarps; ++w) {
+      sums.units += ctl.sums[w].units;
+      sums.row_tiles += ctl.sums[w].row_tiles;
+      sums.seeing += ctl.sums[w].seeing;
+    }
   }
-  total = __reduce_add_sync(0xffffffffu, total);
+  const int used = int(clamp64(end_of_last, 0, a.tokens)), row_tiles = div_up(used * a.group, kRows);
+  int total = sums.units;
   int pre = prefix_units(a, used);
   if (pre > 0) {
     // The shorter line: row tiles of all requests together against the prefix and of
     // each against its own keys, or of each against both.  2560 query tokens of four
     // requests over 8192 shared keys: 136 us apart, 119 in one, with no partial results
     // but of cut items.
-    row_tiles_alone = __reduce_add_sync(0xffffffffu, row_tiles_alone);
-    seeing = __reduce_add_sync(0xffffffffu, seeing);
-    const int64_t both = int64_t(row_tiles_alone) * (key_tiles + kItemCost) - int64_t(seeing) * kItemCost;
+    const int64_t both = int64_t(sums.row_tiles) * (key_tiles + kItemCost) - int64_t(sums.seeing) * kItemCost;
     if (both * a.k_heads <= pre) {
       joint = key_tiles;
       total += int(both);
@@ -646,8 +676,6 @@ __device__ void produce(const AttendArgs& a, Control& ctl, const CUtensorMap* km
     BoxPlace at_k, at_v, next_k, next_v;
     at_k.ask(a, p, own, 0, a.box_k);
     for (int j = 0; j <= p.tiles && ok; ++j) {
-      next_k.ask(a, p, own, j + 1, a.box_k);
-      next_v.ask(a, p, own, j, a.box_v);
       if (j < p.tiles) {
         const int block = at_k.checked(a);
 #pragma unroll 1
@@ -669,6 +697,8 @@ __device__ void produce(const AttendArgs& a, Control& ctl, const CUtensorMap* km
           }
         }
       }
+      next_k.ask(a, p, own, j + 1, a.box_k);
+      next_v.ask(a, p, own, j, a.box_v);
       if (j > 0) {
         const int block = at_v.checked(a);
 #pragma unroll 1
@@ -813,6 +843,15 @@ __device__ void softmax_rows(const AttendArgs& a, Control& ctl, Swap& swap, uint
   const uint32_t mine = tmem + (uint32_t(warp * 32) << 16);
   const uint32_t my_s = mine + kColS + half * 64, my_o = mine + kColO + half * kHalfLanes;
   const float c = a.scale;
+  if (a.batch > 32) {
+    const int w = (threadIdx.x >> 5) - kSoftmaxWarp0;
+    Request first;
+    const LineSums sums = add_up(a, 32 * (1 + w), 32 * (1 + kSoftmaxWarps), first);
+    if (lane == 0) {
+      ctl.sums[w] = sums;
+      mbar_arrive(&ctl.added);
+    }
+  }
   PieceReader pieces;
   Piece p;
   uint32_t tile = 0, swaps = 0;
@@ -1016,6 +1055,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&ctl.pv_done[i], 1);
     }
     mbar_init(&ctl.q_first, 32 * kSoftmaxWarps);
+    mbar_init(&ctl.added, kSoftmaxWarps);
     mbar_init(&ctl.q_full, 32);
     mbar_init(&ctl.q_empty, 1);
     mbar_init(&ctl.o_free, kSoftmaxWarps);
