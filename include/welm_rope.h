@@ -411,16 +411,17 @@ int welm_rope_kv_append(void* q, const void* k, const void* v, const int64_t* po
  * query_starts == NULL gives every request one token (n_tokens == batch_size).
  * A row that sees no key becomes zeros, its lse minus infinity.  lse (may be
  * NULL, [n_tokens, num_q_heads] FP32) receives log sum_j p_j.  Rows of no
- * request are left as they were (fill_unused == 0), or become such rows too
- * (fill_unused == 1).
+ * request are left as they were in out (fill_unused == 0) or become zeros too
+ * (fill_unused == 1); their lse is minus infinity.
  *
  * The tables, lengths and starts are read on the device, so a captured launch
  * follows their contents.  A length below 0 or above table_width * block_size,
- * and starts that decrease or leave [0, n_tokens], are clamped and raise
- * WELM_ROPE_DEV_BAD_LENGTH; a block outside [0, num_blocks) reads as zeros
- * (keys and values) and raises WELM_ROPE_DEV_BAD_PAGE.  What a page holds
- * behind the last key does not matter, no numbers included; a key that some
- * rows of a request's tile do not see yet must be finite.
+ * and starts that leave [0, n_tokens], are clamped, and with starts that
+ * decrease no row belongs to a request; they raise WELM_ROPE_DEV_BAD_LENGTH.  A
+ * block outside [0, num_blocks) reads as zeros (keys and values) and raises
+ * WELM_ROPE_DEV_BAD_PAGE.  What a page holds behind the last key does not
+ * matter, no numbers included; a key that some rows of a request's tile do not
+ * see yet must be finite.
  *
  * Products take BF16 operands (p rounded to BF16) with FP32 sums; maxima, sums
  * and partial results are FP32; out is rounded once.  Results do not depend on
@@ -431,9 +432,9 @@ int welm_rope_kv_append(void* q, const void* k, const void* v, const int64_t* po
  *
  * The call allocates nothing: `workspace` is device memory of at least the
  * bytes that welm_rope_attend_workspace gives for the same sizes on the current
- * device, 32-byte aligned.  It needs no initial contents and keeps nothing for the next call,
- * but belongs to one call at a time: calls that may overlap on the GPU, replays
- * of two captured graphs among them, need a workspace each.
+ * device, 32-byte aligned.  It needs no initial contents and keeps nothing for
+ * the next call, but belongs to one call at a time: calls that may overlap on
+ * the GPU, replays of two captured graphs among them, need a workspace each.
  */
 int welm_rope_attend_workspace(int64_t n_tokens, int64_t batch_size, int64_t num_q_heads,
                                int64_t num_k_heads, int64_t prefix_len, int64_t* bytes);

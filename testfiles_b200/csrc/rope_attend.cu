@@ -96,7 +96,7 @@ struct AttendArgs {
   int32_t box_k, box_v;         // keys of one TMA box: powers of two that divide block_size, up to 128 and 64
   int32_t slot_rows;            // rows of a workspace slot
   int32_t grid;
-  int32_t fill;                 // 1: rows of no request become zeros
+  int32_t fill;                 // 1: rows of no request become zeros; their lse is minus infinity either way
   float scale;                  // times log2(e)
   struct LineNote* note;        // what the join needs of the line
   int32_t* units_before;        // [batch] units of the own items before each request
@@ -189,9 +189,9 @@ __device__ __forceinline__ int used_tokens(const AttendArgs& a) {
 // many busy.
 struct Line {
   int units, grid, each, more;  // the first `more` runs have each + 1 tiles
-  __device__ __forceinline__ Line(int n, int ctas) : units(n), grid(n < ctas ? n : ctas) {
-    each = grid > 0 ? n / grid : 0;
-    more = n - each * grid;
+  __device__ __forceinline__ Line(int n, int ctas) : units(max(n, 0)), grid(min(units, ctas)) {
+    each = grid > 0 ? units / grid : 0;
+    more = units - each * grid;
   }
   __device__ __forceinline__ int begin(int c) const { return each * c + (c < more ? c : more); }
 };
@@ -199,6 +199,7 @@ struct Line {
 // The line as the join kernel reads it; divisions are by each and each + 1.
 struct LineNote {
   int32_t pre, joint, each, more;
+  int32_t nothing;  // 1: no row belongs to a request
   Divisor by_each, by_longer;
   __device__ __forceinline__ int cta_of(int u) const {
     const int longer = more * (each + 1);
@@ -232,6 +233,7 @@ struct Piece {
 // What the line is made of, of one head of some requests.
 struct LineSums {
   int units, row_tiles, seeing;  // own items' units; row tiles, and those that see own keys
+  int decreasing;                // requests that end before they start
 };
 
 struct Control {
@@ -435,7 +437,7 @@ __device__ __forceinline__ bool load_queries(const AttendArgs& a, Control& ctl, 
 // `kept` becomes the lane's first request.
 __device__ __forceinline__ LineSums add_up(const AttendArgs& a, int first, int step, Request& kept) {
   const int lane = threadIdx.x & 31;
-  LineSums sums{0, 0, 0};
+  LineSums sums{0, 0, 0, 0};
   RawRequest next;
   if (first + lane < a.batch) next.load(a, first + lane);
 #pragma unroll 1
@@ -447,11 +449,13 @@ __device__ __forceinline__ LineSums add_up(const AttendArgs& a, int first, int s
     sums.units += r.all_units(a, -1);
     sums.row_tiles += n;
     sums.seeing += n == 0 ? 0 : r.seeing_before(a, n - 1) + (r.len > 0);
+    sums.decreasing += raw.end < raw.start;
     if (b == first + lane) kept = r;
   }
   sums.units = __reduce_add_sync(0xffffffffu, sums.units);
   sums.row_tiles = __reduce_add_sync(0xffffffffu, sums.row_tiles);
   sums.seeing = __reduce_add_sync(0xffffffffu, sums.seeing);
+  sums.decreasing = __reduce_add_sync(0xffffffffu, sums.decreasing);
   return sums;
 }
 
@@ -492,10 +496,14 @@ __device__ void list_pieces(const AttendArgs& a, Control& ctl, uint32_t q) {
       sums.units += ctl.sums[w].units;
       sums.row_tiles += ctl.sums[w].row_tiles;
       sums.seeing += ctl.sums[w].seeing;
+      sums.decreasing += ctl.sums[w].decreasing;
     }
   }
-  const int used = int(clamp64(end_of_last, 0, a.tokens)), row_tiles = div_up(used * a.group, kRows);
-  int total = sums.units;
+  // Starts that decrease would let many requests claim the same tokens, more work
+  // than any batch of this size has: nothing is done then.
+  const int used = sums.decreasing ? 0 : int(clamp64(end_of_last, 0, a.tokens));
+  const int row_tiles = div_up(used * a.group, kRows);
+  int total = sums.decreasing ? 0 : sums.units;
   int pre = prefix_units(a, used);
   if (pre > 0) {
     // The shorter line: row tiles of all requests together against the prefix and of
@@ -613,6 +621,7 @@ __device__ void list_pieces(const AttendArgs& a, Control& ctl, uint32_t q) {
     LineNote note;
     note.pre = pre;
     note.joint = joint;
+    note.nothing = sums.decreasing > 0;
     note.each = line.each;
     note.more = line.more;
     note.by_each = Divisor(max(line.each, 1));
@@ -1115,6 +1124,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 struct RowParts {
   int cta[2], count[2], in_tile[2];  // prefix and own item: first CTA, CTAs, row of the item
   int live;                          // 1: this kernel writes the row
+  int unused;                        // 1: a row of no request
   int token, head;
 };
 
@@ -1150,8 +1160,9 @@ __device__ __forceinline__ RowParts find_parts(const AttendArgs& a, const LineNo
   raw.load(a, b);
   const int units_before = a.units_before[b];
   const Request q = raw.checked(a, false);
-  if (token >= used || token < q.first || token >= q.first + q.count) {  // a row of no request
+  if (note.nothing || token >= used || token < q.first || token >= q.first + q.count) {  // a row of no request
     r.live = a.fill;
+    r.unused = 1;
     return r;
   }
   const int pre = note.pre;
@@ -1160,8 +1171,9 @@ __device__ __forceinline__ RowParts find_parts(const AttendArgs& a, const LineNo
     if (tiles == 0) return;
     // Within the line whatever is read here: lengths that another stream changes
     // between the two kernels give wrong rows, but no address outside the workspace.
-    r.cta[x] = min(note.cta_of(first + kItemCost), a.grid - 1);
-    r.count[x] = min(note.cta_of(first + kItemCost + tiles - 1), a.grid - 1) - r.cta[x] + 1;
+    auto cta = [&](int u) { return min(max(note.cta_of(u), 0), a.grid - 1); };
+    r.cta[x] = cta(first + kItemCost);
+    r.count[x] = max(cta(first + kItemCost + tiles - 1) - r.cta[x] + 1, 0);
   };
   if (pre > 0) {
     const int packed = token * a.group + g, key_tiles = div_up(a.prefix_len, kKeys);
@@ -1267,17 +1279,17 @@ __global__ void __launch_bounds__(kGroups == 1 ? 256 : 128 * kGroups, kResident)
         sum.add(s_o[w][8][in_grp], s_o[w][9][in_grp], v);
       }
     }
-    if (!r.live) continue;
     const bool none = sum.l == 0.0f;
+    if ((r.live || r.unused) && a.lse != nullptr && lanes8 == 0)
+      a.lse[int64_t(r.token) * a.q_heads + r.head] =
+          none ? -INFINITY : (sum.m + log2f(sum.l)) * 0.6931471805599453f;
+    if (!r.live) continue;
     const float inv = none ? 0.0f : 1.0f / sum.l;
     uint4 packed_out = make_uint4(0, 0, 0, 0);
     if (!none)
       packed_out = make_uint4(pack_bf16x2(sum.o[0] * inv, sum.o[1] * inv), pack_bf16x2(sum.o[2] * inv, sum.o[3] * inv),
                               pack_bf16x2(sum.o[4] * inv, sum.o[5] * inv), pack_bf16x2(sum.o[6] * inv, sum.o[7] * inv));
     *reinterpret_cast<uint4*>(a.out + r.token * a.out_token + r.head * a.out_head + lanes8 * 8) = packed_out;
-    if (a.lse != nullptr && lanes8 == 0)
-      a.lse[int64_t(r.token) * a.q_heads + r.head] =
-          none ? -INFINITY : (sum.m + log2f(sum.l)) * 0.6931471805599453f;
   }
 }
 

@@ -372,6 +372,8 @@ PyObject* kv_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (q) no_grad("rope_kv_append", *q);
   no_grad("rope_kv_append", k);
   no_grad("rope_kv_append", v);
+  no_grad("rope_kv_append", key_cache);
+  no_grad("rope_kv_append", value_cache);
   check(k, "key", at::kBFloat16, index);
   check(v, "v", at::kBFloat16, index);
   const Rows kr = rows_of(k, "key"), vr = rows_of(v, "v");
@@ -440,6 +442,8 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
   OptTensor workspace = opt_tensor_arg(args[11], "workspace");
   const OptTensor status = opt_tensor_arg(args[12], "status");
   no_grad("attend_shared_prefix", q);
+  no_grad("attend_shared_prefix", key_cache);
+  no_grad("attend_shared_prefix", value_cache);
   check(q, "query", at::kBFloat16, index);
   const Rows qr = rows_of(q, "query");
   const auto key_strides = check_cache(key_cache, "key_cache", index);

@@ -767,7 +767,8 @@ def main(argv: Optional[list[str]] = None) -> int:
     if args.kv_write or args.fused_qkv or args.paged_decode or args.multi_axis:
         iters = 0 if args.time else args.iters
         if args.paged_decode:
-            rec = time_paged_decode(*(int(x) for x in args.paged_decode.split(",")), device, sets=args.sets, iters=iters)
+            batch, prefix, length = (int(x) for x in args.paged_decode.split(","))
+            rec = time_paged_decode(batch, prefix, length, device, sets=args.sets, iters=iters)
         elif args.multi_axis:
             if args.multi_axis <= 0:
                 parser.error("--multi-axis needs a positive token count")

@@ -89,7 +89,9 @@ def rope_multi_axis(
 
     Arguments as for :func:`rope_multi_axis_inplace`; q and k keep their values
     and may have any strides, the results are contiguous.  A token with a
-    position outside the cache is copied as it is, its gradient too.
+    position outside the cache is copied as it is, its gradient too.  A backward
+    pass can be captured into a graph where torch's own can: while no eager graph
+    of the same leaves is alive.
     """
     return (_module or _binding()).multi_axis(q, k, positions, cos_sin_cache, sections, interleaved, inverse, status)
 
@@ -170,14 +172,15 @@ def attend_shared_prefix(
 
     Returns ``out``, and with ``return_lse`` also the logarithm of each row's
     sum of exponentials (float32 ``[tokens, q_heads]``).  A row that sees no key
-    is zeros, its logarithm minus infinity; so are rows of no request in an
-    ``out`` that the call allocates, while a given ``out`` keeps them.
+    is zeros, its logarithm minus infinity; so are rows of no request, but that
+    a given ``out``, which must not overlap q, keeps them as they were.
 
     ``workspace``: device memory of :func:`attend_workspace_bytes`, 32-byte
     aligned, for one call at a time; by default the call takes it from torch's
     allocator.  Lengths, starts and tables are read on the device, so a captured
-    call follows them; ``prefix_len`` is part of the capture.  There is no
-    backward pass.
+    call follows them; ``prefix_len`` is part of the capture.  What a page holds
+    behind the last key does not matter; a key that some rows of a request do
+    not see yet must be finite.  There is no backward pass.
     """
     return (_module or _binding()).attend(q, key_cache, value_cache, block_table, seq_lens, query_starts, prefix_table,
                                           prefix_len, scale, out, return_lse, workspace, status)

@@ -174,6 +174,30 @@ def test_rows_of_no_request():
     agree(batch, (out[:3], lse[:3]))
 
 
+def test_rows_of_no_request_in_a_given_out_keep_their_values_but_have_an_lse():
+    batch = Batch([70, 20], counts=[2, 1], prefix=100, spare=400)
+    for prefix_len in (0, 100):
+        given = torch.full_like(batch.q, 7.0)
+        torch.full((403, 6), math.nan, dtype=torch.float32, device=DEV)  # what the allocator may hand out next
+        _, lse = batch.run(out=given, prefix_len=prefix_len, prefix_table=batch.prefix_table if prefix_len else None)
+        assert (given[3:] == 7.0).all() and (lse[3:] == -math.inf).all() and torch.isfinite(lse[:3]).all()
+
+
+@pytest.mark.parametrize("batch_size,at", [(3, 1), (100, 70)])
+@pytest.mark.parametrize("prefix", [0, 200])
+def test_with_starts_that_decrease_no_row_belongs_to_a_request(batch_size, at, prefix):
+    """Else the requests could claim the same tokens again and again."""
+    batch = Batch([64] * batch_size, counts=[2] * batch_size, prefix=prefix)
+    starts = torch.tensor(batch.starts, device=DEV)
+    starts[at] = batch.tokens
+    out, lse = batch.run(query_starts=starts)
+    assert batch.status.item() == _native.DEV_BAD_LENGTH
+    assert (out == 0).all() and (lse == -math.inf).all()
+    given = torch.full_like(batch.q, 7.0)
+    batch.run(query_starts=starts, out=given)
+    assert (given == 7.0).all()
+
+
 def test_strides():
     """q and out inside wider tensors, a head-major cache, pages with room between them."""
     batch = Batch([70, 3, 200], counts=[1, 3, 2], prefix=130, heads=(8, 2))

@@ -145,6 +145,8 @@ def tensors():
     (dict(key_cache=lambda t: t.expand(2, 16, 2, 256), value_cache=lambda t: t.expand(2, 16, 2, 256)), ValueError),
     (dict(key_cache=lambda t: t[:, :1].expand(2, 16, 1, 256)), RuntimeError),
     (dict(k=lambda t: t.requires_grad_()), ValueError), (dict(status=torch.zeros(1)), TypeError),
+    (dict(key_cache=lambda t: t.requires_grad_()), ValueError),
+    (dict(value_cache=lambda t: t.requires_grad_()), ValueError),
     (dict(sections=(16, 16)), ValueError),
 ])
 def test_append_refuses(change, error):
@@ -180,6 +182,8 @@ def test_multi_axis_inplace_refuses(change, error):
 @pytest.mark.parametrize("change,error", [
     (dict(q=lambda t: t[:3]), ValueError), (dict(q=lambda t: t.half()), TypeError),
     (dict(q=lambda t: t.requires_grad_()), ValueError), (dict(block_table=lambda t: t.long()), TypeError),
+    (dict(key_cache=lambda t: t.requires_grad_()), ValueError),
+    (dict(value_cache=lambda t: t.requires_grad_()), ValueError),
     (dict(block_table=lambda t: t[0]), ValueError), (dict(seq_lens=lambda t: t.int()), TypeError),
     (dict(seq_lens=lambda t: t[:2]), ValueError), (dict(query_starts=torch.zeros(3, dtype=torch.int64)), ValueError),
     (dict(prefix_len=17), ValueError), (dict(prefix_len=-1), ValueError), (dict(prefix_table=None), ValueError),
