@@ -30,7 +30,7 @@
 //   4..11  softmax: two threads a row, 64 keys each; rescaling of O; results.
 //          At first they help to add up the line and bring the first Q rows
 // S and O live in TMEM, S twice, so that the softmax of one tile runs beside
-// the products of its neighbours; P (BF16) takes the place of S.  P is rounded
+// the products of its neighbours; P (BF16) takes columns of S.  P is rounded
 // to BF16 because the product with the BF16 values takes both operands in one
 // type; l sums the unrounded p, and S, m, l and O are FP32.
 
@@ -59,7 +59,14 @@ constexpr int kPieces = 4;             // ring of piece descriptors
 constexpr int kThreads = 384;
 constexpr int kSoftmaxWarp0 = 4, kSoftmaxWarps = 8;
 constexpr int kPieceReaders = 3 + kSoftmaxWarps;  // producer, two issuers, softmax warps
-constexpr uint32_t kColS = 0, kColO = 256;  // TMEM columns: S (and P) of even and odd tiles, then O
+// TMEM columns.  S (128 columns) and P (64) of three tiles in turn share the first
+// 256, in quarters: S(t) in 0 and 1, P(t) in 0; S(t + 1) in 2 and 3, P(t + 1) in 3;
+// S(t + 2) in 1 and 2, P(t + 2) in 2.  Then the scores of two tiles in three need
+// not wait for the products before them, only for S to have been read: 2560 query
+// tokens 119.2 us with S and P of a tile in the same half, 116.4 so.
+constexpr uint32_t kColO = 256;
+__host__ __device__ constexpr uint32_t col_s(uint32_t third) { return third == 0 ? 0 : third == 1 ? 128 : 64; }
+__host__ __device__ constexpr uint32_t col_p(uint32_t third) { return third == 0 ? 0 : third == 1 ? 192 : 128; }
 constexpr long long kWaitClocks = 1ll << 32;  // about two seconds
 constexpr float kRescaleStep = 8.0f;   // O is rescaled when the maximum grows by more than 2^8
 
@@ -239,7 +246,7 @@ struct LineSums {
 
 struct Control {
   uint64_t full_k[kStagesK], empty_k[kStagesK], full_v[kStagesV], empty_v[kStagesV];
-  uint64_t s_full[2], p_full[2], pv_done[2];
+  uint64_t s_full[2], s_read[2], p_full[4], pv_done[4];
   uint64_t q_first, q_full, q_empty, o_free, drained[2];
   uint64_t swap[4];  // the two warps of 32 rows
   uint64_t piece_full[kPieces], piece_empty[kPieces];
@@ -758,23 +765,25 @@ __device__ __forceinline__ void drain(uint64_t* bar) {
 // other's (both waits take some 300 clocks even when they are over).
 //
 // The products of a tile take 2050 clocks by themselves.  Beside the copies they
-// take some 2600: those of the scores read Q and K from shared memory at 128
+// take 2600 to 2800: those of the scores read Q and K from shared memory at 128
 // bytes a clock, all that it has, so that a tile's 128 KB (Q, K), 64 KB (V) and
 // 128 KB of copies written make 2500.
 //
-// S(t) = Q K(t)^T, once P(t - 2), which takes the same columns, has been used.
+// S(t) = Q K(t)^T, once what its columns held before has been used: S(t - 1)
+// read, but for the second of three tiles, and the products with P(t - 3) done, or
+// for the second with P(t - 2); the third's wait for S(t - 1) says so too.
 __device__ void issue_scores(Control& ctl, uint32_t q, uint32_t ring, uint32_t tmem) {
   constexpr uint32_t kIdesc = instr_desc(kKeys, false);
   const uint64_t q_desc = operand_desc(q, 16, 1024);
   PieceReader pieces;
   Piece p;
-  uint32_t t = 0, n = 0;  // tiles and halves of K so far
+  uint32_t t = 0, n = 0, third = 0;  // tiles and halves of K so far; t % 3
   bool ok = true;
   for (uint32_t np = 0; ok && pieces.next(ctl, p); ++np) {
     const int tiles = int(uniform(p.tiles));
-    for (int j = 0; ok && j < tiles; ++j, ++t) {
+    for (int j = 0; ok && j < tiles; ++j, ++t, third = third == 2 ? 0 : third + 1) {
       const uint32_t buf = t & 1;
-      const uint32_t d = tmem + kColS + buf * kKeys;
+      const uint32_t d = uniform(tmem + col_s(third));
       if (j == 0) {
         ok = np == 0 ? mbar_wait(ctl, &ctl.q_first, 0) : mbar_wait(ctl, &ctl.q_full, (np & 1) ^ 1);
         // the Q rows came by ordinary asynchronous copies
@@ -785,7 +794,11 @@ __device__ void issue_scores(Control& ctl, uint32_t q, uint32_t ring, uint32_t t
         const uint32_t s = uniform(n % kStagesK);
         const uint64_t k_desc = operand_desc(ring + s * kStageBytes, 16, 1024);
         ok = ok && mbar_wait(ctl, &ctl.full_k[s], (n / kStagesK) & 1);
-        if (half == 0) ok = ok && (t < 2 || mbar_wait(ctl, &ctl.pv_done[buf], ((t >> 1) & 1) ^ 1));
+        if (half == 0) {
+          const uint32_t used = t - (third == 1 ? 2 : 3), read = t - 1;
+          if (third < 2 && t >= 3) ok = ok && mbar_wait(ctl, &ctl.pv_done[used & 3], (used >> 2) & 1);
+          if (third != 1 && t >= 2) ok = ok && mbar_wait(ctl, &ctl.s_read[read & 1], (read >> 1) & 1);
+        }
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tmem_fence_after();
@@ -819,14 +832,13 @@ __device__ void issue_values(const AttendArgs& a, Control& ctl, uint32_t ring, u
   for (uint32_t ks = 0; ks < kHalfKeys / 16; ++ks) at[ks] = (ks / per * per * 16 * 512 + ks % per * 16 * 128) >> 4;
   PieceReader pieces;
   Piece p;
-  uint32_t t = 0, n = 0;
+  uint32_t t = 0, n = 0, third = 0;
   bool ok = true;
   for (uint32_t np = 0; ok && pieces.next(ctl, p); ++np) {
     const int tiles = int(uniform(p.tiles));
-    for (int j = 0; ok && j < tiles; ++j, ++t) {
-      const uint32_t buf = t & 1;
-      // P: keys 0..63 in the first 32 columns of S, keys 64..127 in those from column 64
-      const uint32_t p_at = tmem + kColS + buf * kKeys;
+    for (int j = 0; ok && j < tiles; ++j, ++t, third = third == 2 ? 0 : third + 1) {
+      const uint32_t buf = t & 3;
+      const uint32_t p_at = uniform(tmem + col_p(third));
 #pragma unroll
       for (int half = 0; half < 2; ++half, ++n) {
         const uint32_t s = uniform(n % kStagesV);
@@ -834,14 +846,14 @@ __device__ void issue_values(const AttendArgs& a, Control& ctl, uint32_t ring, u
         ok = ok && mbar_wait(ctl, &ctl.full_v[s], (n / kStagesV) & 1);
         if (half == 0)
           ok = ok && (j > 0 || mbar_wait(ctl, &ctl.o_free, (np & 1) ^ 1)) &&
-               mbar_wait(ctl, &ctl.p_full[buf], (t >> 1) & 1);
+               mbar_wait(ctl, &ctl.p_full[buf], (t >> 2) & 1);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tmem_fence_after();
         if (elect_one()) {
 #pragma unroll
           for (int ks = 0; ks < kHalfKeys / 16; ++ks)
-            mma_ts(tmem + kColO, p_at + half * 64 + ks * 8, v_desc + at[ks], kIdesc, j + half + ks > 0);
+            mma_ts(tmem + kColO, p_at + half * 32 + ks * 8, v_desc + at[ks], kIdesc, j + half + ks > 0);
           if (half == 1) mma_commit(&ctl.pv_done[buf]);
           mma_commit(&ctl.empty_v[s]);
         }
@@ -862,7 +874,7 @@ __device__ void softmax_rows(const AttendArgs& a, Control& ctl, Swap& swap, uint
   const int half = (threadIdx.x >> 5) >= kSoftmaxWarp0 + 4;
   const int row = warp * 32 + lane;
   const uint32_t mine = tmem + (uint32_t(warp * 32) << 16);
-  const uint32_t my_s = mine + kColS + half * 64, my_o = mine + kColO + half * kHalfLanes;
+  const uint32_t my_o = mine + kColO + half * kHalfLanes;
   const float c = a.scale;
   if (a.batch > 32) {
     const int w = (threadIdx.x >> 5) - kSoftmaxWarp0;
@@ -875,7 +887,7 @@ __device__ void softmax_rows(const AttendArgs& a, Control& ctl, Swap& swap, uint
   }
   PieceReader pieces;
   Piece p;
-  uint32_t tile = 0, swaps = 0;
+  uint32_t tile = 0, third = 0, swaps = 0;
   // hands `value` to the row's other thread and returns that thread's
   auto trade = [&](float value, float& other) {
     const uint32_t parity = swaps & 1;
@@ -901,14 +913,20 @@ __device__ void softmax_rows(const AttendArgs& a, Control& ctl, Swap& swap, uint
     const int own_left = seen - behind + p.shared_tiles * kKeys, all_left = own_left - seen + p.keys;
     float m = -INFINITY, l = 0.0f;
     for (int j = 0; j < p.tiles; ++j) {
-      const uint32_t t = tile + j, buf = t & 1, ph = (t >> 1) & 1;
-      if (!__all_sync(0xffffffffu, mbar_wait(ctl, &ctl.s_full[buf], ph))) return;
+      const uint32_t t = tile + j, buf = t & 1;
+      const uint32_t my_s = mine + col_s(third) + half * 64, my_p = mine + col_p(third) + half * 32;
+      third = third == 2 ? 0 : third + 1;
+      if (!__all_sync(0xffffffffu, mbar_wait(ctl, &ctl.s_full[buf], (t >> 1) & 1))) return;
       tmem_fence_after();
+      if (!busy && lane == 0) mbar_arrive(&ctl.s_read[buf]);
       if (busy) {
         uint32_t s[2][32];
-        tmem_load32(my_s + buf * kKeys, s[0]);
-        tmem_load32(my_s + buf * kKeys + 32, s[1]);
+        tmem_load32(my_s, s[0]);
+        tmem_load32(my_s + 32, s[1]);
         tmem_load_wait();
+        tmem_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ctl.s_read[buf]);
         // of these 64 keys, those that the row sees
         const int left = (j < in_shared ? shared_left : own_left) - j * kKeys;
         if (left < 64) {
@@ -928,7 +946,7 @@ __device__ void softmax_rows(const AttendArgs& a, Control& ctl, Swap& swap, uint
         const bool grown = row < p.rows && (top - m) * c > kRescaleStep;
         if (j > 0 && __any_sync(0xffffffffu, grown)) {
           const uint32_t tp = t - 1;
-          if (!__all_sync(0xffffffffu, mbar_wait(ctl, &ctl.pv_done[tp & 1], (tp >> 1) & 1))) return;
+          if (!__all_sync(0xffffffffu, mbar_wait(ctl, &ctl.pv_done[tp & 3], (tp >> 2) & 1))) return;
           tmem_fence_after();
           const float f = grown ? exp2_approx((m - top) * c) : 1.0f;
           l *= f;
@@ -958,8 +976,9 @@ __device__ void softmax_rows(const AttendArgs& a, Control& ctl, Swap& swap, uint
           pk[i / 2] = pack_bf16x2(p0, p1);
         }
         l += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+        // of columns that the row's other thread may have had in S: it had read them when it gave its maximum
         __syncwarp();
-        tmem_store32(my_s + buf * kKeys, pk);
+        tmem_store32(my_p, pk);
         tmem_store_wait();
       }
       // V rows past the keys weigh nothing, but what their page holds may be
@@ -968,7 +987,7 @@ __device__ void softmax_rows(const AttendArgs& a, Control& ctl, Swap& swap, uint
       const int whole = (j < in_shared ? shared_left : all_left) - j * kKeys;
       if (whole < kHalfKeys) {
         // V(t - 1), the stage's last contents, has landed if it has been used
-        if (t > 0 && !__all_sync(0xffffffffu, mbar_wait(ctl, &ctl.pv_done[buf ^ 1], ((t - 1) >> 1) & 1))) return;
+        if (t > 0 && !__all_sync(0xffffffffu, mbar_wait(ctl, &ctl.pv_done[(t - 1) & 3], ((t - 1) >> 2) & 1))) return;
         const uint32_t n = 2 * t + half, st = n % kStagesV;
         if (!__all_sync(0xffffffffu, mbar_wait(ctl, &ctl.full_v[st], (n / kStagesV) & 1))) return;
         uint8_t* v = ring + (kStagesK + st) * kStageBytes;
@@ -982,11 +1001,11 @@ __device__ void softmax_rows(const AttendArgs& a, Control& ctl, Swap& swap, uint
       }
       tmem_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&ctl.p_full[buf]);
+      if (lane == 0) mbar_arrive(&ctl.p_full[t & 3]);
     }
     // O of the piece
     const uint32_t tl = tile + p.tiles - 1;
-    if (!__all_sync(0xffffffffu, mbar_wait(ctl, &ctl.pv_done[tl & 1], (tl >> 1) & 1))) return;
+    if (!__all_sync(0xffffffffu, mbar_wait(ctl, &ctl.pv_done[tl & 3], (tl >> 2) & 1))) return;
     tmem_fence_after();
     if (busy) {
       float other;
@@ -1072,6 +1091,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&ctl.s_full[i], 1);
+      mbar_init(&ctl.s_read[i], kSoftmaxWarps);
+    }
+    for (int i = 0; i < 4; ++i) {
       mbar_init(&ctl.p_full[i], kSoftmaxWarps);
       mbar_init(&ctl.pv_done[i], 1);
     }

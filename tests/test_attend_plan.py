@@ -307,3 +307,33 @@ def test_a_stage_is_looked_at_only_when_its_last_contents_are_known_to_have_land
                         assert last_t <= (t - 1 if t in starts else t - 2) if last_v else last_t <= t
                 else:  # behind pv_done(t - 2); the issuer itself took K before t
                     assert last_t <= t - 2 if last_v else last_t < t
+
+
+def test_scores_wait_for_all_that_their_columns_held():
+    """S(t) and P(t) lie in quarters of 256 TMEM columns.  What issue_scores waits for before S(t), with what those
+    waits prove, covers every S that was to be read and every P that was to be used where S(t) goes; P(t) lies in S(t).
+    No barrier is waited for that may be a phase ahead or behind."""
+    s_at, p_at = [{0, 1}, {2, 3}, {1, 2}], [0, 3, 2]
+    read, used = {}, {}  # issue_scores(t): S read and P used up to these tiles
+    for t in range(60):
+        third = t % 3
+        assert p_at[third] in s_at[third]
+        read[t], used[t] = read.get(t - 1, -1), used.get(t - 1, -1)
+        if third < 2 and t >= 3:
+            wait = t - (2 if third == 1 else 3)
+            assert wait - 4 <= used[t] and wait + 4 >= t  # pv_done, four phases
+            used[t] = max(used[t], wait)
+            read[t] = max(read[t], wait)
+        if third != 1 and t >= 2:
+            assert t - 3 <= read[t] and t + 1 >= t  # s_read, two phases
+            read[t] = max(read[t], t - 1)
+            used[t] = max(used[t], used[t - 1])
+        for u in range(t):
+            if s_at[u % 3] & s_at[third]:
+                assert u <= read[t], (t, u)
+            if p_at[u % 3] in s_at[third]:
+                assert u <= used[t], (t, u)
+        # S(t) is there: the softmax warps look at pv_done(t - 1), and their next phases of s_full and p_full
+        assert t - 5 <= used[t]
+        assert t - 2 <= read[t], "s_full(t) must not complete before every warp has seen s_full(t - 2)"
+        assert t - 4 <= used[t], "p_full(t) must not complete before its last phase has been used"
