@@ -4,9 +4,8 @@
 //
 // A small launch takes the GPU about 2 us.  The same checks and call through
 // Python and ctypes took 12 us (multi-axis, 16 tokens), 16 us (append, 32
-// tokens) and 23 us (attention, one request), and the differentiable form 147 us
-// for 44 us of device work, so these operators check their arguments, allocate
-// and record gradients here.  Python's wrappers (paged.py) carry the signatures
+// tokens) and 23 us (attention, one request), and the differentiable form 147 us,
+// so these operators check their arguments, allocate and record gradients here.  Python's wrappers (paged.py) carry the signatures
 // and the documentation.
 
 #include <torch/csrc/autograd/python_variable.h>
@@ -17,11 +16,15 @@
 #include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
-#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 
 #include <array>
 #include <cmath>
 #include <limits>
+#include <memory>
+#include <mutex>
 #include <stdexcept>
 #include <string>
 
@@ -30,7 +33,6 @@
 namespace {
 
 using at::Tensor;
-using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 using OptTensor = std::optional<Tensor>;
 
@@ -62,8 +64,10 @@ const char* dtype_name(at::ScalarType t) {
 
 void check(const Tensor& t, const char* name, at::ScalarType dtype, c10::DeviceIndex index) {
   TORCH_CHECK_VALUE(t.defined(), name, " is required");
-  TORCH_CHECK_TYPE(t.scalar_type() == dtype, name, " must be ", dtype_name(dtype), ", got ", dtype_name(t.scalar_type()));
-  TORCH_CHECK_VALUE(t.is_cuda() && t.get_device() == index, name, " is on ", t.device(), ", expected cuda:", int(index));
+  TORCH_CHECK_TYPE(t.scalar_type() == dtype, name, " must be ", dtype_name(dtype), ", got ",
+                   dtype_name(t.scalar_type()));
+  TORCH_CHECK_VALUE(t.is_cuda() && t.get_device() == index, name, " is on ", t.device(), ", expected cuda:",
+                    int(index));
 }
 
 c10::DeviceIndex device_index(const Tensor& t) {
@@ -234,43 +238,65 @@ variable_list rotated(const Tensor& x, const char* x_name, const OptTensor& y, c
   return {x_out};
 }
 
-// Rotated copies of x and y; the gradient of a rotation is the inverse rotation.
-struct MultiAxis : torch::autograd::Function<MultiAxis> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& x, const OptTensor& y, const Tensor& positions,
-                               const Tensor& cos_sin, const std::vector<int64_t>& sections, bool interleaved,
-                               bool inverse, const char* x_name, const OptTensor& status) {
-    ctx->save_for_backward({positions, cos_sin});
-    ctx->saved_data["sections"] = sections;
-    ctx->saved_data["interleaved"] = interleaved;
-    ctx->saved_data["inverse"] = inverse;
-    ctx->saved_data["x"] = x.requires_grad();
-    ctx->saved_data["y"] = y && y->requires_grad();
-    ctx->set_materialize_grads(false);
-    return rotated(x, x_name, y, positions, cos_sin, {sections_of(sections), interleaved, inverse}, status);
-  }
+variable_list differentiable(const Tensor& x, const char* x_name, const OptTensor& y, const Tensor& positions,
+                             const Tensor& cos_sin, const Turn& turn, const OptTensor& status);
 
-  static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    const variable_list saved = ctx->get_saved_variables();
-    const std::vector<int64_t> sections = ctx->saved_data["sections"].toIntVector();
-    const bool interleaved = ctx->saved_data["interleaved"].toBool();
-    const bool inverse = !ctx->saved_data["inverse"].toBool();
-    Tensor dx = ctx->saved_data["x"].toBool() ? grads[0] : Tensor();
-    Tensor dy = grads.size() > 1 && ctx->saved_data["y"].toBool() ? grads[1] : Tensor();
+// The gradient of a rotation is the inverse rotation.  A node of its own holds
+// what that needs as it is: a forward and a backward pass take 61 us of host time
+// (35 us of a view's, with no kernel at all), and 67 through torch's custom
+// functions, which box and look up every argument.
+struct MultiAxisBackward : torch::autograd::Node {
+  torch::autograd::SavedVariable positions, cos_sin;
+  Turn turn;
+
+  variable_list apply(variable_list&& grads) override {
+    const std::lock_guard<std::mutex> lock(mutex_);
+    const Tensor at = positions.unpack(), rows = cos_sin.unpack();
+    const Turn back_turn{turn.sections, turn.interleaved, !turn.inverse};
+    Tensor dx = task_should_compute_output(0) ? grads[0] : Tensor();
+    Tensor dy = num_outputs() > 1 && task_should_compute_output(1) ? grads[1] : Tensor();
     if (dx.defined() || dy.defined()) {
       const bool both = dx.defined() && dy.defined();
-      const Tensor& first = dx.defined() ? dx : dy;
-      const OptTensor second = both ? OptTensor(dy) : std::nullopt;
-      const variable_list back =
-          at::GradMode::is_enabled()
-              ? apply(first, second, saved[0], saved[1], sections, interleaved, inverse, "gradient", std::nullopt)
-              : rotated(first, "gradient", second, saved[0], saved[1], {sections_of(sections), interleaved, inverse},
-                        std::nullopt);
+      const variable_list back = differentiable(dx.defined() ? dx : dy, "gradient", both ? OptTensor(dy) : std::nullopt,
+                                                at, rows, back_turn, std::nullopt);
       (dx.defined() ? dx : dy) = back[0];
       if (both) dy = back[1];
     }
-    return {dx, dy, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+    if (num_outputs() == 1) return {dx};
+    return {dx, dy};
   }
+
+  void release_variables() override {
+    const std::lock_guard<std::mutex> lock(mutex_);
+    positions.reset_data();
+    cos_sin.reset_data();
+  }
+
+  std::string name() const override { return "MultiAxisBackward"; }
 };
+
+// Rotated copies of x and y, with their history where gradients are wanted.
+variable_list differentiable(const Tensor& x, const char* x_name, const OptTensor& y, const Tensor& positions,
+                             const Tensor& cos_sin, const Turn& turn, const OptTensor& status) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!x._fw_grad(0).defined() && !(y && y->_fw_grad(0).defined()),
+                              "rope_multi_axis has no forward-mode derivative");
+  std::shared_ptr<MultiAxisBackward> node;
+  if (at::GradMode::is_enabled() && (x.requires_grad() || (y && y->requires_grad()))) {
+    node = std::shared_ptr<MultiAxisBackward>(new MultiAxisBackward(), torch::autograd::deleteNode);
+    node->set_next_edges(y ? torch::autograd::collect_next_edges(x, *y) : torch::autograd::collect_next_edges(x));
+    node->positions = torch::autograd::SavedVariable(positions, false);
+    node->cos_sin = torch::autograd::SavedVariable(cos_sin, false);
+    node->turn = turn;
+  }
+  variable_list out;
+  {
+    const at::NoGradGuard no_grad;
+    out = rotated(x, x_name, y, positions, cos_sin, turn, status);
+  }
+  if (node)
+    for (const Tensor& t : out) torch::autograd::set_history(t, node);
+  return out;
+}
 
 // ---------------------------------------------------------------------------
 // Python's arguments and results.
@@ -350,9 +376,9 @@ PyObject* multi_axis(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const Tensor q = query_arg(args[0]), k = tensor_arg(args[1], "key");
   device_index(q);
   const variable_list out =
-      MultiAxis::apply(q, OptTensor(k), tensor_arg(args[2], "positions"), tensor_arg(args[3], "cos_sin_cache"),
-                       ints_arg(args[4]), bool_arg(args[5]), bool_arg(args[6]), "query",
-                       opt_tensor_arg(args[7], "status"));
+      differentiable(q, "query", k, tensor_arg(args[2], "positions"), tensor_arg(args[3], "cos_sin_cache"),
+                     {sections_of(ints_arg(args[4])), bool_arg(args[5]), bool_arg(args[6])},
+                     opt_tensor_arg(args[7], "status"));
   return PyTuple_Pack(2, THPObjectPtr(THPVariable_Wrap(out[0])).get(), THPObjectPtr(THPVariable_Wrap(out[1])).get());
   WELM_END
 }

@@ -247,3 +247,45 @@ def test_in_place_write_is_seen_by_autograd():
     welm.rope_multi_axis_inplace(a, b, positions.to(DEV), cos_sin.to(DEV), (16, 8, 8))
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+def test_gradients_of_one_input_and_of_one_output():
+    """Inputs and outputs that no gradient is wanted of or comes from; a second pass through a freed graph is refused."""
+    qkv, q, k, positions, cos_sin = make(33, 3)
+    pos, cache = positions.to(DEV), cos_sin.to(DEV)
+    for wants in ((True, False), (False, True), (True, True)):
+        a, b = (t.to(DEV).contiguous().requires_grad_(w) for t, w in zip((q, k), wants))
+        outs = welm.rope_multi_axis(a, b, pos, cache, (16, 8, 8))
+        for which in (0, 1):
+            w = torch.ones_like(outs[which])
+            got = torch.autograd.grad(outs[which], [t for t in (a, b) if t.requires_grad], w, retain_graph=True,
+                                      allow_unused=True)
+            whole = iter(got)
+            for i, t in enumerate((a, b)):
+                if not t.requires_grad:
+                    continue
+                g = next(whole)
+                if i != which:
+                    assert g is None or (g == 0).all()
+                else:
+                    close(g, torch.ones_like((q, k)[i]), positions, cos_sin, (16, 8, 8), False, inverse=True)
+        outs[0].sum().backward()
+        with pytest.raises(RuntimeError, match="second time"):
+            outs[0].sum().backward()
+
+
+def test_positions_changed_before_the_backward_pass_are_noticed():
+    qkv, q, k, positions, cos_sin = make(5, 3)
+    a, b, pos = q.to(DEV).contiguous().requires_grad_(), k.to(DEV).contiguous(), positions.to(DEV)
+    out = welm.rope_multi_axis(a, b, pos, cos_sin.to(DEV), (16, 8, 8))[0]
+    pos.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+
+
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fwad
+    qkv, q, k, positions, cos_sin = make(5, 3)
+    a, b = q.to(DEV).contiguous(), k.to(DEV).contiguous()
+    with fwad.dual_level(), pytest.raises(NotImplementedError):
+        welm.rope_multi_axis(fwad.make_dual(a, torch.ones_like(a)), b, positions.to(DEV), cos_sin.to(DEV), (16, 8, 8))
