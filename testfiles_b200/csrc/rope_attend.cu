@@ -172,10 +172,15 @@ struct Request {
 // A request as the device arrays have it, and checked.
 struct RawRequest {
   int64_t start, end, len;
-  __device__ __forceinline__ void load(const AttendArgs& a, int b) {
-    start = a.query_starts != nullptr ? __ldg(a.query_starts + b) : b;
-    end = a.query_starts != nullptr ? __ldg(a.query_starts + b + 1) : b + 1;
-    len = __ldg(a.seq_lens + b);
+  __device__ __forceinline__ void load(const AttendArgs& a, int b, bool hint = false) {
+    start = end = b;
+    if (a.query_starts != nullptr) {
+      start = hint ? hint_load(a.query_starts + b) : __ldg(a.query_starts + b);
+      end = hint ? hint_load(a.query_starts + b + 1) : __ldg(a.query_starts + b + 1);
+    } else {
+      ++end;
+    }
+    len = hint ? hint_load(a.seq_lens + b) : __ldg(a.seq_lens + b);
   }
   __device__ __forceinline__ Request checked(const AttendArgs& a, bool tell) const {
     const int64_t lo = clamp64(start, 0, a.tokens), hi = clamp64(end, lo, a.tokens), n = clamp64(len, 0, a.max_len);
@@ -250,11 +255,12 @@ struct Control {
   uint64_t q_first, q_full, q_empty, o_free, drained[2];
   uint64_t swap[4];  // the two warps of 32 rows
   uint64_t piece_full[kPieces], piece_empty[kPieces];
-  uint64_t added;
+  uint64_t added, checked;
   Piece piece[kPieces];
   LineSums sums[kSoftmaxWarps];
   uint32_t tmem;
   int32_t failed;
+  int32_t changed;  // 1: some of the requests were not as hinted
 };
 
 // The two halves of a row's keys swap their maxima (even and odd tiles apart)
@@ -442,23 +448,24 @@ __device__ __forceinline__ bool load_queries(const AttendArgs& a, Control& ctl, 
 
 // Units of the requests from `first` on, a request a lane and then every `step`th
 // after it, one copy of the code, which nobody has run yet, for all of them.
-// `kept` becomes the lane's first request.
-__device__ __forceinline__ LineSums add_up(const AttendArgs& a, int first, int step, Request& kept) {
+// `kept` becomes the lane's first request.  With `hint` the arrays may not be
+// written yet.
+__device__ __forceinline__ LineSums add_up(const AttendArgs& a, int first, int step, bool hint, RawRequest& kept) {
   const int lane = threadIdx.x & 31;
   LineSums sums{0, 0, 0, 0};
   RawRequest next;
-  if (first + lane < a.batch) next.load(a, first + lane);
+  if (first + lane < a.batch) next.load(a, first + lane, hint);
 #pragma unroll 1
   for (int b = first + lane; b < a.batch; b += step) {
     const RawRequest raw = next;
-    if (b + step < a.batch) next.load(a, b + step);
-    const Request r = raw.checked(a, blockIdx.x == 0);
+    if (b + step < a.batch) next.load(a, b + step, hint);
+    const Request r = raw.checked(a, !hint && blockIdx.x == 0);
     const int n = r.row_tiles(a);
     sums.units += r.all_units(a, -1);
     sums.row_tiles += n;
     sums.seeing += n == 0 ? 0 : r.seeing_before(a, n - 1) + (r.len > 0);
     sums.decreasing += raw.end < raw.start;
-    if (b == first + lane) kept = r;
+    if (b == first + lane) kept = raw;
   }
   sums.units = __reduce_add_sync(0xffffffffu, sums.units);
   sums.row_tiles = __reduce_add_sync(0xffffffffu, sums.row_tiles);
@@ -467,21 +474,63 @@ __device__ __forceinline__ LineSums add_up(const AttendArgs& a, int first, int s
   return sums;
 }
 
+// Whether what was read of request `b` before the dependency wait still holds, in
+// every lane; CTA 0 reports what is out of range.
+__device__ __forceinline__ bool still_so(const AttendArgs& a, int b, const RawRequest& hint) {
+  bool same = true;
+  if (b < a.batch) {
+    RawRequest now;
+    now.load(a, b);
+    now.checked(a, blockIdx.x == 0);
+    same = now.start == hint.start && now.end == hint.end && now.len == hint.len;
+  }
+  return __all_sync(0xffffffffu, same);
+}
+
+// While the previous kernel may still run, a batch of a request a lane is added up
+// and the CTA's first piece found from lengths and starts as they are then.  After
+// the dependency wait every warp reads its requests again: if one has changed, all
+// is done again from what it says now.
+__device__ __forceinline__ bool hints(const AttendArgs& a) { return a.batch <= 32 * (1 + kSoftmaxWarps); }
+
 // Adds up the requests' units, finds where this CTA's run begins and lists the
 // run's pieces; CTA 0 also notes the line for the join.  The softmax warps, which
 // have nothing to do yet, add up what is past the first 32 requests: 128 requests
 // over a prefix 33.0 us with one warp for all, eight requests a lane at once, and
 // 32.0 so; one request 11.1 and 10.5.
-__device__ void list_pieces(const AttendArgs& a, Control& ctl, uint32_t q) {
+// Returns true if all has to be done again, without hints.
+__device__ __forceinline__ bool list_once(const AttendArgs& a, Control& ctl, uint32_t q, bool hint) {
   const int lane = threadIdx.x & 31, cta = blockIdx.x;
   const int key_tiles = div_up(a.prefix_len, kKeys);
+  bool entered = !hint, again = false;
+  RawRequest first_raw{0, 0, 0};
+  const int64_t end_of_last = a.query_starts == nullptr ? a.tokens
+                              : hint                    ? hint_load(a.query_starts + a.batch)
+                                                        : __ldg(a.query_starts + a.batch);
+  LineSums sums = add_up(a, 0, 32 * (1 + kSoftmaxWarps), hint, first_raw);
+  // Ends the time of hints; false if they do not hold (any more).
+  auto enter = [&] {
+    if (entered) return true;
+    entered = true;
+    pdl_enter();
+    bool same = still_so(a, lane, first_raw);
+    if (a.query_starts != nullptr) same = same && __ldg(a.query_starts + a.batch) == end_of_last;
+    if (a.batch > 32) {
+      same = __all_sync(0xffffffffu, mbar_wait(ctl, &ctl.checked, 0)) && same;
+      same = same && *reinterpret_cast<volatile int32_t*>(&ctl.changed) == 0;
+    }
+    again = !same;
+    return same;
+  };
   // The 32 requests from `held` on, one a lane: its units, and with those before it in the 32.
   Request mine{0, 0, 0};
+  if (lane < a.batch) mine = first_raw.checked(a, false);
   int held = 0, my_units = 0, my_sum = 0, joint = -1;
   auto hold = [&](int b0) {
     if (b0 != held) {
       held = b0;
       mine = Request{0, 0, 0};
+      if (!enter()) return;
       if (b0 + lane < a.batch) {
         RawRequest raw;
         raw.load(a, b0 + lane);
@@ -495,10 +544,8 @@ __device__ void list_pieces(const AttendArgs& a, Control& ctl, uint32_t q) {
       if (lane >= d) my_sum += x;
     }
   };
-  const int64_t end_of_last = a.query_starts != nullptr ? __ldg(a.query_starts + a.batch) : a.tokens;
-  LineSums sums = add_up(a, 0, 32 * (1 + kSoftmaxWarps), mine);
   if (a.batch > 32) {
-    if (!__all_sync(0xffffffffu, mbar_wait(ctl, &ctl.added, 0))) return;
+    if (!__all_sync(0xffffffffu, mbar_wait(ctl, &ctl.added, 0))) return false;
 #pragma unroll
     for (int w = 0; w < kSoftmaxWarps; ++w) {
       sums.units += ctl.sums[w].units;
@@ -529,6 +576,7 @@ __device__ void list_pieces(const AttendArgs& a, Control& ctl, uint32_t q) {
   int n = 0;
   // every lane holds the piece; lane 0 writes it
   auto emit = [&](const Piece& p) {
+    if (!enter()) return false;
     const int s = n % kPieces;
     const bool ok = __all_sync(0xffffffffu, mbar_wait(ctl, &ctl.piece_empty[s], ((n / kPieces) & 1) ^ 1));
     if (!ok) return false;
@@ -575,6 +623,7 @@ __device__ void list_pieces(const AttendArgs& a, Control& ctl, uint32_t q) {
       held_base += __shfl_sync(0xffffffffu, my_sum, 31);
       if (held + 32 >= a.batch) break;
       hold(held + 32);
+      if (again) break;
       continue;
     }
     const int i = __ffs(past) - 1, b = held + i;
@@ -617,9 +666,10 @@ __device__ void list_pieces(const AttendArgs& a, Control& ctl, uint32_t q) {
       }
     }
   }
-  if (ok) emit(Piece{});
+  if (ok && !again) emit(Piece{});
+  if (again) return true;
   asm volatile("cp.async.wait_all;" ::: "memory");
-  if (cta != 0) return;
+  if (cta != 0) return false;
   // for the join: every request's place on the line
   int before = 0;
   for (int b0 = 0; b0 < a.batch; b0 += 32) {
@@ -638,6 +688,13 @@ __device__ void list_pieces(const AttendArgs& a, Control& ctl, uint32_t q) {
     note.by_longer = Divisor(line.each + 1);
     *a.note = note;
   }
+  return false;
+}
+
+__device__ void list_pieces(const AttendArgs& a, Control& ctl, uint32_t q) {
+  bool hint = hints(a);
+  if (!hint) pdl_enter();
+  while (list_once(a, ctl, q, hint)) hint = false;
 }
 
 // Where a box of keys is in the cache.  The block is looked at when its copies
@@ -876,14 +933,30 @@ __device__ void softmax_rows(const AttendArgs& a, Control& ctl, Swap& swap, uint
   const uint32_t mine = tmem + (uint32_t(warp * 32) << 16);
   const uint32_t my_o = mine + kColO + half * kHalfLanes;
   const float c = a.scale;
-  if (a.batch > 32) {
+  if (a.batch <= 32) {
+    pdl_enter();
+  } else {
     const int w = (threadIdx.x >> 5) - kSoftmaxWarp0;
-    Request first;
-    const LineSums sums = add_up(a, 32 * (1 + w), 32 * (1 + kSoftmaxWarps), first);
-    if (lane == 0) {
-      ctl.sums[w] = sums;
-      mbar_arrive(&ctl.added);
+    bool hint = hints(a);
+    if (!hint) pdl_enter();
+    for (int pass = 0;; ++pass) {
+      RawRequest first{0, 0, 0};
+      const LineSums sums = add_up(a, 32 * (1 + w), 32 * (1 + kSoftmaxWarps), hint, first);
+      if (lane == 0) {
+        ctl.sums[w] = sums;
+        if (pass == 0) mbar_arrive(&ctl.added);
+      }
+      bool same = true;
+      if (hint) {
+        pdl_enter();
+        same = still_so(a, 32 * (1 + w) + lane, first);
+        hint = false;
+        if (!same && lane == 0) *reinterpret_cast<volatile int32_t*>(&ctl.changed) = 1;
+      }
+      if (same) break;
     }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&ctl.checked);
   }
   PieceReader pieces;
   Piece p;
@@ -1099,6 +1172,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     mbar_init(&ctl.q_first, 32 * kSoftmaxWarps);
     mbar_init(&ctl.added, kSoftmaxWarps);
+    mbar_init(&ctl.checked, kSoftmaxWarps);
     mbar_init(&ctl.q_full, 32);
     mbar_init(&ctl.q_empty, 1);
     mbar_init(&ctl.o_free, kSoftmaxWarps);
@@ -1109,6 +1183,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&ctl.piece_empty[i], kPieceReaders);
     }
     ctl.failed = 0;
+    ctl.changed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 0 && elect_one()) {
@@ -1123,9 +1198,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   tmem_fence_before();
   __syncthreads();
   tmem_fence_after();
-  pdl_enter();
   const uint32_t tmem = ctl.tmem;
   const uint32_t q_at = smem_u32(smem), k_at = smem_u32(ring), v_at = k_at + kStagesK * kStageBytes;
+  if (warp < 3) pdl_enter();  // the others first look at hints
   if (warp == 0) {
     produce(a, ctl, &kmap, &vmap, k_at, v_at);
   } else if (warp == 1) {

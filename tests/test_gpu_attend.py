@@ -289,6 +289,45 @@ def test_captured_call_follows_lengths_and_tables():
         agree(batch, (out, lse))
 
 
+@pytest.mark.parametrize("capture", [False, True])
+@pytest.mark.parametrize("lens", [[300, 200], [130, 0], [130, 500]])
+def test_lengths_that_the_call_before_writes(lens, capture):
+    """A call may look at its lengths while the one before still runs: what counts is what that one leaves there.  Here
+    its output, the value of the only key with any weight, is the next call's lengths."""
+    first, second = Batch([1, 1], prefix=1), Batch([300, 500])
+    first.keys[first.prefix_table[0], 0] = -30 * first.q[0, 0]
+    first.keys[first.table[0, 0], 0] = 30 * first.q[0, 0]
+    first.q[:] = first.q[:1, :1]
+    first.values[first.prefix_table[0], 0] = 1.0
+    first.values[first.table[0, 0], 0] = 0.0
+    first.values[first.table[0, 0], 0, 0, :8] = torch.tensor(lens, device=DEV).view(torch.bfloat16)
+    out = torch.empty_like(first.q)
+    stale = torch.tensor([7, 200], device=DEV).view(torch.bfloat16)
+    want = second.run(seq_lens=torch.tensor(lens, device=DEV))
+    args = {**first.args(), "out": out}
+    later = {**second.args(), "seq_lens": out.view(torch.int64).flatten()[:2], "return_lse": True}
+
+    def both():
+        out[0, 0, :8] = stale
+        welm.attend_shared_prefix(first.q, first.keys, first.values, **args)
+        return welm.attend_shared_prefix(second.q, second.keys, second.values, **later)
+
+    got = both()
+    assert out.view(torch.int64).flatten()[:2].tolist() == lens
+    if capture:
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = both()
+    for _ in range(30):
+        if capture:
+            graph.replay()
+        else:
+            got = both()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert second.status.item() == 0
+
+
 def test_two_streams_at_once():
     batches = [Batch([400, 64, 5] * 9, prefix=2000, seed=s) for s in (1, 2)]
     want = [b.run() for b in batches]
