@@ -1237,21 +1237,31 @@ struct RowParts {
   int token, head;
 };
 
-// The last request that starts at or before `token`, found by the whole CTA.
+// The last request that starts at or before `token`, found by the whole CTA before
+// the dependency wait: a hint.
 __device__ __forceinline__ int find_request(const AttendArgs& a, int token, int& shared) {
   if (a.query_starts == nullptr) return token;
   if (threadIdx.x == 0) shared = 0;
   __syncthreads();
   int last = -1;
   for (int b = threadIdx.x; b < a.batch; b += blockDim.x)
-    if (__ldg(a.query_starts + b) <= token) last = b;
+    if (hint_load(a.query_starts + b) <= token) last = b;
   last = __reduce_max_sync(0xffffffffu, last);
   if ((threadIdx.x & 31) == 0 && last > 0) atomicMax(&shared, last);
   __syncthreads();
   return shared;
 }
 
-// `b`: a request that begins at or before the row's token, not far before.
+// The last request from `b` on that starts at or before `token`.
+__device__ __forceinline__ int request_from(const AttendArgs& a, int token, int b, bool hint) {
+  if (a.query_starts == nullptr) return token;
+  while (b + 1 < a.batch &&
+         (hint ? hint_load(a.query_starts + b + 1) : __ldg(a.query_starts + b + 1)) <= token)
+    ++b;
+  return b;
+}
+
+// `b`: the row's request, as far as was known before the dependency wait.
 __device__ __forceinline__ RowParts find_parts(const AttendArgs& a, const LineNote& note, int used, int flat, int b) {
   RowParts r{};
   if (flat >= a.tokens * a.q_heads) return r;
@@ -1259,16 +1269,17 @@ __device__ __forceinline__ RowParts find_parts(const AttendArgs& a, const LineNo
   const int h = a.by_group.of(hq), g = hq - h * a.group;
   r.token = token;
   r.head = hq;
-  if (a.query_starts == nullptr) {
-    b = token;
-  } else {
-    while (b + 1 < a.batch && __ldg(a.query_starts + b + 1) <= token) ++b;
-  }
   // all that has to be read at once, before any of it is looked at
   RawRequest raw;
   raw.load(a, b);
-  const int units_before = a.units_before[b];
-  const Request q = raw.checked(a, false);
+  int units_before = a.units_before[b];
+  Request q = raw.checked(a, false);
+  if (!note.nothing && token < used && (token < q.first || token >= q.first + q.count)) {
+    b = request_from(a, token, 0, false);
+    raw.load(a, b);
+    units_before = a.units_before[b];
+    q = raw.checked(a, false);
+  }
   if (note.nothing || token >= used || token < q.first || token >= q.first + q.count) {  // a row of no request
     r.live = a.fill;
     r.unused = 1;
@@ -1328,10 +1339,12 @@ __global__ void __launch_bounds__(kGroups == 1 ? 256 : 128 * kGroups, kResident)
   __shared__ float s_o[kGroups == 1 ? 1 : kGroups - 1][kGroups == 1 ? 1 : 10][128];
   const int grp = threadIdx.x >> 7, in_grp = threadIdx.x & 127;
   const int lanes8 = in_grp >> 2;  // eight lanes of the head
+  const int flat = min(int(blockIdx.x * kRowsPerCta + threadIdx.x), a.tokens * a.q_heads - 1);
+  int request = find_request(a, a.by_q_heads.of(blockIdx.x * kRowsPerCta), s_request);
+  if (threadIdx.x < kRowsPerCta) request = request_from(a, a.by_q_heads.of(flat), request, true);
   pdl_enter();
   const LineNote note = *a.note;
   const int used = used_tokens(a);
-  const int request = find_request(a, a.by_q_heads.of(blockIdx.x * kRowsPerCta), s_request);
   if (threadIdx.x < kRowsPerCta)
     parts[threadIdx.x] = find_parts(a, note, used, blockIdx.x * kRowsPerCta + threadIdx.x, request);
   __syncthreads();

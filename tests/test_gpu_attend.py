@@ -290,30 +290,37 @@ def test_captured_call_follows_lengths_and_tables():
 
 
 @pytest.mark.parametrize("capture", [False, True])
-@pytest.mark.parametrize("lens", [[300, 200], [130, 0], [130, 500]])
-def test_lengths_that_the_call_before_writes(lens, capture):
-    """A call may look at its lengths while the one before still runs: what counts is what that one leaves there.  Here
-    its output, the value of the only key with any weight, is the next call's lengths."""
-    first, second = Batch([1, 1], prefix=1), Batch([300, 500])
+@pytest.mark.parametrize("name,new,old", [
+    ("seq_lens", [300, 200], [7, 200]), ("seq_lens", [130, 0], [300, 500]), ("seq_lens", [130, 500], [300, 500]),
+    ("query_starts", [0, 130, 384], [0, 256, 384]), ("query_starts", [0, 256, 384], [0, 1, 2]),
+    ("query_starts", [0, 384, 384], [0, 0, 384]), ("query_starts", [0, 130, 384], [9, 5, 1]),
+    ("seq_lens", list(range(130, 180)), [500] * 50), ("seq_lens", [500] * 49 + [0], [500] * 50),
+])
+def test_lengths_and_starts_that_the_call_before_writes(name, new, old, capture):
+    """A call may look at them while the one before still runs: what counts is what that one leaves there.  Here its
+    output, the value of the only key with any weight, is what the next call reads."""
+    first = Batch([1, 1], prefix=1)
+    second = Batch([500] * len(new)) if name == "seq_lens" else Batch([300, 400], counts=[130, 254], prefix=200)
     first.keys[first.prefix_table[0], 0] = -30 * first.q[0, 0]
     first.keys[first.table[0, 0], 0] = 30 * first.q[0, 0]
     first.q[:] = first.q[:1, :1]
     first.values[first.prefix_table[0], 0] = 1.0
     first.values[first.table[0, 0], 0] = 0.0
-    first.values[first.table[0, 0], 0, 0, :8] = torch.tensor(lens, device=DEV).view(torch.bfloat16)
+    n = len(new)
+    first.values[first.table[0, 0], 0, 0, :4 * n] = torch.tensor(new, device=DEV).view(torch.bfloat16)
     out = torch.empty_like(first.q)
-    stale = torch.tensor([7, 200], device=DEV).view(torch.bfloat16)
-    want = second.run(seq_lens=torch.tensor(lens, device=DEV))
+    stale = torch.tensor(old, device=DEV).view(torch.bfloat16)
+    want = second.run(**{name: torch.tensor(new, device=DEV)})
     args = {**first.args(), "out": out}
-    later = {**second.args(), "seq_lens": out.view(torch.int64).flatten()[:2], "return_lse": True}
+    later = {**second.args(), name: out.view(torch.int64).flatten()[:n], "return_lse": True}
 
     def both():
-        out[0, 0, :8] = stale
+        out[0, 0, :4 * n] = stale
         welm.attend_shared_prefix(first.q, first.keys, first.values, **args)
         return welm.attend_shared_prefix(second.q, second.keys, second.values, **later)
 
     got = both()
-    assert out.view(torch.int64).flatten()[:2].tolist() == lens
+    assert out.view(torch.int64).flatten()[:n].tolist() == new
     if capture:
         torch.cuda.synchronize()
         graph = torch.cuda.CUDAGraph()
