@@ -52,8 +52,8 @@ constexpr int kQChunkBytes = kRows * 128;  // 64 lanes of 128 rows
 constexpr int kQBytes = kRows * kHeadDim * 2;
 // What an item costs beside its tiles (its Q rows, its results), in tiles.
 // Measured with 1, 2 and 3 on one B200 (graph replay, us): 128 requests over a
-// prefix 35.8, 34.9, 34.9; 24 requests' verification 24.8, 24.1, 24.6; 48
-// requests without a prefix 27.6, 27.4, 27.4.
+// prefix 32.3, 30.5, 31.4; 256 requests over 32768 shared keys 79.3, 76.4, 79.8;
+// 24 requests' verification 20.7, 21.7, 21.6; 48 requests 24.7, 24.6, 25.1.
 constexpr int kItemCost = 2;
 constexpr int kPieces = 4;             // ring of piece descriptors
 constexpr int kThreads = 384;

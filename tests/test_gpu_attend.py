@@ -98,6 +98,13 @@ def test_decode_with_prefix(prefix, lens):
     assert batch.status.item() == 0
 
 
+@pytest.mark.parametrize("prefix", [0, 70])
+@pytest.mark.parametrize("batch_size", [32, 33, 288, 289, 400])
+def test_batches_around_the_shares_of_the_warps(batch_size, prefix):
+    batch = Batch([1 + 37 * b % 150 for b in range(batch_size)], prefix=prefix)
+    agree(batch, batch.run())
+
+
 @pytest.mark.parametrize("heads", [(6, 1), (8, 2), (4, 4), (12, 2), (1, 1), (130, 1), (256, 2)])
 @pytest.mark.parametrize("block", [8, 16, 24, 64, 128, 192])
 def test_heads_and_pages(heads, block):
