@@ -198,7 +198,8 @@ __device__ __forceinline__ int used_tokens(const AttendArgs& a) {
 // begin(c + 1)).  An item's first kItemCost units stand for its own cost (its
 // rows, its results) and hold no tile; a run that ends among them does nothing
 // for the item.  No run is empty: a line of fewer units than CTAs keeps only as
-// many busy.
+// many busy.  Runs that are longer by a unit come first (with them last, 48
+// requests 25.4 -> 26.3 us, 128 over a prefix 29.9 -> 30.7).
 struct Line {
   int units, grid, each, more;  // the first `more` runs have each + 1 tiles
   __device__ __forceinline__ Line(int n, int ctas) : units(max(n, 0)), grid(min(units, ctas)) {
