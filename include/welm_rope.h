@@ -348,7 +348,7 @@ int welm_rope_ceiling_tma_slices(void* q, void* k, int64_t n_tokens, int64_t q_t
  * be NULL).  q_out == q and k_out == k (with equal strides) rotates in place
  * and moves only the rotated lanes; otherwise whole heads are copied.  The
  * outputs' rows must be apart from one another and, unless in place, from the
- * inputs; input strides may be 0.  positions is [num_axes][n_tokens] with rows
+ * inputs (WELM_ROPE_ERR_BAD_STRIDE otherwise); input strides may be 0.  positions is [num_axes][n_tokens] with rows
  * position_stride apart; an axis of no pairs is not read.  A token with a
  * position outside [0, max_position) on a used axis is left (or copied)
  * unrotated and raises WELM_ROPE_DEV_BAD_POSITION.  Pointers to heads and the

@@ -27,7 +27,7 @@ SOURCES = tuple(CSRC / name for name in (
     "rope_ordinary.cu", "rope_mirror.cu", "rope_kv_write.cu", "rope_tiles.cu", "rope_host_memory.cu",
     "rope_ceiling.cu", "rope_multi_axis.cu", "rope_kv_append.cu", "rope_attend.cu", "rope_abi.cu"))
 HEADERS = (REPO_ROOT / "include" / "welm_rope.h", *(CSRC / name for name in (
-    "rope_device.cuh", "rope_host.cuh", "rope_axes.cuh", "rope_tma.cuh")))
+    "rope_device.cuh", "rope_host.cuh", "rope_axes.cuh", "rope_rows.h", "rope_tma.cuh")))
 LIBRARY = PACKAGE_DIR / "libwelm_rope_b200.so"
 BINDING_SOURCE = CSRC / "torch_binding.cpp"
 BINDING = PACKAGE_DIR / "_welm_torch.so"
@@ -83,7 +83,7 @@ def build_binding(force: bool = False, verbose: bool = False) -> Path:
     import torch
 
     torch_dir = Path(torch.__file__).resolve().parent
-    newer = (BINDING_SOURCE, REPO_ROOT / "include" / "welm_rope.h", torch_dir / "version.py")
+    newer = (BINDING_SOURCE, CSRC / "rope_rows.h", REPO_ROOT / "include" / "welm_rope.h", torch_dir / "version.py")
     if not force and BINDING.exists() and all(p.stat().st_mtime <= BINDING.stat().st_mtime for p in newer):
         return BINDING
     cuda = Path(_nvcc()).resolve().parent.parent
@@ -92,6 +92,7 @@ def build_binding(force: bool = False, verbose: bool = False) -> Path:
         shutil.which("g++") or "c++", "-std=c++17", "-O2", "-Wall", "-fPIC", "-shared", "-fvisibility=hidden",
         f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
         "-I", str(REPO_ROOT / "include"),
+        "-I", str(CSRC),
         "-isystem", str(torch_dir / "include"),
         "-isystem", str(torch_dir / "include" / "torch" / "csrc" / "api" / "include"),
         "-isystem", str(cuda / "include"),

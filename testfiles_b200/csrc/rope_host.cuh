@@ -9,6 +9,7 @@
 #include <utility>
 
 #include "rope_device.cuh"
+#include "rope_rows.h"
 
 namespace {
 // ---------------------------------------------------------------------------

@@ -150,6 +150,16 @@ int welm_rope_multi_axis(const void* q, void* q_out, const void* k, void* k_out,
     a.dst_head[x] = s[3];
   }
   if (!aligned16(cos_sin_cache) || (num_axes > 1 && position_stride < 0)) return WELM_ROPE_ERR_BAD_STRIDE;
+  // No thread may write what another reads or writes.
+  auto rows = [&](const void* at, int x, int first) {
+    return RowSet{reinterpret_cast<uintptr_t>(at), {n_tokens, count[x], 1}, {strides[x][first], strides[x][first + 1], 0}};
+  };
+  if (rows_meet(rows(dst[0], 0, 2), rows(dst[1], 1, 2))) return WELM_ROPE_ERR_BAD_STRIDE;
+  for (int x = 0; x < 2; ++x) {
+    if (src[x] == dst[x]) continue;  // in place: its own rows
+    for (int to = 0; to < 2; ++to)
+      if (rows_meet(rows(src[x], x, 0), rows(dst[to], to, 2))) return WELM_ROPE_ERR_BAD_STRIDE;
+  }
   a.axes.positions = positions;
   a.axes.pos_stride = position_stride;
   a.axes.cache = cos_sin_cache;

@@ -28,6 +28,7 @@
 #include <stdexcept>
 #include <string>
 
+#include "rope_rows.h"
 #include "welm_rope.h"
 
 namespace {
@@ -99,6 +100,15 @@ Rows rows_of(const Tensor& t, const char* name) {
   TORCH_CHECK_VALUE(t.stride(2) == 1 && vectors(t, {r.token, r.head}), name,
                     " must have lane stride 1, other strides that are multiples of 8, and a 16-byte aligned start");
   return r;
+}
+
+// A tensor that the call writes and one that it reads or writes must not share a row.
+RowSet row_set(const Tensor& t, const Rows& r) {
+  return {reinterpret_cast<uintptr_t>(t.const_data_ptr()), {r.tokens, r.heads, 1}, {r.token, r.head, 0}};
+}
+
+void check_apart(const RowSet& a, const char* a_name, const RowSet& b, const char* b_name) {
+  TORCH_CHECK_VALUE(!rows_meet(a, b), a_name, " and ", b_name, " must not overlap");
 }
 
 void check_vector(const Tensor& t, const char* name, int64_t size) {
@@ -206,6 +216,7 @@ void rotate(const Tensor& x, const Tensor& x_out, const char* x_name, const OptT
     b = rows_of(*y, "key");
     b_out = rows_of(*y_out, "key");
     TORCH_CHECK_VALUE(b.tokens == a.tokens, "query and key need the same number of tokens");
+    if (x_out.is_same(x)) check_apart(row_set(x, a), x_name, row_set(*y, b), "key");
   }
   const int64_t position_stride = check_positions(positions, turn.sections, a.tokens, index);
   const int64_t max_position = check_cos_sin(cos_sin, index);

@@ -69,8 +69,8 @@ def rope_multi_axis_inplace(
     the axes that still have some left.  Pair i of axis a is rotated by columns
     i and 32 + i of ``cos_sin_cache[positions[a, t]]``; ``inverse=True`` turns
     the other way.  A token with a position outside the cache is left as it is
-    and flagged.  For tensors that require gradients use
-    :func:`rope_multi_axis`.
+    and flagged.  q and k must not overlap.  For tensors that require gradients
+    use :func:`rope_multi_axis`.
     """
     (_module or _binding()).multi_axis_inplace(q, k, positions, cos_sin_cache, sections, interleaved, inverse, status)
 
