@@ -384,8 +384,10 @@ int welm_rope_multi_axis(const void* q, void* q_out, const void* k, void* k_out,
  * 256]; key_cache_strides and value_cache_strides (HOST memory) give the
  * elements between blocks, between slots of a block and between heads, so a
  * [num_blocks, num_k_heads, block_size, 256] cache is the same call with its
- * strides in that order.  Pointers must be 16-byte aligned and strides
- * multiples of 8 elements.
+ * strides in that order.  q, the key cache and the value cache must not
+ * overlap, nor q and k or v; k and v may lie in the caches where no token's
+ * slot holds a row of another token's k or v.  Pointers must be 16-byte aligned
+ * and strides multiples of 8 elements (WELM_ROPE_ERR_BAD_STRIDE otherwise).
  */
 int welm_rope_kv_append(void* q, const void* k, const void* v, const int64_t* positions,
                         const float* cos_sin_cache, const int32_t* sections, int64_t num_axes,

@@ -149,6 +149,20 @@ int welm_rope_kv_append(void* q, const void* k, const void* v, const int64_t* po
   for (const void* p : {static_cast<const void*>(q), k, v, static_cast<const void*>(cos_sin_cache),
                         static_cast<const void*>(key_cache), static_cast<const void*>(value_cache)})
     if (!aligned16(p)) return WELM_ROPE_ERR_BAD_STRIDE;
+  // No thread may write what another reads or writes.  K and V may lie in the
+  // caches: which of those rows are written depends on the slots.
+  auto rows = [&](const void* at, int64_t heads, int64_t token, int64_t head) {
+    return RowSet{reinterpret_cast<uintptr_t>(at), {n_tokens, heads, 1}, {token, head, 0}};
+  };
+  auto pages = [&](const void* at, const int64_t* s) {
+    return RowSet{reinterpret_cast<uintptr_t>(at), {num_blocks, block_size, num_k_heads}, {s[0], s[1], s[2]}};
+  };
+  const RowSet q_rows = rows(q, num_q_heads, q_token_stride, q_head_stride);
+  const RowSet keys = pages(key_cache, key_cache_strides), values = pages(value_cache, value_cache_strides);
+  if (rows_meet(q_rows, rows(k, num_k_heads, k_token_stride, k_head_stride)) ||
+      rows_meet(q_rows, rows(v, num_k_heads, v_token_stride, v_head_stride)) || rows_meet(q_rows, keys) ||
+      rows_meet(q_rows, values) || rows_meet(keys, values))
+    return WELM_ROPE_ERR_BAD_STRIDE;
   a.q = static_cast<uint16_t*>(q);
   a.k = static_cast<const uint16_t*>(k);
   a.v = static_cast<const uint16_t*>(v);

@@ -172,6 +172,11 @@ std::array<int64_t, 3> check_cache(const Tensor& cache, const char* name, c10::D
   return s;
 }
 
+RowSet page_set(const Tensor& cache, const std::array<int64_t, 3>& s) {
+  return {reinterpret_cast<uintptr_t>(cache.const_data_ptr()), {cache.size(0), cache.size(1), cache.size(2)},
+          {s[0], s[1], s[2]}};
+}
+
 int32_t* status_of(const OptTensor& status, c10::DeviceIndex index) {
   if (!status) return nullptr;
   check(*status, "status", at::kInt, index);
@@ -429,6 +434,15 @@ PyObject* kv_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const auto value_strides = check_cache(value_cache, "value_cache", index);
   TORCH_CHECK_VALUE(value_cache.sizes() == key_cache.sizes() && key_cache.size(2) == kr.heads,
                     "key_cache and value_cache need the same shape, with the heads of key and v");
+  const RowSet keys = page_set(key_cache, key_strides), values = page_set(value_cache, value_strides);
+  if (q) {
+    const RowSet q_rows = row_set(*q, qr);
+    check_apart(q_rows, "query", row_set(k, kr), "key");
+    check_apart(q_rows, "query", row_set(v, vr), "v");
+    check_apart(q_rows, "query", keys, "key_cache");
+    check_apart(q_rows, "query", values, "value_cache");
+  }
+  check_apart(keys, "key_cache", values, "value_cache");
   int32_t* const device_status = status_of(status, index);
   const c10::cuda::CUDAGuard guard(index);
   done("welm_rope_kv_append",

@@ -125,7 +125,9 @@ def rope_kv_append(
     ``[axes, tokens]`` with ``sections`` (see :func:`rope_multi_axis_inplace`).
     A negative slot marks a padding token, which is left alone, its q row too;
     so is a token whose slot or position is out of range, and it is flagged.
-    The slots of one call must differ.
+    The slots of one call must differ.  q and the two caches must not overlap,
+    nor q and k or v; k and v may lie in the caches where no token's slot holds
+    a row of another token's k or v.
     """
     (_module or _binding()).kv_append(q, k, v, positions, cos_sin_cache, slot_mapping, key_cache, value_cache, sections,
                                       interleaved, status)

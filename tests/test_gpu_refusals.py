@@ -27,3 +27,27 @@ def test_q_and_k_that_overlap():
     q_out, _ = welm.rope_multi_axis(**axes_args(q=whole, k=whole))  # copies may come from the same rows
     assert q_out.shape == whole.shape
     welm.rope_multi_axis_inplace(**axes_args(q=whole[:, :6], k=whole[:, 6:7]))
+
+
+def test_append_with_tensors_that_overlap():
+    def append(**change):
+        args = {**tensors(), **change}
+        welm.rope_kv_append(**args)
+        return args
+
+    t = tensors()
+    whole = torch.zeros((4, 8, 256), dtype=torch.bfloat16, device=DEV)
+    pages = torch.zeros((2, 2, 16, 1, 256), dtype=torch.bfloat16, device=DEV)
+    flat = pages.view(-1, 1, 256)
+    for bad in (dict(value_cache=t["key_cache"], key_cache=t["key_cache"]), dict(q=whole, k=whole[:, 7:]),
+                dict(q=whole, v=whole[:, :1]), dict(q=flat[:4], key_cache=pages[:, 0], value_cache=pages[:, 1]),
+                dict(q=flat[16:20], key_cache=pages[:, 0], value_cache=pages[:, 1])):
+        with pytest.raises(ValueError, match="overlap"):
+            append(**bad)
+    # interleaved caches, views of one projection, and keys that are rotated where they lie
+    append(q=whole[:, :6], k=whole[:, 6:7], v=whole[:, 7:], key_cache=pages[:, 0], value_cache=pages[:, 1])
+    keys = torch.randn((32, 1, 256), device=DEV).to(torch.bfloat16)
+    cos_sin = torch.randn((8, 64), device=DEV)
+    want = append(k=keys[:4].clone(), cos_sin_cache=cos_sin)["key_cache"].view(32, 1, 256)[:4]
+    append(q=None, k=keys[:4], key_cache=keys.view(2, 16, 1, 256), cos_sin_cache=cos_sin)
+    assert torch.equal(keys[:4], want)

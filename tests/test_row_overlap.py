@@ -11,7 +11,7 @@ import subprocess
 import pytest
 
 from testfiles_b200 import _native, build
-from test_paged_refusals import AXES, FAKE, multi_axis
+from test_paged_refusals import AXES, FAKE, append, i64, multi_axis
 
 SOURCE = r"""
 #include "rope_rows.h"
@@ -98,3 +98,14 @@ def test_multi_axis_refuses_q_and_k_that_share_rows():
     assert multi_axis(k=other, qo=other, ko=far) == _native.ERR_BAD_STRIDE
     assert multi_axis(k=other, qo=far, ko=FAKE) == _native.ERR_BAD_STRIDE
     assert set(AXES) >= {"q", "qo", "k", "ko"}
+
+
+def test_append_refuses_what_it_writes_to_overlap():
+    """Q, keys and values are written: none may share a row with another, nor Q with what is read."""
+    qkv = dict(q=FAKE, k=FAKE + 2 * 1536, v=FAKE + 2 * 1792)
+    far, page = 1 << 30, 2 * 4096
+    for bad in (dict(q=None, hq=0, kc=far, vc=far),  # one cache for both
+                dict(qkv, kc=far, vc=far + 3 * page), dict(qkv, kc=FAKE, vc=far), dict(qkv, kc=far, vc=FAKE + 2 * 2048),
+                dict(qkv, k=FAKE + 2 * 1280, kc=far, vc=2 * far), dict(qkv, v=FAKE, kc=far, vc=2 * far),
+                dict(qkv, kc=far, vc=far + 2 * 256, ks=i64(8192, 512, 256), vs=i64(8192, 256, 256))):
+        assert append(**bad) == _native.ERR_BAD_STRIDE, bad
