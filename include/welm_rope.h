@@ -430,7 +430,8 @@ int welm_rope_kv_append(void* q, const void* k, const void* v, const int64_t* po
  * timing.  scale must be positive and finite (WELM_ROPE_ERR_BAD_MODE).
  * block_size must be a multiple of 8.  The caches' strides as for
  * welm_rope_kv_append; q may repeat rows (stride 0), out may not, and out must
- * not overlap q.  Pointers must be 16-byte aligned, strides multiples of 8.
+ * not overlap q or a cache.  Pointers must be 16-byte aligned, strides multiples
+ * of 8 (WELM_ROPE_ERR_BAD_STRIDE otherwise).
  *
  * The call allocates nothing: `workspace` is device memory of at least the
  * bytes that welm_rope_attend_workspace gives for the same sizes on the current

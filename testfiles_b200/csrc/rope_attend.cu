@@ -1553,6 +1553,13 @@ int welm_rope_attend(const void* q, void* out, float* lse, const void* key_cache
   for (const void* p : {q, static_cast<const void*>(out), key_cache, value_cache})
     if (!aligned16(p)) return WELM_ROPE_ERR_BAD_STRIDE;
   if (reinterpret_cast<uintptr_t>(workspace) & 31u) return WELM_ROPE_ERR_BAD_STRIDE;
+  // Rows of out are written while others are still computed from q and the caches.
+  const RowSet out_rows{reinterpret_cast<uintptr_t>(out), {n_tokens, num_q_heads, 1}, {out_token_stride, out_head_stride, 0}};
+  if (rows_meet(out_rows, {reinterpret_cast<uintptr_t>(q), {n_tokens, num_q_heads, 1}, {q_token_stride, q_head_stride, 0}}))
+    return WELM_ROPE_ERR_BAD_STRIDE;
+  for (const auto& [cache, s] : {std::pair(key_cache, key_cache_strides), std::pair(value_cache, value_cache_strides)})
+    if (rows_meet(out_rows, {reinterpret_cast<uintptr_t>(cache), {num_blocks, block_size, num_k_heads}, {s[0], s[1], s[2]}}))
+      return WELM_ROPE_ERR_BAD_STRIDE;
   const int sms = current_sm_count();
   if (sms <= 0) {
     cudaGetLastError();

@@ -534,6 +534,12 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
     out = at::empty(q.sizes(), q.options());
   }
   const Rows outr = rows_of(*out, "out");
+  if (!fill) {
+    const RowSet out_rows = row_set(*out, outr);
+    check_apart(out_rows, "out", row_set(q, qr), "query");
+    check_apart(out_rows, "out", page_set(key_cache, key_strides), "key_cache");
+    check_apart(out_rows, "out", page_set(value_cache, value_strides), "value_cache");
+  }
   Tensor lse;
   if (return_lse) lse = at::empty({qr.tokens, qr.heads}, q.options().dtype(at::kFloat));
   int32_t* const device_status = status_of(status, index);

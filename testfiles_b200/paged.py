@@ -175,7 +175,7 @@ def attend_shared_prefix(
     Returns ``out``, and with ``return_lse`` also the logarithm of each row's
     sum of exponentials (float32 ``[tokens, q_heads]``).  A row that sees no key
     is zeros, its logarithm minus infinity; so are rows of no request, but that
-    a given ``out``, which must not overlap q, keeps them as they were.
+    a given ``out``, which must not overlap q or a cache, keeps them as they were.
 
     ``workspace``: device memory of :func:`attend_workspace_bytes`, 32-byte
     aligned, for one call at a time; by default the call takes it from torch's

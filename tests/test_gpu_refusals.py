@@ -51,3 +51,23 @@ def test_append_with_tensors_that_overlap():
     want = append(k=keys[:4].clone(), cos_sin_cache=cos_sin)["key_cache"].view(32, 1, 256)[:4]
     append(q=None, k=keys[:4], key_cache=keys.view(2, 16, 1, 256), cos_sin_cache=cos_sin)
     assert torch.equal(keys[:4], want)
+
+
+def attend_args(**change):
+    t = tensors()
+    args = dict(q=t["q"], key_cache=t["key_cache"], value_cache=t["value_cache"],
+                block_table=torch.zeros((4, 1), dtype=torch.int32, device=DEV),
+                seq_lens=torch.ones(4, dtype=torch.int64, device=DEV))
+    return {**args, **change}
+
+
+def test_an_out_that_overlaps_what_attention_reads():
+    q = torch.zeros((4, 12, 256), dtype=torch.bfloat16, device=DEV)
+    pages = torch.zeros((2, 16, 1, 256), dtype=torch.bfloat16, device=DEV)
+    for bad in (dict(q=q[:, :6], out=q[:, :6]), dict(q=q[:, :6], out=q[:, 5:11]),
+                dict(key_cache=pages, out=pages.view(-1)[:6144].view(4, 6, 256)),
+                dict(value_cache=pages, out=pages.view(-1)[:6144].view(4, 6, 256))):
+        with pytest.raises(ValueError, match="overlap"):
+            welm.attend_shared_prefix(**attend_args(**bad))
+    args = attend_args(q=q[:, :6], out=q[:, 6:])
+    assert welm.attend_shared_prefix(**args) is args["out"]  # heads of one tensor, apart

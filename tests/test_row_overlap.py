@@ -11,7 +11,7 @@ import subprocess
 import pytest
 
 from testfiles_b200 import _native, build
-from test_paged_refusals import AXES, FAKE, append, i64, multi_axis
+from test_paged_refusals import AXES, FAKE, append, attend, i64, multi_axis
 
 SOURCE = r"""
 #include "rope_rows.h"
@@ -109,3 +109,11 @@ def test_append_refuses_what_it_writes_to_overlap():
                 dict(qkv, k=FAKE + 2 * 1280, kc=far, vc=2 * far), dict(qkv, v=FAKE, kc=far, vc=2 * far),
                 dict(qkv, kc=far, vc=far + 2 * 256, ks=i64(8192, 512, 256), vs=i64(8192, 256, 256))):
         assert append(**bad) == _native.ERR_BAD_STRIDE, bad
+
+
+def test_attend_refuses_an_out_that_overlaps_what_it_reads():
+    far, page = 1 << 30, 2 * 4096
+    for bad in (dict(kc=far, vc=far), dict(q=FAKE + 2 * 256, kc=far, vc=far), dict(out=far, vc=2 * far),
+                dict(out=far, kc=2 * far), dict(out=far + 3 * page, kc=far, vc=2 * far),
+                dict(q=2 * far, out=far - 2 * 5376, kc=3 * far, vc=far)):  # its last rows in the first page
+        assert attend(**{**dict(kc=far, vc=far), **bad}) == _native.ERR_BAD_STRIDE, bad
