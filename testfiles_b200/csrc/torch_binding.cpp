@@ -184,8 +184,14 @@ int32_t* status_of(const OptTensor& status, c10::DeviceIndex index) {
   return static_cast<int32_t*>(status->data_ptr());
 }
 
-// Refuses a tensor whose gradient the call would lose.
+// Refuses a tensor whose tangent the call would lose or leave behind.
+void no_tangent(const char* entry, const Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!(t.defined() && t._fw_grad(0).defined()), entry, " has no forward-mode derivative");
+}
+
+// Refuses a tensor whose gradient or tangent the call would lose.
 void no_grad(const char* entry, const Tensor& t) {
+  no_tangent(entry, t);
   TORCH_CHECK_VALUE(!(t.defined() && t.requires_grad() && at::GradMode::is_enabled()), entry,
                     " has no backward pass: call it under torch.no_grad() or on detached tensors");
 }
@@ -294,8 +300,8 @@ struct MultiAxisBackward : torch::autograd::Node {
 // Rotated copies of x and y, with their history where gradients are wanted.
 variable_list differentiable(const Tensor& x, const char* x_name, const OptTensor& y, const Tensor& positions,
                              const Tensor& cos_sin, const Turn& turn, const OptTensor& status) {
-  TORCH_CHECK_NOT_IMPLEMENTED(!x._fw_grad(0).defined() && !(y && y->_fw_grad(0).defined()),
-                              "rope_multi_axis has no forward-mode derivative");
+  no_tangent("rope_multi_axis", x);
+  if (y) no_tangent("rope_multi_axis", *y);
   std::shared_ptr<MultiAxisBackward> node;
   if (at::GradMode::is_enabled() && (x.requires_grad() || (y && y->requires_grad()))) {
     node = std::shared_ptr<MultiAxisBackward>(new MultiAxisBackward(), torch::autograd::deleteNode);

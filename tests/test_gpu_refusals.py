@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import testfiles_b200 as welm
 from test_paged_refusals import DEV, tensors
@@ -71,3 +72,21 @@ def test_an_out_that_overlaps_what_attention_reads():
             welm.attend_shared_prefix(**attend_args(**bad))
     args = attend_args(q=q[:, :6], out=q[:, 6:])
     assert welm.attend_shared_prefix(**args) is args["out"]  # heads of one tensor, apart
+
+
+@pytest.mark.parametrize("entry,args,names", [
+    (welm.rope_multi_axis_inplace, axes_args, ("q", "k")),
+    (welm.rope_kv_append, lambda **c: {**tensors(), **c}, ("q", "k", "v", "key_cache", "value_cache")),
+    (welm.attend_shared_prefix, attend_args, ("q", "key_cache", "value_cache", "out")),
+])
+def test_forward_mode_tensors(entry, args, names):
+    """Their tangents would be lost, or stay as they were beside a tensor that has changed."""
+    for name in names:
+        given = args()
+        plain = given.get(name, torch.zeros((4, 6, 256), dtype=torch.bfloat16, device=DEV))
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(plain, torch.ones_like(plain))
+            for ctx in (torch.enable_grad, torch.no_grad):
+                with ctx(), pytest.raises(NotImplementedError, match="forward-mode"):
+                    entry(**args(**{name: dual}))
+        assert (plain == 0).all()
