@@ -384,7 +384,9 @@ PyObject* multi_axis_inplace(PyObject*, PyObject* const* args, Py_ssize_t n) {
   device_index(q);
   no_grad("rope_multi_axis_inplace", q);
   no_grad("rope_multi_axis_inplace", k);
-  rotate(q, q, "query", k, k, tensor_arg(args[2], "positions"), tensor_arg(args[3], "cos_sin_cache"),
+  const Tensor cos_sin = tensor_arg(args[3], "cos_sin_cache");
+  no_grad("rope_multi_axis_inplace", cos_sin);
+  rotate(q, q, "query", k, k, tensor_arg(args[2], "positions"), cos_sin,
          {sections_of(ints_arg(args[4])), bool_arg(args[5]), bool_arg(args[6])}, opt_tensor_arg(args[7], "status"));
   written(q);
   written(k);
@@ -397,8 +399,10 @@ PyObject* multi_axis(PyObject*, PyObject* const* args, Py_ssize_t n) {
   arity(n, 8);
   const Tensor q = query_arg(args[0]), k = tensor_arg(args[1], "key");
   device_index(q);
+  const Tensor cos_sin = tensor_arg(args[3], "cos_sin_cache");
+  no_grad("the cos_sin_cache of rope_multi_axis", cos_sin);
   const variable_list out =
-      differentiable(q, "query", k, tensor_arg(args[2], "positions"), tensor_arg(args[3], "cos_sin_cache"),
+      differentiable(q, "query", k, tensor_arg(args[2], "positions"), cos_sin,
                      {sections_of(ints_arg(args[4])), bool_arg(args[5]), bool_arg(args[6])},
                      opt_tensor_arg(args[7], "status"));
   return PyTuple_Pack(2, THPObjectPtr(THPVariable_Wrap(out[0])).get(), THPObjectPtr(THPVariable_Wrap(out[1])).get());
@@ -420,6 +424,7 @@ PyObject* kv_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
   if (q) no_grad("rope_kv_append", *q);
   no_grad("rope_kv_append", k);
   no_grad("rope_kv_append", v);
+  no_grad("rope_kv_append", cos_sin);
   no_grad("rope_kv_append", key_cache);
   no_grad("rope_kv_append", value_cache);
   check(k, "key", at::kBFloat16, index);

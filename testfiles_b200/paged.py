@@ -85,7 +85,8 @@ def rope_multi_axis(
     inverse: bool = False,
     status: Optional[torch.Tensor] = None,
 ) -> tuple[torch.Tensor, torch.Tensor]:
-    """Rotated copies of Q and K, differentiable in both (any number of times).
+    """Rotated copies of Q and K, differentiable in both (any number of times)
+    and in nothing else: a cos_sin_cache that requires a gradient is refused.
 
     Arguments as for :func:`rope_multi_axis_inplace`; q and k keep their values
     and may have any strides, the results are contiguous.  A token with a

@@ -90,3 +90,18 @@ def test_forward_mode_tensors(entry, args, names):
                 with ctx(), pytest.raises(NotImplementedError, match="forward-mode"):
                     entry(**args(**{name: dual}))
         assert (plain == 0).all()
+
+
+@pytest.mark.parametrize("entry,args", [
+    (welm.rope_multi_axis_inplace, axes_args), (welm.rope_multi_axis, axes_args),
+    (welm.rope_kv_append, lambda **c: {**tensors(), **c}),
+])
+def test_a_cos_sin_cache_whose_gradient_would_be_lost(entry, args):
+    table = torch.zeros((8, 64), device=DEV, requires_grad=True)
+    with pytest.raises(ValueError, match="no backward pass"):
+        entry(**args(cos_sin_cache=table))
+    with torch.no_grad():
+        entry(**args(cos_sin_cache=table))
+    entry(**args(cos_sin_cache=table.detach()))
+    with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
+        entry(**args(cos_sin_cache=forward_ad.make_dual(table.detach(), torch.ones((8, 64), device=DEV))))
