@@ -427,7 +427,8 @@ int welm_rope_kv_append(void* q, const void* k, const void* v, const int64_t* po
  *
  * Products take BF16 operands (p rounded to BF16) with FP32 sums; maxima, sums
  * and partial results are FP32; out is rounded once.  Results do not depend on
- * timing.  scale must be positive and finite (WELM_ROPE_ERR_BAD_MODE).
+ * timing.  scale must be positive, and log2(e) times as much finite in FP32
+ * (WELM_ROPE_ERR_BAD_MODE).
  * block_size must be a multiple of 8.  The caches' strides as for
  * welm_rope_kv_append; q may repeat rows (stride 0), out may not, and out must
  * not overlap q or a cache.  Pointers must be 16-byte aligned, strides multiples

@@ -34,6 +34,8 @@
 // to BF16 because the product with the BF16 values takes both operands in one
 // type; l sums the unrounded p, and S, m, l and O are FP32.
 
+#include <cmath>
+
 #include "rope_tma.cuh"
 
 namespace {
@@ -68,6 +70,7 @@ constexpr uint32_t kColO = 256;
 __host__ __device__ constexpr uint32_t col_s(uint32_t third) { return third == 0 ? 0 : third == 1 ? 128 : 64; }
 __host__ __device__ constexpr uint32_t col_p(uint32_t third) { return third == 0 ? 0 : third == 1 ? 192 : 128; }
 constexpr long long kWaitClocks = 1ll << 32;  // about two seconds
+constexpr float kLog2E = 1.4426950408889634f;
 constexpr float kRescaleStep = 8.0f;   // O is rescaled when the maximum grows by more than 2^8
 
 // Division by a number that the host knows: x / d for 0 <= x < 2^31 as one
@@ -1531,7 +1534,8 @@ int welm_rope_attend(const void* q, void* out, float* lse, const void* key_cache
        (row_tiles + batch_size) * ((table_width * block_size + kKeys - 1) / kKeys + kItemCost)) * num_k_heads >=
       INT32_MAX)
     return WELM_ROPE_ERR_BAD_SIZE;
-  if (!(scale > 0.0f) || scale > 3.0e38f || (fill_unused != 0 && fill_unused != 1)) return WELM_ROPE_ERR_BAD_MODE;
+  // in FP32, as the kernels multiply by it
+  if (!(scale > 0.0f) || !std::isfinite(scale * kLog2E) || (fill_unused != 0 && fill_unused != 1)) return WELM_ROPE_ERR_BAD_MODE;
   if (n_tokens == 0 || batch_size == 0) return WELM_ROPE_OK;
   if (block_size % 8 != 0 || num_blocks == 0) return WELM_ROPE_ERR_BAD_SIZE;
   if (!q || !out || !key_cache || !value_cache || !seq_lens || !workspace || !key_cache_strides ||
@@ -1605,7 +1609,7 @@ int welm_rope_attend(const void* q, void* out, float* lse, const void* key_cache
   a.slot_rows = int32_t(n_tokens * group < kRows ? n_tokens * group : kRows);
   a.grid = sms;
   a.fill = int32_t(fill_unused);
-  a.scale = scale * 1.4426950408889634f;
+  a.scale = scale * kLog2E;
   char* base = static_cast<char*>(workspace);
   a.note = reinterpret_cast<LineNote*>(base + w.note);
   a.units_before = reinterpret_cast<int32_t*>(base + w.units);

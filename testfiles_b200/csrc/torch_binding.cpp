@@ -535,7 +535,9 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
                           (prefix_table->size(0) <= 1 || prefix_table->stride(0) == 1),
                       "prefix_table must be a contiguous 1-D int32 tensor with a block for every prefix key");
   }
-  TORCH_CHECK_VALUE(scale > 0.0 && scale < 3.0e38, "scale must be positive and finite, got ", scale);
+  // the kernels multiply by scale log2(e) in FP32
+  TORCH_CHECK_VALUE(float(scale) > 0.0f && std::isfinite(float(scale) * 1.4426950408889634f),
+                    "scale must be positive and finite in FP32, log2(e) times as much too, got ", scale);
   const bool fill = !out;
   if (out) {
     check(*out, "out", at::kBFloat16, index);

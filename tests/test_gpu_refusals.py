@@ -105,3 +105,9 @@ def test_a_cos_sin_cache_whose_gradient_would_be_lost(entry, args):
     entry(**args(cos_sin_cache=table.detach()))
     with forward_ad.dual_level(), pytest.raises(NotImplementedError, match="forward-mode"):
         entry(**args(cos_sin_cache=forward_ad.make_dual(table.detach(), torch.ones((8, 64), device=DEV))))
+
+
+@pytest.mark.parametrize("scale", [1e-60, 2.9e38, 1e60, float("inf"), float("nan"), -1.0])
+def test_scales_that_fp32_does_not_hold(scale):
+    with pytest.raises(ValueError, match="scale"):
+        welm.attend_shared_prefix(**attend_args(scale=scale))
