@@ -1422,6 +1422,18 @@ __global__ void __launch_bounds__(kGroups == 1 ? 256 : 128 * kGroups, kResident)
   }
 }
 
+// No request: every row is one of none.  Eight lanes of a row a thread.
+__global__ void __launch_bounds__(256) rope_attend_none_kernel(const __grid_constant__ AttendArgs a) {
+  pdl_enter();
+  const int64_t item = int64_t(blockIdx.x) * blockDim.x + threadIdx.x;
+  const int row = int(item >> 5), lanes8 = int(item & 31);
+  if (row >= a.tokens * a.q_heads) return;
+  const int token = a.by_q_heads.of(row), head = row - token * a.q_heads;
+  if (a.fill)
+    *reinterpret_cast<uint4*>(a.out + token * a.out_token + head * a.out_head + lanes8 * 8) = make_uint4(0, 0, 0, 0);
+  if (a.lse != nullptr && lanes8 == 0) a.lse[row] = -INFINITY;
+}
+
 // ---------------------------------------------------------------------------
 // Host side.
 // ---------------------------------------------------------------------------
@@ -1536,7 +1548,24 @@ int welm_rope_attend(const void* q, void* out, float* lse, const void* key_cache
     return WELM_ROPE_ERR_BAD_SIZE;
   // in FP32, as the kernels multiply by it
   if (!(scale > 0.0f) || !std::isfinite(scale * kLog2E) || (fill_unused != 0 && fill_unused != 1)) return WELM_ROPE_ERR_BAD_MODE;
-  if (n_tokens == 0 || batch_size == 0) return WELM_ROPE_OK;
+  if (n_tokens == 0 || (batch_size == 0 && fill_unused == 0 && lse == nullptr)) return WELM_ROPE_OK;
+  if (batch_size == 0) {
+    if (fill_unused && !out) return WELM_ROPE_ERR_NULL_POINTER;
+    if (fill_unused && (!rows_apart<2>({n_tokens, num_q_heads}, {out_token_stride, out_head_stride}) ||
+                        ((out_token_stride | out_head_stride) & 7) || !aligned16(out)))
+      return WELM_ROPE_ERR_BAD_STRIDE;
+    AttendArgs none{};
+    none.out = static_cast<uint16_t*>(out);
+    none.lse = lse;
+    none.out_token = out_token_stride;
+    none.out_head = out_head_stride;
+    none.tokens = int32_t(n_tokens);
+    none.q_heads = int32_t(num_q_heads);
+    none.by_q_heads = Divisor(num_q_heads);
+    none.fill = int32_t(fill_unused);
+    return launch(rope_attend_none_kernel, unsigned((n_tokens * num_q_heads + 7) / 8), 256, 0,
+                  static_cast<cudaStream_t>(stream), none);
+  }
   if (block_size % 8 != 0 || num_blocks == 0) return WELM_ROPE_ERR_BAD_SIZE;
   if (!q || !out || !key_cache || !value_cache || !seq_lens || !workspace || !key_cache_strides ||
       !value_cache_strides || (table_width > 0 && !block_table) || (prefix_len > 0 && !prefix_table))
