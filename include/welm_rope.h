@@ -434,6 +434,11 @@ int welm_rope_kv_append(void* q, const void* k, const void* v, const int64_t* po
  * not overlap q or a cache.  Pointers must be 16-byte aligned, strides multiples
  * of 8 (WELM_ROPE_ERR_BAD_STRIDE otherwise).
  *
+ * The kernel waits for its own copies and products, each time for about two
+ * seconds at most.  Should a wait not end, every row of a request and its lse
+ * become NaN and WELM_ROPE_DEV_WAIT_TIMEOUT is raised (WELM_ROPE_GIVE_UP=1 in
+ * the environment, read once, makes every call end so, to test a caller).
+ *
  * The call allocates nothing: `workspace` is device memory of at least the
  * bytes that welm_rope_attend_workspace gives for the same sizes on the current
  * device, 32-byte aligned.  It needs no initial contents and keeps nothing for

@@ -108,7 +108,9 @@ struct AttendArgs {
   int32_t grid;
   int32_t fill;                 // 1: rows of no request become zeros; their lse is minus infinity either way
   float scale;                  // times log2(e)
+  int32_t give_up;              // 1: at the first wait that is not over
   struct LineNote* note;        // what the join needs of the line
+  int32_t* gave_up;             // [grid] 1: a wait of the CTA did not end
   int32_t* units_before;        // [batch] units of the own items before each request
   // Partial results.  O is laid out [32][rows][8 lanes]: the threads of a warp,
   // a row each, then write (and a row's reader reads) whole 32-byte sectors.
@@ -1186,7 +1188,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&ctl.piece_full[i], 1);
       mbar_init(&ctl.piece_empty[i], kPieceReaders);
     }
-    ctl.failed = 0;
+    ctl.failed = a.give_up;
     ctl.changed = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -1205,6 +1207,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = ctl.tmem;
   const uint32_t q_at = smem_u32(smem), k_at = smem_u32(ring), v_at = k_at + kStagesK * kStageBytes;
   if (warp < 3) pdl_enter();  // the others first look at hints
+  // stored here, so that the kernel's end does not wait for it
+  if (tid == 0) a.gave_up[blockIdx.x] = 0;
   if (warp == 0) {
     produce(a, ctl, &kmap, &vmap, k_at, v_at);
   } else if (warp == 1) {
@@ -1219,7 +1223,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   tmem_fence_before();
   __syncthreads();
-  if (tid == 0 && ctl.failed) raise_status(a.status, WELM_ROPE_DEV_WAIT_TIMEOUT);
+  if (tid == 0 && ctl.failed) {
+    a.gave_up[blockIdx.x] = 1;
+    raise_status(a.status, WELM_ROPE_DEV_WAIT_TIMEOUT);
+  }
   if (warp == 1) {
     tmem_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
@@ -1234,10 +1241,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 // may have many); with kGroups == 1 a CTA of two such groups joins 32 rows.
 // The first threads work out where the parts of the CTA's rows are, a row each.
 // ---------------------------------------------------------------------------
+// A row that this kernel writes; of no request; of a request; of one whose result is lost.
+enum RowIs { kWritten = 1, kUnused = 2, kAsked = 4, kLost = 8 };
+
 struct RowParts {
   int cta[2], count[2], in_tile[2];  // prefix and own item: first CTA, CTAs, row of the item
-  int live;                          // 1: this kernel writes the row
-  int unused;                        // 1: a row of no request
+  int is;                            // bits of the following; 0: past the last row
   int token, head;
 };
 
@@ -1284,9 +1293,9 @@ __device__ __forceinline__ RowParts find_parts(const AttendArgs& a, const LineNo
     units_before = a.units_before[b];
     q = raw.checked(a, false);
   }
-  if (note.nothing || token >= used || token < q.first || token >= q.first + q.count) {  // a row of no request
-    r.live = a.fill;
-    r.unused = 1;
+  r.is = token < used && token >= q.first && token < q.first + q.count ? kAsked : 0;
+  if (note.nothing || r.is == 0) {  // a row of no request
+    r.is |= a.fill ? kUnused | kWritten : kUnused;
     return r;
   }
   const int pre = note.pre;
@@ -1307,7 +1316,7 @@ __device__ __forceinline__ RowParts find_parts(const AttendArgs& a, const LineNo
   const int units = Request::units(q.tiles(a, rt), note.joint);
   place(1, pre + units_before + q.units_before(a, rt, note.joint) * a.k_heads + h * units,
         max(units - kItemCost, 0), packed % kRows);
-  r.live = pre > 0 || r.count[1] != 1;  // otherwise the first kernel wrote the row
+  if (pre > 0 || r.count[1] != 1) r.is |= kWritten;  // otherwise the first kernel wrote the row
   return r;
 }
 
@@ -1354,11 +1363,24 @@ __global__ void __launch_bounds__(kGroups == 1 ? 256 : 128 * kGroups, kResident)
   const int used = used_tokens(a);
   if (threadIdx.x < kRowsPerCta)
     parts[threadIdx.x] = find_parts(a, note, used, blockIdx.x * kRowsPerCta + threadIdx.x, request);
-  __syncthreads();
+  int lost = 0;  // read by the last threads, as the first are busy
+#pragma unroll 1
+  for (int c = blockDim.x - 1 - threadIdx.x; c < a.grid; c += blockDim.x) lost |= a.gave_up[c];
+  // Where a CTA of the first kernel gave up, the note and the partial results may be
+  // whatever the workspace held before, and rows may not have been written: none of
+  // it is read, and every row of a request becomes no number.
+  if (__syncthreads_or(lost)) {
+    if (threadIdx.x < kRowsPerCta) {
+      RowParts& r = parts[threadIdx.x];
+      r.count[0] = r.count[1] = 0;
+      if (r.is & kAsked) r.is |= kWritten | kLost;
+    }
+    __syncthreads();
+  }
   const int64_t all = int64_t(a.tokens) * a.q_heads;
   for (int row = (kGroups == 1 ? 4 * grp : 0) + (in_grp & 3); row < kRowsPerCta; row += 8) {
-    const RowParts r = parts[row];
-    const int count = r.live ? r.count[0] + r.count[1] : 0;
+    const RowParts& r = parts[row];
+    const int count = r.is & kWritten ? r.count[0] + r.count[1] : 0;
     const int h = a.by_group.of(r.head);
     // the row among the whole items' rows
     const int64_t packed = int64_t(h) * a.tokens * a.group + int64_t(r.token) * a.group + (r.head - h * a.group);
@@ -1408,11 +1430,12 @@ __global__ void __launch_bounds__(kGroups == 1 ? 256 : 128 * kGroups, kResident)
         sum.add(s_o[w][8][in_grp], s_o[w][9][in_grp], v);
       }
     }
+    if (r.is & kLost) sum.l = __int_as_float(0x7fc00000);
     const bool none = sum.l == 0.0f;
-    if ((r.live || r.unused) && a.lse != nullptr && lanes8 == 0)
+    if ((r.is & (kWritten | kUnused)) && a.lse != nullptr && lanes8 == 0)
       a.lse[int64_t(r.token) * a.q_heads + r.head] =
           none ? -INFINITY : (sum.m + log2f(sum.l)) * 0.6931471805599453f;
-    if (!r.live) continue;
+    if (!(r.is & kWritten)) continue;
     const float inv = none ? 0.0f : 1.0f / sum.l;
     uint4 packed_out = make_uint4(0, 0, 0, 0);
     if (!none)
@@ -1439,7 +1462,7 @@ __global__ void __launch_bounds__(256) rope_attend_none_kernel(const __grid_cons
 // ---------------------------------------------------------------------------
 // Layout of the workspace, in bytes from its base.
 struct Workspace {
-  int64_t note, units, slot_ml, slot_o, part_ml, part_o, bytes;
+  int64_t note, gave_up, units, slot_ml, slot_o, part_ml, part_o, bytes;
 };
 
 Workspace attend_workspace(int64_t tokens, int64_t batch, int64_t q_heads, int64_t group, int64_t prefix_len,
@@ -1450,7 +1473,8 @@ Workspace attend_workspace(int64_t tokens, int64_t batch, int64_t q_heads, int64
   const int64_t parts = prefix_len > 0 ? 2 * tokens * q_heads : 0;
   Workspace w;
   w.note = 0;
-  w.units = 256;
+  w.gave_up = 256;
+  w.units = w.gave_up + up(grid * 4);
   static_assert(sizeof(LineNote) <= 256, "line note");
   w.slot_ml = w.units + up(batch * 4);
   w.slot_o = w.slot_ml + up(slots * 8);
@@ -1487,6 +1511,16 @@ bool attend_sizes_ok(int64_t tokens, int64_t batch, int64_t q_heads, int64_t k_h
   if (tokens < 0 || batch < 0 || q_heads < 1 || k_heads < 1 || prefix_len < 0) return false;
   if (q_heads % k_heads != 0 || batch > kMaxItems || prefix_len > kMaxItems) return false;
   return q_heads <= kMaxItems && tokens <= kMaxItems / q_heads;
+}
+
+// WELM_ROPE_GIVE_UP=1 in the environment makes every call behave as one of whose
+// waits has not ended, for tests of what becomes of it.
+bool give_up() {
+  static const bool at_once = [] {
+    const char* v = std::getenv("WELM_ROPE_GIVE_UP");
+    return v != nullptr && v[0] == '1';
+  }();
+  return at_once;
 }
 
 int launch_attend(const CUtensorMap& kmap, const CUtensorMap& vmap, const AttendArgs& a, cudaStream_t stream) {
@@ -1641,6 +1675,8 @@ int welm_rope_attend(const void* q, void* out, float* lse, const void* key_cache
   a.scale = scale * kLog2E;
   char* base = static_cast<char*>(workspace);
   a.note = reinterpret_cast<LineNote*>(base + w.note);
+  a.gave_up = reinterpret_cast<int32_t*>(base + w.gave_up);
+  a.give_up = give_up();
   a.units_before = reinterpret_cast<int32_t*>(base + w.units);
   a.slot_ml = reinterpret_cast<float*>(base + w.slot_ml);
   a.slot_o = reinterpret_cast<float*>(base + w.slot_o);

@@ -184,6 +184,12 @@ def attend_shared_prefix(
     call follows them; ``prefix_len`` is part of the capture.  What a page holds
     behind the last key does not matter; a key that some rows of a request do
     not see yet must be finite.  There is no backward pass.
+
+    The kernel waits for its own copies and products, each time for about two
+    seconds at most.  Should a wait not end, every row of a request, and its
+    logarithm, becomes NaN, and ``status`` receives
+    ``WELM_ROPE_DEV_WAIT_TIMEOUT`` (``WELM_ROPE_GIVE_UP=1`` in the environment
+    makes every call end so, to test a program's answer to it).
     """
     return (_module or _binding()).attend(q, key_cache, value_cache, block_table, seq_lens, query_starts, prefix_table,
                                           prefix_len, scale, out, return_lse, workspace, status)
