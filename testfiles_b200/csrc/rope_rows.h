@@ -17,15 +17,22 @@ struct RowSet {
   int64_t extent[3], stride[3];
 };
 
+// Elements from the first lane to behind the last; 0 where there are no rows.
+inline __int128 rows_span(const RowSet& r) {
+  __int128 span = WELM_ROPE_HEAD_DIM;
+  for (int i = 0; i < 3; ++i) {
+    if (r.extent[i] <= 0) return 0;
+    span += __int128(r.stride[i]) * (r.extent[i] - 1);
+  }
+  return span;
+}
+
 // The dimensions of a RowSet that step, the largest stride first.
 struct RowDims {
   int n = 0;
   int64_t extent[3], stride[3];
-  __int128 span = WELM_ROPE_HEAD_DIM;  // elements from the first lane to behind the last
-  bool none = false;                   // no rows
   explicit RowDims(const RowSet& r) {
     for (int i = 0; i < 3; ++i) {
-      if (r.extent[i] <= 0) none = true;
       if (r.extent[i] <= 1 || r.stride[i] == 0) continue;
       int at = n++;
       for (; at > 0 && stride[at - 1] < r.stride[i]; --at) {
@@ -34,7 +41,6 @@ struct RowDims {
       }
       stride[at] = r.stride[i];
       extent[at] = r.extent[i];
-      span += __int128(r.stride[i]) * (r.extent[i] - 1);
     }
   }
 };
@@ -43,15 +49,15 @@ struct RowDims {
 // dimensions below do, displaced by d + (j - i) T; only displacements within
 // their spans have to be looked at, one or two where rows of equal steps
 // interleave.  Exact, unless that takes more than `steps` of them: then true.
-inline bool rows_meet_at(const RowDims& a, int ai, __int128 span_a, const RowDims& b, int bi, __int128 span_b,
-                         __int128 d, int& steps) {
+template <typename Int>
+bool rows_meet_at(const RowDims& a, int ai, Int span_a, const RowDims& b, int bi, Int span_b, Int d, int& steps) {
   if (d >= span_a || -d >= span_b) return false;
   if (ai == a.n && bi == b.n) return true;
   const int64_t sa = ai < a.n ? a.stride[ai] : 0, sb = bi < b.n ? b.stride[bi] : 0;
-  const __int128 step = sa > sb ? sa : sb;
-  __int128 lo = 0, hi = 0;
+  const Int step = sa > sb ? sa : sb;
+  Int lo = 0, hi = 0;
   if (sa == step) {
-    lo = -__int128(a.extent[ai] - 1);
+    lo = -Int(a.extent[ai] - 1);
     span_a += lo * step;
     ++ai;
   }
@@ -60,22 +66,25 @@ inline bool rows_meet_at(const RowDims& a, int ai, __int128 span_a, const RowDim
     span_b -= hi * step;
     ++bi;
   }
-  auto floor_div = [](__int128 x, __int128 y) { return x / y - (x % y < 0); };
-  const __int128 first = -floor_div(span_b - 1 + d, step), last = floor_div(span_a - 1 - d, step);
+  auto floor_div = [](Int x, Int y) { return x / y - (x % y < 0); };
+  const Int first = -floor_div(span_b - 1 + d, step), last = floor_div(span_a - 1 - d, step);
   if (lo < first) lo = first;
   if (hi > last) hi = last;
-  for (__int128 m = lo; m <= hi; ++m) {
+  for (Int m = lo; m <= hi; ++m) {
     if (--steps < 0 || rows_meet_at(a, ai, span_a, b, bi, span_b, d + m * step, steps)) return true;
   }
   return false;
 }
 
 inline bool rows_meet(const RowSet& x, const RowSet& y) {
+  const __int128 span_x = rows_span(x), span_y = rows_span(y);
+  const __int128 d = (__int128(y.at) - __int128(x.at)) / 2;  // rows begin at even addresses
+  if (d >= span_x || -d >= span_y || span_x == 0 || span_y == 0) return false;
   const RowDims a(x), b(y);
-  if (a.none || b.none) return false;
-  const __int128 bytes = __int128(y.at) - __int128(x.at);
   int steps = 4096;
-  return rows_meet_at(a, 0, a.span, b, 0, b.span, bytes / 2, steps);
+  // the usual case in 64 bits, whose divisions are ten times as fast
+  if (((span_x | span_y) >> 61) == 0) return rows_meet_at<int64_t>(a, 0, span_x, b, 0, span_y, d, steps);
+  return rows_meet_at<__int128>(a, 0, span_x, b, 0, span_y, d, steps);
 }
 
 }  // namespace

@@ -102,7 +102,8 @@ Rows rows_of(const Tensor& t, const char* name) {
   return r;
 }
 
-// A tensor that the call writes and one that it reads or writes must not share a row.
+// A tensor that the call writes and one that it reads or writes must not share a
+// row.  The library refuses that; only then is it looked up here which they are.
 RowSet row_set(const Tensor& t, const Rows& r) {
   return {reinterpret_cast<uintptr_t>(t.const_data_ptr()), {r.tokens, r.heads, 1}, {r.token, r.head, 0}};
 }
@@ -227,19 +228,20 @@ void rotate(const Tensor& x, const Tensor& x_out, const char* x_name, const OptT
     b = rows_of(*y, "key");
     b_out = rows_of(*y_out, "key");
     TORCH_CHECK_VALUE(b.tokens == a.tokens, "query and key need the same number of tokens");
-    if (x_out.is_same(x)) check_apart(row_set(x, a), x_name, row_set(*y, b), "key");
   }
   const int64_t position_stride = check_positions(positions, turn.sections, a.tokens, index);
   const int64_t max_position = check_cos_sin(cos_sin, index);
   int32_t* const device_status = status_of(status, index);
   const c10::cuda::CUDAGuard guard(index);
-  done("welm_rope_multi_axis",
-       welm_rope_multi_axis(x.const_data_ptr(), x_out.data_ptr(), y ? y->const_data_ptr() : nullptr,
-                            y ? y_out->data_ptr() : nullptr, positions.const_data_ptr<int64_t>(),
-                            cos_sin.const_data_ptr<float>(), turn.sections.pairs, turn.sections.axes, turn.interleaved,
-                            turn.inverse, a.tokens, a.heads, b.heads, a.token, a.head, a_out.token, a_out.head, b.token,
-                            b.head, b_out.token, b_out.head, position_stride, max_position, device_status,
-                            stream_of(index)));
+  const int result =
+      welm_rope_multi_axis(x.const_data_ptr(), x_out.data_ptr(), y ? y->const_data_ptr() : nullptr,
+                           y ? y_out->data_ptr() : nullptr, positions.const_data_ptr<int64_t>(),
+                           cos_sin.const_data_ptr<float>(), turn.sections.pairs, turn.sections.axes, turn.interleaved,
+                           turn.inverse, a.tokens, a.heads, b.heads, a.token, a.head, a_out.token, a_out.head, b.token,
+                           b.head, b_out.token, b_out.head, position_stride, max_position, device_status,
+                           stream_of(index));
+  if (result == WELM_ROPE_ERR_BAD_STRIDE && y) check_apart(row_set(x_out, a_out), x_name, row_set(*y_out, b_out), "key");
+  done("welm_rope_multi_axis", result);
 }
 
 // x in a layout that the kernel reads.
@@ -445,24 +447,27 @@ PyObject* kv_append(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const auto value_strides = check_cache(value_cache, "value_cache", index);
   TORCH_CHECK_VALUE(value_cache.sizes() == key_cache.sizes() && key_cache.size(2) == kr.heads,
                     "key_cache and value_cache need the same shape, with the heads of key and v");
-  const RowSet keys = page_set(key_cache, key_strides), values = page_set(value_cache, value_strides);
-  if (q) {
-    const RowSet q_rows = row_set(*q, qr);
-    check_apart(q_rows, "query", row_set(k, kr), "key");
-    check_apart(q_rows, "query", row_set(v, vr), "v");
-    check_apart(q_rows, "query", keys, "key_cache");
-    check_apart(q_rows, "query", values, "value_cache");
-  }
-  check_apart(keys, "key_cache", values, "value_cache");
   int32_t* const device_status = status_of(status, index);
   const c10::cuda::CUDAGuard guard(index);
-  done("welm_rope_kv_append",
-       welm_rope_kv_append(q ? q->data_ptr() : nullptr, k.const_data_ptr(), v.const_data_ptr(),
-                           positions.const_data_ptr<int64_t>(), cos_sin.const_data_ptr<float>(), sections.pairs,
-                           sections.axes, interleaved, slots.const_data_ptr<int64_t>(), key_cache.data_ptr(),
-                           value_cache.data_ptr(), kr.tokens, qr.heads, kr.heads, qr.token, qr.head, kr.token, kr.head,
-                           vr.token, vr.head, key_cache.size(0), key_cache.size(1), key_strides.data(),
-                           value_strides.data(), position_stride, max_position, device_status, stream_of(index)));
+  const int result =
+      welm_rope_kv_append(q ? q->data_ptr() : nullptr, k.const_data_ptr(), v.const_data_ptr(),
+                          positions.const_data_ptr<int64_t>(), cos_sin.const_data_ptr<float>(), sections.pairs,
+                          sections.axes, interleaved, slots.const_data_ptr<int64_t>(), key_cache.data_ptr(),
+                          value_cache.data_ptr(), kr.tokens, qr.heads, kr.heads, qr.token, qr.head, kr.token, kr.head,
+                          vr.token, vr.head, key_cache.size(0), key_cache.size(1), key_strides.data(),
+                          value_strides.data(), position_stride, max_position, device_status, stream_of(index));
+  if (result == WELM_ROPE_ERR_BAD_STRIDE) {
+    const RowSet keys = page_set(key_cache, key_strides), values = page_set(value_cache, value_strides);
+    if (q) {
+      const RowSet q_rows = row_set(*q, qr);
+      check_apart(q_rows, "query", row_set(k, kr), "key");
+      check_apart(q_rows, "query", row_set(v, vr), "v");
+      check_apart(q_rows, "query", keys, "key_cache");
+      check_apart(q_rows, "query", values, "value_cache");
+    }
+    check_apart(keys, "key_cache", values, "value_cache");
+  }
+  done("welm_rope_kv_append", result);
   if (q) written(*q);
   written(key_cache);
   written(value_cache);
@@ -547,12 +552,6 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
     out = at::empty(q.sizes(), q.options());
   }
   const Rows outr = rows_of(*out, "out");
-  if (!fill) {
-    const RowSet out_rows = row_set(*out, outr);
-    check_apart(out_rows, "out", row_set(q, qr), "query");
-    check_apart(out_rows, "out", page_set(key_cache, key_strides), "key_cache");
-    check_apart(out_rows, "out", page_set(value_cache, value_strides), "value_cache");
-  }
   Tensor lse;
   if (return_lse) lse = at::empty({qr.tokens, qr.heads}, q.options().dtype(at::kFloat));
   int32_t* const device_status = status_of(status, index);
@@ -567,14 +566,21 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
                           (reinterpret_cast<uintptr_t>(workspace->data_ptr()) & 31u) == 0,
                       "workspace must be contiguous, 32-byte aligned and hold ", need, " bytes");
     const c10::cuda::CUDAGuard guard(index);
-    done("welm_rope_attend",
-         welm_rope_attend(q.const_data_ptr(), out->data_ptr(), return_lse ? lse.data_ptr<float>() : nullptr,
-                          key_cache.const_data_ptr(), value_cache.const_data_ptr(), table.const_data_ptr<int32_t>(),
-                          lens.const_data_ptr<int64_t>(), starts ? starts->const_data_ptr<int64_t>() : nullptr,
-                          prefix_len > 0 ? prefix_table->const_data_ptr<int32_t>() : nullptr, prefix_len, qr.tokens,
-                          batch, qr.heads, k_heads, qr.token, qr.head, outr.token, outr.head, width, table.stride(0),
-                          blocks, block_size, key_strides.data(), value_strides.data(), float(scale), fill,
-                          workspace->data_ptr(), size, device_status, stream_of(index)));
+    const int result =
+        welm_rope_attend(q.const_data_ptr(), out->data_ptr(), return_lse ? lse.data_ptr<float>() : nullptr,
+                         key_cache.const_data_ptr(), value_cache.const_data_ptr(), table.const_data_ptr<int32_t>(),
+                         lens.const_data_ptr<int64_t>(), starts ? starts->const_data_ptr<int64_t>() : nullptr,
+                         prefix_len > 0 ? prefix_table->const_data_ptr<int32_t>() : nullptr, prefix_len, qr.tokens,
+                         batch, qr.heads, k_heads, qr.token, qr.head, outr.token, outr.head, width, table.stride(0),
+                         blocks, block_size, key_strides.data(), value_strides.data(), float(scale), fill,
+                         workspace->data_ptr(), size, device_status, stream_of(index));
+    if (result == WELM_ROPE_ERR_BAD_STRIDE) {
+      const RowSet out_rows = row_set(*out, outr);
+      check_apart(out_rows, "out", row_set(q, qr), "query");
+      check_apart(out_rows, "out", page_set(key_cache, key_strides), "key_cache");
+      check_apart(out_rows, "out", page_set(value_cache, value_strides), "value_cache");
+    }
+    done("welm_rope_attend", result);
   } else {  // no request
     if (fill) out->zero_();
     if (return_lse) lse.fill_(-std::numeric_limits<float>::infinity());
