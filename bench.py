@@ -259,7 +259,8 @@ def timed_steps(step, count: int, dist, device, stream) -> float:
 # Result checks of the GPU arm: after timing, each leg runs once more on
 # pristine inputs; rank 0 gathers every rank's rows (NCCL all_gather when N > 1)
 # and compares their SHA-256 with the digest of the reference's own outputs
-# for that configuration, recorded by tests/golden/gen_golden.py.
+# for that configuration, recorded by tests/golden/gen_golden.py (where this
+# host's inputs are the recorded ones; else with the oracle's).
 # ---------------------------------------------------------------------------
 GOLDEN_OUTPUTS = REPO / "tests" / "golden" / "golden_outputs.json"
 L2_BYTES = 126 * 1024 * 1024
@@ -277,11 +278,40 @@ def sha256_rows(t: torch.Tensor) -> str:
     return hashlib.sha256(t.numpy().tobytes()).hexdigest()
 
 
-def golden_outputs(case_name: str) -> dict | None:
+def golden_case(case_name: str) -> dict | None:
     try:
-        return json.loads(GOLDEN_OUTPUTS.read_text())["cases"][case_name]["outputs"]
+        return json.loads(GOLDEN_OUTPUTS.read_text())["cases"][case_name]
     except Exception:  # noqa: BLE001
         return None
+
+
+def golden_outputs(case_name: str) -> dict | None:
+    rec = golden_case(case_name)
+    return rec and rec["outputs"]
+
+
+def expected_outputs(case_name: str) -> tuple[dict, str] | None:
+    """Digests of the outputs of `case_name`, and whose outputs they are.
+
+    The recorded digests hold for the recorded inputs.  The cos/sin table is
+    computed on the host, whose math library may round some entries otherwise;
+    the outputs to expect are then the oracle's for this host's inputs."""
+    from testfiles_b200 import workloads
+
+    rec = golden_case(case_name)
+    if rec is None:
+        return None
+    inp = workloads.make_inputs(workloads.find_case(case_name), "cpu")
+    if sha256_rows(inp.cache) == rec["cache"] and all(
+            sha256_rows(getattr(inp, name)) == rec["inputs"][name] for name in ("query", "key", "positions")):
+        return rec["outputs"], (f"SHA-256 of the reference's own outputs for {case_name} "
+                                f"({GOLDEN_OUTPUTS.relative_to(REPO)}), per request")
+    from oracle import rope_oracle
+
+    q, k = rope_oracle.reference_outputs(inp.query, inp.key, inp.positions, inp.last_index, inp.cache)
+    return {"query": sha256_rows(q), "key": sha256_rows(k)}, (
+        f"SHA-256 of the oracle's outputs for {case_name}, per request (this host's cos/sin table or inputs are not "
+        f"those of {GOLDEN_OUTPUTS.relative_to(REPO)})")
 
 
 def gather_rows(dist, t: torch.Tensor, counts: list[int]) -> torch.Tensor | None:
@@ -300,9 +330,10 @@ def parity_record(dist, rank: int, q: torch.Tensor, k: torch.Tensor, q_counts: l
     k_all = gather_rows(dist, k, k_counts)
     if rank != 0:
         return None
-    want = golden_outputs(case_name)
-    if want is None:
+    found = expected_outputs(case_name)
+    if found is None:
         return {"bit_exact": None, "reason": f"no golden digest for {case_name}"}
+    want, whose = found
     ok = True
     for qc, kc in zip(q_all.chunk(copies), k_all.chunk(copies)):
         ok &= sha256_rows(qc) == want["query"] and sha256_rows(kc) == want["key"]
@@ -313,8 +344,7 @@ def parity_record(dist, rank: int, q: torch.Tensor, k: torch.Tensor, q_counts: l
         "max_abs_k": 0.0 if ok else None,
         "max_ulp": 0 if ok else None,
         "rows_checked": {"query": int(q_all.shape[0]), "key": int(k_all.shape[0])},
-        "compared_with": f"SHA-256 of the reference's own outputs for {case_name} "
-                         f"({GOLDEN_OUTPUTS.relative_to(REPO)}), per request",
+        "compared_with": whose,
         "gathered": "NCCL all_gather to rank 0" if dist is not None else "single rank",
     }
 
