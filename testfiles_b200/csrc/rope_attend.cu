@@ -675,6 +675,7 @@ __device__ __forceinline__ bool list_once(const AttendArgs& a, Control& ctl, uin
   if (ok && !again) emit(Piece{});
   if (again) return true;
   asm volatile("cp.async.wait_all;" ::: "memory");
+  if (lane == 0) a.gave_up[cta] = 0;  // now, so that the kernel's end does not wait for it
   if (cta != 0) return false;
   // for the join: every request's place on the line
   int before = 0;
@@ -1207,8 +1208,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = ctl.tmem;
   const uint32_t q_at = smem_u32(smem), k_at = smem_u32(ring), v_at = k_at + kStagesK * kStageBytes;
   if (warp < 3) pdl_enter();  // the others first look at hints
-  // stored here, so that the kernel's end does not wait for it
-  if (tid == 0) a.gave_up[blockIdx.x] = 0;
   if (warp == 0) {
     produce(a, ctl, &kmap, &vmap, k_at, v_at);
   } else if (warp == 1) {
@@ -1241,12 +1240,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 // may have many); with kGroups == 1 a CTA of two such groups joins 32 rows.
 // The first threads work out where the parts of the CTA's rows are, a row each.
 // ---------------------------------------------------------------------------
-// A row that this kernel writes; of no request; of a request; of one whose result is lost.
-enum RowIs { kWritten = 1, kUnused = 2, kAsked = 4, kLost = 8 };
-
 struct RowParts {
   int cta[2], count[2], in_tile[2];  // prefix and own item: first CTA, CTAs, row of the item
-  int is;                            // bits of the following; 0: past the last row
+  int live;                          // 1: this kernel writes the row
+  int unused;                        // 1: a row of no request
   int token, head;
 };
 
@@ -1293,9 +1290,9 @@ __device__ __forceinline__ RowParts find_parts(const AttendArgs& a, const LineNo
     units_before = a.units_before[b];
     q = raw.checked(a, false);
   }
-  r.is = token < used && token >= q.first && token < q.first + q.count ? kAsked : 0;
-  if (note.nothing || r.is == 0) {  // a row of no request
-    r.is |= a.fill ? kUnused | kWritten : kUnused;
+  if (note.nothing || token >= used || token < q.first || token >= q.first + q.count) {  // a row of no request
+    r.live = a.fill;
+    r.unused = 1;
     return r;
   }
   const int pre = note.pre;
@@ -1316,8 +1313,29 @@ __device__ __forceinline__ RowParts find_parts(const AttendArgs& a, const LineNo
   const int units = Request::units(q.tiles(a, rt), note.joint);
   place(1, pre + units_before + q.units_before(a, rt, note.joint) * a.k_heads + h * units,
         max(units - kItemCost, 0), packed % kRows);
-  if (pre > 0 || r.count[1] != 1) r.is |= kWritten;  // otherwise the first kernel wrote the row
+  r.live = pre > 0 || r.count[1] != 1;  // otherwise the first kernel wrote the row
   return r;
+}
+
+// Where a CTA of the first kernel gave up, the note and the partial results may be
+// whatever the workspace held before, and rows may not have been written: none of
+// it is read, and every row of a request becomes no number.  Apart from the join, so
+// that it costs that no registers.
+__device__ __noinline__ void no_numbers(const AttendArgs& a, int first_row, int rows) {
+  const int used = used_tokens(a);
+  for (int i = threadIdx.x; i < rows * 32; i += blockDim.x) {
+    const int flat = first_row + (i >> 5), lanes8 = i & 31;
+    if (flat >= a.tokens * a.q_heads) continue;
+    const int token = a.by_q_heads.of(flat), head = flat - token * a.q_heads;
+    RawRequest raw;
+    raw.load(a, request_from(a, token, 0, false));
+    const Request q = raw.checked(a, false);
+    const bool asked = token < used && token >= q.first && token < q.first + q.count;
+    if (a.lse != nullptr && lanes8 == 0) a.lse[flat] = __int_as_float(asked ? 0x7fc00000 : 0xff800000);
+    if (!asked && !a.fill) continue;
+    const uint32_t v = asked ? 0x7fc07fc0u : 0u;
+    *reinterpret_cast<uint4*>(a.out + token * a.out_token + head * a.out_head + lanes8 * 8) = make_uint4(v, v, v, v);
+  }
 }
 
 // Running join of partial results (m, l, eight lanes of O).
@@ -1366,21 +1384,14 @@ __global__ void __launch_bounds__(kGroups == 1 ? 256 : 128 * kGroups, kResident)
   int lost = 0;  // read by the last threads, as the first are busy
 #pragma unroll 1
   for (int c = blockDim.x - 1 - threadIdx.x; c < a.grid; c += blockDim.x) lost |= a.gave_up[c];
-  // Where a CTA of the first kernel gave up, the note and the partial results may be
-  // whatever the workspace held before, and rows may not have been written: none of
-  // it is read, and every row of a request becomes no number.
   if (__syncthreads_or(lost)) {
-    if (threadIdx.x < kRowsPerCta) {
-      RowParts& r = parts[threadIdx.x];
-      r.count[0] = r.count[1] = 0;
-      if (r.is & kAsked) r.is |= kWritten | kLost;
-    }
-    __syncthreads();
+    no_numbers(a, blockIdx.x * kRowsPerCta, kRowsPerCta);
+    return;
   }
   const int64_t all = int64_t(a.tokens) * a.q_heads;
   for (int row = (kGroups == 1 ? 4 * grp : 0) + (in_grp & 3); row < kRowsPerCta; row += 8) {
-    const RowParts& r = parts[row];
-    const int count = r.is & kWritten ? r.count[0] + r.count[1] : 0;
+    const RowParts r = parts[row];
+    const int count = r.live ? r.count[0] + r.count[1] : 0;
     const int h = a.by_group.of(r.head);
     // the row among the whole items' rows
     const int64_t packed = int64_t(h) * a.tokens * a.group + int64_t(r.token) * a.group + (r.head - h * a.group);
@@ -1430,12 +1441,11 @@ __global__ void __launch_bounds__(kGroups == 1 ? 256 : 128 * kGroups, kResident)
         sum.add(s_o[w][8][in_grp], s_o[w][9][in_grp], v);
       }
     }
-    if (r.is & kLost) sum.l = __int_as_float(0x7fc00000);
     const bool none = sum.l == 0.0f;
-    if ((r.is & (kWritten | kUnused)) && a.lse != nullptr && lanes8 == 0)
+    if ((r.live || r.unused) && a.lse != nullptr && lanes8 == 0)
       a.lse[int64_t(r.token) * a.q_heads + r.head] =
           none ? -INFINITY : (sum.m + log2f(sum.l)) * 0.6931471805599453f;
-    if (!(r.is & kWritten)) continue;
+    if (!r.live) continue;
     const float inv = none ? 0.0f : 1.0f / sum.l;
     uint4 packed_out = make_uint4(0, 0, 0, 0);
     if (!none)
