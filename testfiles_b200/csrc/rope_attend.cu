@@ -1549,9 +1549,10 @@ int launch_attend(const CUtensorMap& kmap, const CUtensorMap& vmap, const Attend
   if (rows <= 4 * a.grid) return launch(rope_attend_join_kernel<4, 4, 1>, unsigned((rows + 3) / 4), 512, 0, stream, a);
   if (rows <= 8 * a.grid) return launch(rope_attend_join_kernel<4, 3, 2>, unsigned((rows + 3) / 4), 512, 0, stream, a);
   // More rows keep the SMs busy with one group to a row.  Both kernels' us with two
-  // groups and with one: 4200 rows 57.8 and 63.8, 6000 33.2 and 37.0, 7200 36.3 and
-  // 38.0, 7800 38.8 and 38.9, 8200 40.6 and 40.0, 9000 42.7 and 40.8, 12000 53.5 and 47.5.
-  if (rows <= 52 * a.grid) return launch(rope_attend_join_kernel<2, 3, 1>, unsigned((rows + 3) / 4), 256, 0, stream, a);
+  // groups and with one: decode over a prefix, 4200 rows 57.0 and 61.2, 6000 79.3 and
+  // 81.2, 7200 94.8 and 96.4, 8400 110.3 and 107.5; a prompt's chunk, 4200 rows 28.2
+  // and 31.0, 6000 34.6 and 34.5, 7200 38.0 and 35.7, 9000 45.0 and 38.7.
+  if (rows <= 40 * a.grid) return launch(rope_attend_join_kernel<2, 3, 1>, unsigned((rows + 3) / 4), 256, 0, stream, a);
   return launch(rope_attend_join_kernel<1, 2, 1>, unsigned((rows + 31) / 32), 256, 0, stream, a);
 }
 

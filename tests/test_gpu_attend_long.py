@@ -161,7 +161,7 @@ def test_rows_that_do_not_rise_are_left_alone():
 
 @pytest.mark.parametrize("requests", [701, 1003, 1501])
 def test_many_rows_with_a_prefix_are_joined(requests):
-    """More than 4096 rows, or than 52 an SM, some in whole items and some in cut ones, of requests with own keys and without."""
+    """More than 4096 rows, or than 40 an SM, some in whole items and some in cut ones, of requests with own keys and without."""
     lens = [[0, 1, 64, 129, 300][b % 5] for b in range(requests)]
     batch = Batch(lens, prefix=4000)
     plan = plan_of(batch, (6, 1))
