@@ -54,8 +54,8 @@ constexpr int kQChunkBytes = kRows * 128;  // 64 lanes of 128 rows
 constexpr int kQBytes = kRows * kHeadDim * 2;
 // What an item costs beside its tiles (its Q rows, its results), in tiles.
 // Measured with 1, 2 and 3 on one B200 (graph replay, us): 128 requests over a
-// prefix 32.3, 30.5, 31.4; 256 requests over 32768 shared keys 79.3, 76.4, 79.8;
-// 24 requests' verification 20.7, 21.7, 21.6; 48 requests 24.7, 24.6, 25.1.
+// prefix 31.2, 29.6, 30.6; 48 requests 24.7, 24.6, 25.3; 24 requests' verification
+// 20.7, 22.0, 21.6; 256 requests over 32768 shared keys 84 to 89 with each.
 constexpr int kItemCost = 2;
 constexpr int kPieces = 4;             // ring of piece descriptors
 constexpr int kThreads = 384;
@@ -496,7 +496,9 @@ __device__ __forceinline__ bool still_so(const AttendArgs& a, int b, const RawRe
 // While the previous kernel may still run, a batch of a request a lane is added up
 // and the CTA's first piece found from lengths and starts as they are then.  After
 // the dependency wait every warp reads its requests again: if one has changed, all
-// is done again from what it says now.
+// is done again from what it says now.  128 requests over a prefix, in a row of
+// calls 30.4 -> 29.5 us; behind an append, which is too short to hide it, a layer's
+// step 41.6 -> 42.4.
 __device__ __forceinline__ bool hints(const AttendArgs& a) { return a.batch <= 32 * (1 + kSoftmaxWarps); }
 
 // Adds up the requests' units, finds where this CTA's run begins and lists the
@@ -1371,7 +1373,8 @@ __global__ void __launch_bounds__(kGroups == 1 ? 256 : 128 * kGroups, kResident)
   const int grp = threadIdx.x >> 7, in_grp = threadIdx.x & 127;
   const int lanes8 = in_grp >> 2;  // eight lanes of the head
   // The next kernel may already take the SMs that the first one has left: one
-  // request 10.3 -> 9.7 us in a row of calls, 24 requests' verification 21.8 -> 22.1.
+  // request 10.3 -> 9.7 us in a row of calls, 24 requests' verification 21.5 -> 22.0;
+  // between an append and a projection no difference.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int flat = min(int(blockIdx.x * kRowsPerCta + threadIdx.x), a.tokens * a.q_heads - 1);
   int request = find_request(a, a.by_q_heads.of(blockIdx.x * kRowsPerCta), s_request);
